@@ -367,6 +367,40 @@ int lego_hip_hbm_probe(const void* in, void* out, unsigned long long bytes, int 
  * an fp16 GEMM whose data movement costs nothing. */
 int lego_hip_mfma_probe(const void* operands, float* sink, int shape, int iters, int workgroups, void* stream);
 
+/* Attention operators.  Tensors are [batch][token][head][element] of 16-bit elements (element 0 fp16, 1 bfloat16) with whole 16-byte chunks: bases aligned to
+ * 16 bytes, strides (in elements, between batches, tokens and heads; 0 where a dimension has one entry or is shared) multiples of 8, a head of 8, 16, ... 128 elements
+ * that lie after one another; tokens at most 8388480 elements apart.  Sizes and strides are host arrays. */
+
+/* Room for lego_hip_attention_fwd (backward 0; none without documents) or lego_hip_attention_bwd. sizes: batch, queries, keys, query heads, key heads, head elements;
+ * query head h reads key head h / (query heads / key heads). */
+int lego_hip_attention_workspace_bytes(const long long* sizes, int documents, int backward, unsigned long long* bytes);
+
+/* out = softmax(s) v over the keys that a query sees, lse[batch][head][query] = log of the sum of exp(s) (fp32; -infinity and zeros in out for a query that sees none), with
+ * s = scale * q.k, then softcap * tanh(s / softcap) where softcap is positive, then less slopes[head] * |distance| where slopes (fp32) is given.
+ * Query i stands at position i + keys - queries.  It sees key j if
+ *   causal is 0, or j is no later, or j < prefix[batch] (int32, given with causal 1 only), and
+ *   documents (int32 [batch][keys], given for queries <= keys only) is null, or holds the same number, not negative, at both positions.
+ * Keys of a negative document are never read, whatever they hold.  strides: of q, k, v and out, three each.
+ * workspace (16-byte aligned): what lego_hip_attention_workspace_bytes says, null where that is 0. */
+int lego_hip_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const long long* sizes, const long long* strides, float scale,
+                           float softcap, const float* slopes, const int* documents, const int* prefix, int causal, int element, void* workspace,
+                           unsigned long long workspace_bytes, void* stream);
+
+/* Gradients of q, k and v from that of out; out and lse as the forward pass left them.  Queries that see no key give and get none.
+ * strides: of q, k, v, out, dout, dq, dk and dv, three each.  The result does not depend on the order in which workgroups run. */
+int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                           const long long* sizes, const long long* strides, float scale, float softcap, const float* slopes, const int* documents, const int* prefix,
+                           int causal, int element, void* workspace, unsigned long long workspace_bytes, void* stream);
+
+/* Rotary positions of queries and keys (k and k_out null: of q alone): pairs (a, b) of a head's first `part` elements become
+ * magnitude * (a cos t - b sin t, b cos t + a sin t), t = position * frequency in 64 bits; inverse 1: with -t, the gradient.  Pair i is elements (2 i, 2 i + 1) where
+ * interleaved is 1, else (i, i + part / 2).  The other elements are copied.
+ * sizes: batch, tokens, query heads, key heads (0 without k), head elements, part (even, 2 to 256, at most the head).
+ * strides (elements): of q, k, q_out and k_out, three each, then of positions two (batch, token).  positions: int32, or int64 where wide_positions is 1;
+ * frequencies: part / 2 doubles.  element: 0 fp16, 1 bfloat16, 2 fp32; any alignment of elements. */
+int lego_hip_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions, const double* frequencies, const long long* sizes,
+                    const long long* strides, int interleaved, float magnitude, int inverse, int element, int wide_positions, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,7 +14,7 @@ import sys
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
-from .kernels import gemm, layernorm_bwd, lud, nw, rowwise, stencil, transpose
+from .kernels import attention, gemm, layernorm_bwd, lud, nw, rotary, rowwise, stencil, transpose
 from .kernels.common import BANNER, CSRC, GENERATED
 from .lego_hip import HIPCC_FLAGS, hipcc_path
 
@@ -191,6 +191,10 @@ def collect():
     units.append(stu)
     luu, mlu = lud.emit()
     units.append(luu)
+    atu, mat = attention.emit()
+    units += atu
+    rou, mro = rotary.emit()
+    units.append(rou)
 
     h = [f"// {BANNER}", "#pragma once", "#include <hip/hip_runtime.h>", "",
          "hipError_t lego_transpose_any_launch(const void*, void*, int, int, int, hipStream_t);"]
@@ -306,6 +310,14 @@ def collect():
           f"#define LEGO_STENCIL_BRICK {mst['B']}", f"#define LEGO_STENCIL_MAX_RADIUS {mst['MAX_RADIUS']}",
           f"#define LEGO_STENCIL_STAR_MAX_RADIUS {mst['STAR_MAX_RADIUS']}", "",
           "hipError_t lego_lud_f32_launch(float*, int, hipStream_t);", "hipError_t lego_lud_f32_plan(int, int*, int, int*);", f"#define LEGO_LUD_BLOCK {mlu['B']}", ""]
+    h += ["struct AttentionArgs;", "struct RotaryArgs;"]
+    h += [f"hipError_t lego_attention_{way}_{d}_d{head}_launch(const AttentionArgs&, hipStream_t);"
+          for way in ("fwd", "bwd") for d in mat["ELEMENTS"] for head in mat["HEADS"]]
+    h += ["hipError_t lego_attention_tiles_launch(const int*, int2*, int, int, hipStream_t);",
+          "hipError_t lego_attention_delta_launch(const AttentionArgs&, int, hipStream_t);",
+          "hipError_t lego_attention_join_launch(const AttentionArgs&, int, hipStream_t);",
+          "hipError_t lego_rotary_launch(const RotaryArgs&, int, int, int, int, hipStream_t);",
+          f"#define LEGO_ATTENTION_MAX_HEAD {mat['MAX_HEAD']}", f"#define LEGO_ROTARY_MAX_PART {mro['MOST']}", ""]
     return units, "\n".join(h)
 
 
@@ -366,8 +378,10 @@ def _compile(src: Path, incremental: bool = False) -> Path:
     obj = OBJ_DIR / (src.stem + ".o")
     if incremental and obj.exists():
         # the generated text is only rewritten when it changes, so modification times tell
-        # (only the hand-written ABI file includes the two headers)
+        # (only the hand-written ABI files include the first two headers)
         deps = [src] + ([GENERATED / "launchers.h", ROOT / "include" / "lego_hip.h"] if src.parent == CSRC else [])
+        if "attention_args.h" in src.read_text():
+            deps.append(CSRC / "attention_args.h")
         newest = max(p.stat().st_mtime for p in deps)
         if obj.stat().st_mtime > newest:
             return obj
@@ -430,7 +444,7 @@ def _build_extension(src: Path, path: Path, incremental: bool) -> Path:
 def build(verbose=True, incremental=False):
     """Generate, compile every translation unit for gfx950 and link liblego_hip.so, then the two extension modules.  With
     ``incremental`` a translation unit whose object file is newer than its source is kept."""
-    sources = generate() + [CSRC / "lego_hip_abi.hip"]
+    sources = generate() + [CSRC / "lego_hip_abi.hip", CSRC / "lego_hip_attention.hip"]
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     with ThreadPoolExecutor(max_workers=8) as pool:
         objs = list(pool.map(lambda s: _compile(s, incremental), sources))

@@ -1,0 +1,43 @@
+// What the attention kernels' launchers take from the entry points.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+// rows of one tensor: elements between batches, tokens and heads
+struct Strides { long long batch, token, head; };
+
+// the score function's constants
+struct Scores {
+  float scale, scale_log2;      // of q.k; times log2 e
+  float cap_in, cap_log2;       // 2 scale log2(e) / cap; cap log2(e)
+};
+
+struct AttentionArgs {
+  const void *q, *k, *v, *out, *dout;
+  void *o, *dq, *dk, *dv;
+  float* lse;                   // [batch][head][query], natural logarithm
+  float* delta;                 // the same, of the backward pass: sum of out * dout
+  float* ups;                   // [batch][head][tile of 64 queries]: power of two that brings the tile's largest dout to 1..2
+  const float* slopes;          // [head], or null
+  const int* documents;         // [batch][key], or null
+  int2* tiles;                  // [batch][tile of 64 keys]: lowest and highest document
+  const int* prefix;            // [batch], or null
+  float* parts;                 // dk and dv of parts of the query heads that share a key head: [part][dk, dv][batch][key head][key][head element], or null
+  Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
+  Scores scores;
+  int batch, queries, keys, heads, key_heads, head;
+  int causal, capped;
+  int heads_per_part;           // query heads whose sums one workgroup forms
+};
+
+struct RotaryArgs {
+  const void *q, *k;
+  void *qo, *ko;
+  const void* positions;        // 32 or 64 bits
+  const double* frequencies;    // radians a position, [part / 2]
+  long long position_batch, position_token;      // elements between positions
+  Strides sq, sk, sqo, sko;
+  unsigned batch, tokens, heads, key_heads, head, part;
+  float magnitude;
+  int inverse;
+};

@@ -1,0 +1,566 @@
+// generated by lego_amd (python -m lego_amd.build) -- do not edit; edit the generator
+//
+// Attention, backward: dQ, dK and dV from dO, f16, up to 128 head elements.
+//   P = exp(score(Q K^T) - lse),  dS = P * (dO V^T - delta),  dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K
+// with delta and lse of the rows.  Two kernels, each of which owns what it writes, so that no sum is shared and none depends on an order of arrival: one
+// goes through the queries for 128 keys and sums dK and dV, four products a tile, the other through the keys for 128 queries and sums dQ, three.  A single
+// kernel would need five products and not seven, and would add dQ up through memory.
+// A lane holds one column of everything, a key in the first kernel and a query in the second; P and dS are the second operands of their products as they lie in the registers.
+// P and dS are rounded to the operands' type, which their products take; the sums are fp32.  P carries a factor of 2^8, and dS the power of two that
+// brings the largest dO of its tile (dQ: of its row) to 1..2, so that small gradients do not sink below fp16's smallest numbers.
+// Index expressions printed from LEGO layouts:
+//   LDS tile   OrderBy(GenP((64, 16), row*16 + (chunk ^ key(row)))).TileBy([64, 16])
+//   launch     OrderBy(Col(per_xcd, 8)).TileBy([per_xcd, 8])[Row(per_xcd, 8).inv(wg)]; pid = ((batch, head), block of queries, last first)
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "attention_args.h"
+
+namespace {
+
+typedef _Float16 elt_t;
+typedef elt_t elt2 __attribute__((ext_vector_type(2)));
+typedef elt_t elt8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr unsigned DC = 128;               // head elements that are computed; elements from the head's size on are zeros
+constexpr unsigned KS = DC / 16, DB = DC / 32;   // MFMA steps along the head, blocks of 32 head elements
+constexpr unsigned PITCH = 128;           // elements between the rows of a tile in LDS
+constexpr unsigned ROWS = 64;                   // rows of a tile in LDS
+constexpr unsigned TILE = ROWS * PITCH * 2;     // bytes
+constexpr unsigned WAVES = 4;
+constexpr unsigned COPIES = TILE / 1024 / WAVES; // memory->LDS instructions of a wave for a tile
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float16v mfma(elt8 a, elt8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ float16v zeros()
+{
+  float16v z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+  return z;
+}
+
+// Two fp32 values as a pair of the operands' type, rounded to nearest.
+__device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector(float2v{a, b}, elt2)); }
+
+// The sixteen values that a lane holds of a 32 x 32 accumulator block (column lane % 32; value r is row 8 (r / 4) + 4 (lane / 32) + r % 4)
+// as the second operand of two MFMA steps over the block's rows.  The steps sum over the rows in the order in which a lane holds them:
+// rows 16 s + 4 (lane / 32) + 0..3 and 16 s + 8 + 4 (lane / 32) + 0..3, and the first operand is read in that order (transposed()).
+struct Operands { elt8 step[2]; };
+__device__ __forceinline__ Operands as_operands(const float16v& x)
+{
+  Operands o;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    o.step[s] = __builtin_bit_cast(elt8, u32x4{pack(x[8 * s], x[8 * s + 1]), pack(x[8 * s + 2], x[8 * s + 3]), pack(x[8 * s + 4], x[8 * s + 5]), pack(x[8 * s + 6], x[8 * s + 7])});
+  return o;
+}
+
+// A tile in LDS: OrderBy(GenP((64, 16), row*16 + (chunk ^ key(row)))).TileBy([64, 16])
+// with chunks of 16 bytes; the key makes both kinds of reads, 16 bytes of 16 rows in a row and transposing ones of 64 bytes of four rows, free of bank
+// conflicts.  rows(): the first operand whose rows are the tile's (block of 32 rows, step of 16 head elements); transposed(): the first operand whose rows
+// are 32 head elements (block `db`) and whose sum goes over 16 of the tile's rows, in as_operands()'s order.
+struct Reader {
+  unsigned row_at, tr_at;       // bytes within a tile
+  __device__ __forceinline__ explicit Reader(unsigned lane)
+  {
+    const unsigned l32 = lane % 32, lhi = lane / 32, l16 = lane % 16, lgrp = lane / 16;
+    row_at = 16 * (16*l32 + ((lhi) ^ (4*(l32 % 4) + ((l32)/(4)) % 4)));
+    tr_at = 16 * (64*lhi + ((2*(lgrp % 2) + ((l16 % 4)/(2))) ^ (lhi + 4*((l16)/(4)))) + 16*((l16)/(4))) + 8 * (l16 % 2);
+    (void)lgrp;
+  }
+  __device__ __forceinline__ elt8 rows(const char* tile, unsigned block, unsigned ks) const
+  {
+    return *reinterpret_cast<const elt8*>(tile + (row_at ^ (32 * ks)) + block * (32 * PITCH * 2));
+  }
+  // rows 16 * step .. of the tile
+  __device__ __forceinline__ elt8 transposed(const char* tile, unsigned step, unsigned db) const
+  {
+    const char* const at = tile + step * (16 * PITCH * 2);
+    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + (tr_at ^ (64 * db))));
+    const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + (tr_at ^ (64 * db) ^ 32) + 8 * PITCH * 2));
+    return __builtin_bit_cast(elt8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// Fills a tile from rows of memory: lane l of copy `it` of wave w fetches the 16-byte chunk that belongs into slot 64 (WAVES it + w) + l.  Chunks past
+// the head's size, rows past the last one and rows that `skip` names lie outside the descriptor, for which zeros are written.  Inline assembly, as the compiler orders
+// every LDS read after all outstanding memory->LDS loads it knows of; a scalar write of M0 needs one wait state before the instruction that reads it.
+constexpr unsigned kOutside = 0x80000000u;
+struct Filler {
+  unsigned offset, step, row0, bytes;     // of this lane's first chunk; between copies; its row; a row's extent
+  __device__ __forceinline__ Filler(unsigned lane, unsigned wave, unsigned stride_bytes, unsigned head)
+  {
+    row0 = 4*wave + ((lane)/(16));
+    const unsigned chunk = ((lane % 16) ^ (wave + 4*((lane)/(16))));
+    step = (ROWS / COPIES) * stride_bytes;
+    bytes = 2 * head;
+    offset = 8 * chunk < head ? row0 * stride_bytes + 16 * chunk : kOutside;
+  }
+  // `rows` rows of the tile exist, at least one
+  template <class Skip>
+  __device__ __forceinline__ void operator()(const elt_t* base, size_t first, unsigned stride_bytes, unsigned rows, unsigned lds, const Skip& skip) const
+  {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base) + first * stride_bytes;
+    const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
+                        (unsigned)__builtin_amdgcn_readfirstlane((min(rows, ROWS) - 1) * stride_bytes + bytes), 0x00020000u};
+#pragma unroll
+    for (unsigned it = 0; it < COPIES; ++it) {
+      const unsigned row = row0 + it * (ROWS / COPIES);
+      unsigned off = offset + it * step;
+      if (row >= rows || skip(row)) off = kOutside;
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds + it * (WAVES * 1024)) : "memory", "m0");
+    }
+  }
+};
+__device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Score function, in units of log2 e: what the exponential takes.  CAP: cap * tanh(scale q.k / cap) as cap (1 - 2 / (e^(2x) + 1)); its derivative by
+// scale q.k is 1 - tanh^2.  BIAS: less slope * |distance|.
+template <bool CAP>
+__device__ __forceinline__ float score(float qk, const Scores& f)
+{
+  if (!CAP) return f.scale_log2 * qk;
+  const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
+  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+}
+
+// The same and the derivative of the score by scale * q.k.
+template <bool CAP>
+__device__ __forceinline__ float score(float qk, const Scores& f, float& slope)
+{
+  slope = 1.0f;
+  if (!CAP) return f.scale_log2 * qk;
+  const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
+  slope = 4.0f * r * (1.0f - r);
+  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+}
+
+// What of the keys the queries of a block see.  Query i stands at position i + shift; it sees keys below limit(i), of its own document.
+struct Seen {
+  int keys, shift, prefix;      // prefix: -1 where queries see all keys
+  __device__ __forceinline__ int limit(int i) const { return prefix < 0 ? keys : min(keys, max(max(i + shift + 1, prefix), 0)); }
+};
+
+// Documents of a tile of 64 positions: the lowest and highest number (negative: padding).  Tiles that share no document with the others need no look at all; where
+// both hold one and the same document, nothing has to be compared.
+__device__ __forceinline__ bool apart(int2 a, int2 b) { return a.y < 0 || b.y < 0 || a.y < b.x || b.y < a.x; }
+__device__ __forceinline__ bool same(int2 a, int2 b) { return a.x == a.y && b.x == b.y && a.x == b.x; }
+
+// The tiles that a workgroup goes through, in order: 64 at a time are looked at, a lane each.
+template <class Look>
+struct Walk {
+  const Look& look;             // (tile) -> bit 0: needed, bit 1: documents have to be compared
+  unsigned lane, base, end;
+  unsigned long long need = 0, compare = 0;
+  __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin_, unsigned end_) : look(look_), lane(lane_), base(begin_), end(end_) { fetch(); }
+  __device__ __forceinline__ void fetch()
+  {
+    const unsigned tile = base + lane;
+    const unsigned bits = tile < end ? look(tile) : 0u;
+    need = __builtin_amdgcn_ballot_w64((bits & 1u) != 0);
+    compare = __builtin_amdgcn_ballot_w64((bits & 2u) != 0);
+  }
+  // the next tile, with bit 31 where documents have to be compared, or ~0u
+  __device__ __forceinline__ unsigned next()
+  {
+    while (need == 0) {
+      if (base + 64 >= end) return ~0u;
+      base += 64;
+      fetch();
+    }
+    const unsigned at = (unsigned)__builtin_ctzll(need);
+    need &= need - 1;
+    return (base + at) | ((unsigned)(compare >> at) & 1u) << 31;
+  }
+};
+
+// a value and the other half of the wavefront's, joined
+typedef unsigned pair_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float across_max(float x)
+{
+  const pair_t p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+}
+__device__ __forceinline__ float across_sum(float x)
+{
+  const pair_t p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(p.x) + __uint_as_float(p.y);
+}
+
+// Stores the columns of a wave's transposed result, blocks of 32 head elements: lane l holds element 8 (r / 4) + 4 (l / 32) + r % 4 of column l % 32.  Neighbouring
+// groups of four change places between the halves, so that a lane stores 16 bytes at a time.
+template <unsigned BLOCKS>
+__device__ __forceinline__ void store_columns(const float16v (&acc)[BLOCKS], elt_t* row, unsigned lane, unsigned head, float factor)
+{
+  const unsigned lhi = lane / 32;
+#pragma unroll
+  for (unsigned db = 0; db < BLOCKS; ++db)
+#pragma unroll
+    for (unsigned g = 0; g < 2; ++g) {
+      u32x2 w[2];
+#pragma unroll
+      for (unsigned e = 0; e < 2; ++e) {
+        const unsigned lo = pack(factor * acc[db][8 * g + 2 * e], factor * acc[db][8 * g + 2 * e + 1]);
+        const unsigned hi = pack(factor * acc[db][8 * g + 4 + 2 * e], factor * acc[db][8 * g + 4 + 2 * e + 1]);
+        const pair_t both = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+        w[0][e] = both.x;
+        w[1][e] = both.y;
+      }
+      const unsigned d = 32 * db + 16 * g + 8 * lhi;
+      if (row && d < head) *reinterpret_cast<u32x4*>(row + d) = u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+    }
+}
+
+}  // namespace
+
+namespace {
+
+constexpr float kShift = 8.0f;        // P is held as 2^kShift P
+constexpr float kUnshift = 1.0f / (1 << 8);
+
+// 64 floats of a row-wise statistic into LDS, by one wavefront; rows past the last one read as zeros
+__device__ __forceinline__ void fill_rows(const float* base, unsigned rows, unsigned lane, unsigned lds)
+{
+  const uintptr_t at = reinterpret_cast<uintptr_t>(base);
+  const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
+                      (unsigned)__builtin_amdgcn_readfirstlane(4 * min(rows, ROWS)), 0x00020000u};
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(4 * lane), "s"(rsrc), "s"(lds) : "memory", "m0");
+}
+
+template <bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * WAVES, 1) lego_attention_dkv_f16_d128_kernel(AttentionArgs a, unsigned per_xcd)
+{
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 1024];      // Q and dO, twice; lse and delta, twice
+  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
+  const unsigned blocks = (a.keys + 32 * WAVES - 1) / (32 * WAVES), group = a.heads / a.key_heads, parts = group / a.heads_per_part;
+  const unsigned wg = blockIdx.x;
+  const unsigned pid = per_xcd*(wg % 8) + ((wg)/(8));
+  if (pid >= blocks * parts * a.key_heads * a.batch) return;
+  const unsigned block = pid % blocks, part = pid / blocks % parts, hk = pid / blocks / parts % a.key_heads, b = pid / blocks / parts / a.key_heads;
+  const int k0 = (int)(32 * WAVES * block), k_last = min(k0 + 32 * (int)WAVES, a.keys) - 1;
+  const int w0 = k0 + 32 * (int)wave, key = w0 + (int)l32;
+  const int shift = a.keys - a.queries, prefix = a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : a.keys;
+  // a query sees a key from this row on
+  const auto from = [&](int j) { return j < prefix ? INT32_MIN : j - shift; };
+  const int from_key = from(key), from_w0 = from(w0), from_w1 = from(min(w0 + 31, a.keys - 1));
+  const int* const documents = a.documents ? a.documents + (size_t)b * a.keys : nullptr;
+  const int2* const tiles = documents ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
+
+  elt8 kv[KS], vv[KS];
+  {
+    const elt_t* const krow = static_cast<const elt_t*>(a.k) + (size_t)b * a.sk.batch + (size_t)min(key, a.keys - 1) * a.sk.token + (size_t)hk * a.sk.head;
+    const elt_t* const vrow = static_cast<const elt_t*>(a.v) + (size_t)b * a.sv.batch + (size_t)min(key, a.keys - 1) * a.sv.token + (size_t)hk * a.sv.head;
+#pragma unroll
+    for (unsigned ks = 0; ks < KS; ++ks) {
+      const unsigned d = 16 * ks + 8 * lhi;
+      kv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(krow + d) : elt8{};
+      vv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(vrow + d) : elt8{};
+    }
+  }
+  const int own_document = documents ? documents[min(key, a.keys - 1)] : 0;
+  int2 own_tiles = {0, 0};
+  if (documents) {
+    own_tiles = tiles[k0 / 64];
+    for (int t = k0 / 64 + 1; t <= k_last / 64; ++t) own_tiles = {min(own_tiles.x, tiles[t].x), max(own_tiles.y, tiles[t].y)};
+  }
+
+  const unsigned q_stride = 2 * (unsigned)a.sq.token, do_stride = 2 * (unsigned)a.sdo.token;
+  const Filler fill_q(lane, wave, q_stride, a.head), fill_do(lane, wave, do_stride, a.head);
+  const Reader read(lane);
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  const unsigned lds_base = (unsigned)(uintptr_t)(lds_ptr)lds, lds_at = lds_base + wave * 1024;
+  const auto fill = [&](unsigned h, unsigned tile, unsigned buffer) {
+    const unsigned first = 64 * (tile & 0x7fffffffu), rows = a.queries - first;
+    const elt_t* const qb = static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch + (size_t)h * a.sq.head;
+    const elt_t* const dob = static_cast<const elt_t*>(a.dout) + (size_t)b * a.sdo.batch + (size_t)h * a.sdo.head;
+    const size_t row = ((size_t)b * a.heads + h) * a.queries + first;
+    const unsigned at = lds_at + buffer * (2 * TILE);
+    if (wave < 2) fill_rows((wave ? a.delta : a.lse) + row, rows, lane, lds_base + 4 * TILE + buffer * 512 + wave * 256);
+    if (tile >> 31) {      // rows that see no key are read as zeros, whatever they hold
+      const auto skip = [&](unsigned r) { return a.lse[row + min(r, rows - 1)] == -INFINITY; };
+      fill_q(qb, first, q_stride, rows, at, skip);
+      fill_do(dob, first, do_stride, rows, at + TILE, skip);
+    } else {
+      const auto skip = [](unsigned) { return false; };
+      fill_q(qb, first, q_stride, rows, at, skip);
+      fill_do(dob, first, do_stride, rows, at + TILE, skip);
+    }
+  };
+  const auto look = [&](unsigned tile) -> unsigned {
+    const int first = (int)(64 * tile);
+    const unsigned empty = first + shift < 0 && a.causal ? 2u : 0u;      // rows before the first key
+    if (!documents) return 1u | empty;
+    const int t0 = (first + shift) / 64, t1 = (min(first + 63, a.queries - 1) + shift) / 64;
+    const int2 t = t0 == t1 ? tiles[t0] : int2{min(tiles[t0].x, tiles[t1].x), max(tiles[t0].y, tiles[t1].y)};
+    return apart(t, own_tiles) ? 0u : same(t, own_tiles) ? 1u : 3u;
+  };
+
+  float16v dk[DB], dv[DB];
+#pragma unroll
+  for (unsigned db = 0; db < DB; ++db) dk[db] = dv[db] = zeros();
+  float up = 0.0f;                 // the power of two that dk carries (fp16)
+  const unsigned h0 = hk * group + part * a.heads_per_part, h1 = h0 + a.heads_per_part;
+  const unsigned begin = k0 < prefix ? 0u : (unsigned)max(k0 - shift, 0) / 64, end = (unsigned)(a.queries + 63) / 64;
+  typedef Walk<decltype(look)> Queries;
+  Queries walk(look, lane, begin, end);
+  unsigned h = h0;
+  const auto advance = [&](unsigned& head) {      // the next tile of the heads in turn
+    unsigned tile = walk.next();
+    while (tile == ~0u && head + 1 < h1) {
+      ++head;
+      walk.base = begin;
+      walk.fetch();
+      tile = walk.next();
+    }
+    return tile;
+  };
+  unsigned now = advance(h), buffer = 0;
+  if (now != ~0u) fill(h, now, 0);
+  while (now != ~0u) {
+    unsigned next_h = h;
+    const unsigned next = advance(next_h);
+    wait_for_copies();
+    __syncthreads();
+    if (next != ~0u) fill(next_h, next, buffer ^ 1);
+    const char* const qt = lds + buffer * (2 * TILE);
+    const char* const dot = qt + TILE;
+    const float* const lse_s = reinterpret_cast<const float*>(lds + 4 * TILE + buffer * 512);
+    const int first = (int)(64 * (now & 0x7fffffffu));
+    const bool compare = documents && now >> 31;
+    const float slope = BIAS ? kLog2e * a.slopes[h] : 0.0f;
+    const float tile_up = a.ups[((size_t)b * a.heads + h) * end + first / 64];
+    if (up == 0.0f) up = tile_up;
+    if (tile_up < up) {
+      const float down = tile_up / up;
+      up = tile_up;
+#pragma unroll
+      for (unsigned db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[db][r] *= down;
+    }
+    const float c = up * kUnshift;
+    if (first + 63 >= from_w0) {
+#pragma unroll
+      for (unsigned qb = 0; qb < 2; ++qb) {
+        float16v s = zeros(), dp = zeros();
+#pragma unroll
+        for (unsigned ks = 0; ks < KS; ++ks) {
+          s = mfma(read.rows(qt, qb, ks), kv[ks], s);
+          dp = mfma(read.rows(dot, qb, ks), vv[ks], dp);
+        }
+        // rows first + 32 qb + 8 (r / 4) + 4 lhi + r % 4
+        const int row0 = first + 32 * (int)qb + 4 * (int)lhi;
+        const bool edge = first + 32 * (int)qb < from_w1;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4v lse = *reinterpret_cast<const float4v*>(lse_s + 32 * qb + 8 * g + 4 * lhi);
+          const float4v delta = *reinterpret_cast<const float4v*>(lse_s + 64 + 32 * qb + 8 * g + 4 * lhi);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e, row = row0 + 8 * g + e;
+            float bend;
+            float x = score<CAP>(s[r], a.scores, bend);
+            if (BIAS) x -= slope * fabsf((float)(row + shift - key));
+            float p = __builtin_amdgcn_exp2f(x - (kLog2e * lse[e] - kShift));
+            float ds = p * (c * (dp[r] - delta[e]));
+            if (CAP) ds *= bend;
+            if (edge && row < from_key) p = ds = 0.0f;
+            if (compare && !(own_document >= 0 && row < a.queries && documents[min(row, a.queries - 1) + shift] == own_document)) p = ds = 0.0f;
+            s[r] = p;
+            dp[r] = ds;
+          }
+        }
+        const Operands p = as_operands(s), ds = as_operands(dp);
+#pragma unroll
+        for (unsigned st = 0; st < 2; ++st)
+#pragma unroll
+          for (unsigned db = 0; db < DB; ++db) {
+            dv[db] = mfma(read.transposed(dot, 2 * qb + st, db), p.step[st], dv[db]);
+            dk[db] = mfma(read.transposed(qt, 2 * qb + st, db), ds.step[st], dk[db]);
+          }
+      }
+    }
+    now = next;
+    h = next_h;
+    buffer ^= 1;
+  }
+  const float k_factor = up == 0.0f ? 0.0f : a.scores.scale / up, v_factor = kUnshift;
+  if (!a.parts) {
+    const bool mine = key < a.keys;
+    store_columns<DB>(dk, mine ? static_cast<elt_t*>(a.dk) + (size_t)b * a.sdk.batch + (size_t)key * a.sdk.token + (size_t)hk * a.sdk.head : nullptr, lane, a.head, k_factor);
+    store_columns<DB>(dv, mine ? static_cast<elt_t*>(a.dv) + (size_t)b * a.sdv.batch + (size_t)key * a.sdv.token + (size_t)hk * a.sdv.head : nullptr, lane, a.head, v_factor);
+    return;
+  }
+  if (key >= a.keys) return;
+  const size_t rows = (size_t)a.batch * a.key_heads * a.keys, row = ((size_t)b * a.key_heads + hk) * a.keys + key;
+  float* const dk_at = a.parts + ((size_t)(2 * part) * rows + row) * a.head;
+  float* const dv_at = dk_at + rows * a.head;
+#pragma unroll
+  for (unsigned db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const unsigned d = 32 * db + 8 * g + 4 * lhi;
+      if (d >= (unsigned)a.head) continue;
+      *reinterpret_cast<float4v*>(dk_at + d) = float4v{k_factor * dk[db][4 * g], k_factor * dk[db][4 * g + 1], k_factor * dk[db][4 * g + 2], k_factor * dk[db][4 * g + 3]};
+      *reinterpret_cast<float4v*>(dv_at + d) = float4v{v_factor * dv[db][4 * g], v_factor * dv[db][4 * g + 1], v_factor * dv[db][4 * g + 2], v_factor * dv[db][4 * g + 3]};
+    }
+}
+
+template <bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_f16_d128_kernel(AttentionArgs a, unsigned per_xcd)
+{
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];      // K and V, twice
+  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
+  const unsigned blocks = (a.queries + 32 * WAVES - 1) / (32 * WAVES);
+  const unsigned wg = blockIdx.x;
+  const unsigned pid = per_xcd*(wg % 8) + ((wg)/(8));
+  if (pid >= blocks * a.heads * a.batch) return;
+  const unsigned block = blocks - 1 - pid % blocks, h = pid / blocks % a.heads, b = pid / blocks / a.heads;
+  const unsigned hk = h / (a.heads / a.key_heads);
+  const int q0 = (int)(32 * WAVES * block), q_last = min(q0 + 32 * (int)WAVES, a.queries) - 1;
+  const int w0 = q0 + 32 * (int)wave, i = w0 + (int)l32;
+  const Seen seen{a.keys, a.keys - a.queries, a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : -1};
+  const int limit = seen.limit(i), limit_w0 = seen.limit(w0), limit_w1 = seen.limit(min(w0 + 31, q_last));
+  const int* const documents = a.documents ? a.documents + (size_t)b * a.keys : nullptr;
+  const int2* const tiles = documents ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
+  const size_t stat = ((size_t)b * a.heads + h) * a.queries + min(i, a.queries - 1);
+  const float lse = a.lse[stat], delta = a.delta[stat];
+
+  elt8 qv[KS], dov[KS];
+  {
+    const elt_t* const qrow = static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch + (size_t)min(i, a.queries - 1) * a.sq.token + (size_t)h * a.sq.head;
+    const elt_t* const dorow = static_cast<const elt_t*>(a.dout) + (size_t)b * a.sdo.batch + (size_t)min(i, a.queries - 1) * a.sdo.token + (size_t)h * a.sdo.head;
+#pragma unroll
+    for (unsigned ks = 0; ks < KS; ++ks) {
+      const unsigned d = 16 * ks + 8 * lhi;
+      qv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(qrow + d) : elt8{};
+      dov[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(dorow + d) : elt8{};
+    }
+  }
+  // the power of two that brings the row's largest dO to 1..2
+  float largest = 0.0f;
+#pragma unroll
+  for (unsigned ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf((float)dov[ks][e]));
+  largest = across_max(largest);
+  const float up = largest > 0.0f && largest < INFINITY ? __builtin_amdgcn_ldexpf(1.0f, 1 - __builtin_amdgcn_frexp_expf(largest)) : 1.0f;
+  const float c = up * kUnshift;
+  const int own_document = documents ? documents[min(i, a.queries - 1) + seen.shift] : 0;
+  int2 own_tiles = {0, 0};
+  if (documents) {
+    own_tiles = tiles[(q0 + seen.shift) / 64];
+    for (int t = (q0 + seen.shift) / 64 + 1; t <= (q_last + seen.shift) / 64; ++t) own_tiles = {min(own_tiles.x, tiles[t].x), max(own_tiles.y, tiles[t].y)};
+  }
+  const float slope = BIAS ? kLog2e * a.slopes[h] : 0.0f;
+
+  const elt_t* const kb = static_cast<const elt_t*>(a.k) + (size_t)b * a.sk.batch + (size_t)hk * a.sk.head;
+  const elt_t* const vb = static_cast<const elt_t*>(a.v) + (size_t)b * a.sv.batch + (size_t)hk * a.sv.head;
+  const unsigned k_stride = 2 * (unsigned)a.sk.token, v_stride = 2 * (unsigned)a.sv.token;
+  const Filler fill_k(lane, wave, k_stride, a.head), fill_v(lane, wave, v_stride, a.head);
+  const Reader read(lane);
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
+  const auto fill = [&](unsigned tile, unsigned buffer) {
+    const unsigned first = 64 * (tile & 0x7fffffffu), rows = a.keys - first;
+    const unsigned at = lds_at + buffer * (2 * TILE);
+    if (tile >> 31) {      // padding among the keys is read as zeros, whatever it holds
+      const auto skip = [&](unsigned row) { return documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
+      fill_k(kb, first, k_stride, rows, at, skip);
+      fill_v(vb, first, v_stride, rows, at + TILE, skip);
+    } else {
+      const auto skip = [](unsigned) { return false; };
+      fill_k(kb, first, k_stride, rows, at, skip);
+      fill_v(vb, first, v_stride, rows, at + TILE, skip);
+    }
+  };
+  const auto look = [&](unsigned tile) -> unsigned {
+    if (!documents) return 1u;
+    const int2 t = tiles[tile];
+    return apart(t, own_tiles) ? 0u : same(t, own_tiles) ? 1u : 3u;
+  };
+
+  float16v dq[DB];
+#pragma unroll
+  for (unsigned db = 0; db < DB; ++db) dq[db] = zeros();
+  Walk<decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
+  unsigned now = walk.next(), buffer = 0;
+  if (now != ~0u) fill(now, 0);
+  while (now != ~0u) {
+    const unsigned next = walk.next();
+    wait_for_copies();
+    __syncthreads();
+    if (next != ~0u) fill(next, buffer ^ 1);
+    const char* const kt = lds + buffer * (2 * TILE);
+    const char* const vt = kt + TILE;
+    const int first = (int)(64 * (now & 0x7fffffffu));
+    const bool compare = now >> 31;
+    if (first < limit_w1) {
+#pragma unroll
+      for (unsigned kb2 = 0; kb2 < 2; ++kb2) {
+        float16v s = zeros(), dp = zeros();
+#pragma unroll
+        for (unsigned ks = 0; ks < KS; ++ks) {
+          s = mfma(read.rows(kt, kb2, ks), qv[ks], s);
+          dp = mfma(read.rows(vt, kb2, ks), dov[ks], dp);
+        }
+        const int key0 = first + (int)(32 * kb2 + 4 * lhi);
+        const bool edge = first + 32 * (int)kb2 + 32 > limit_w0;
+        const float distance0 = (float)(i + seen.shift - key0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = key0 + 8 * (r / 4) + r % 4;
+          float bend;
+          float x = score<CAP>(s[r], a.scores, bend);
+          if (BIAS) x -= slope * fabsf(distance0 - (float)(8 * (r / 4) + r % 4));
+          const float p = __builtin_amdgcn_exp2f(x - (kLog2e * lse - kShift));
+          float ds = p * (c * (dp[r] - delta));
+          if (CAP) ds *= bend;
+          if (edge && key >= limit) ds = 0.0f;
+          if (compare && !(own_document >= 0 && documents[min(key, a.keys - 1)] == own_document)) ds = 0.0f;
+          dp[r] = ds;
+        }
+        const Operands ds = as_operands(dp);
+#pragma unroll
+        for (unsigned st = 0; st < 2; ++st)
+#pragma unroll
+          for (unsigned db = 0; db < DB; ++db) dq[db] = mfma(read.transposed(kt, 2 * kb2 + st, db), ds.step[st], dq[db]);
+      }
+    }
+    now = next;
+    buffer ^= 1;
+  }
+  elt_t* const row = i < a.queries ? static_cast<elt_t*>(a.dq) + (size_t)b * a.sdq.batch + (size_t)i * a.sdq.token + (size_t)h * a.sdq.head : nullptr;
+  store_columns<DB>(dq, row, lane, a.head, a.scores.scale / up);
+}
+
+}  // namespace
+
+hipError_t lego_attention_bwd_f16_d128_launch(const AttentionArgs& a, hipStream_t stream)
+{
+  const auto launch = [&](auto kernel, unsigned blocks) {
+    const unsigned per_xcd = (blocks + 8 - 1) / 8;
+    hipLaunchKernelGGL(kernel, dim3(per_xcd * 8), dim3(64 * WAVES), 0, stream, a, per_xcd);
+    return hipGetLastError();
+  };
+  const auto both = [&](auto dkv, auto dq) {
+    const unsigned keys = (unsigned)(a.keys + 32 * WAVES - 1) / (32 * WAVES), queries = (unsigned)(a.queries + 32 * WAVES - 1) / (32 * WAVES);
+    const hipError_t e = launch(dkv, keys * (unsigned)(a.heads / a.heads_per_part) * (unsigned)a.batch);
+    return e != hipSuccess ? e : launch(dq, queries * (unsigned)a.heads * (unsigned)a.batch);
+  };
+  if (a.capped && a.slopes) return both(lego_attention_dkv_f16_d128_kernel<true, true>, lego_attention_dq_f16_d128_kernel<true, true>);
+  if (a.capped) return both(lego_attention_dkv_f16_d128_kernel<true, false>, lego_attention_dq_f16_d128_kernel<true, false>);
+  if (a.slopes) return both(lego_attention_dkv_f16_d128_kernel<false, true>, lego_attention_dq_f16_d128_kernel<false, true>);
+  return both(lego_attention_dkv_f16_d128_kernel<false, false>, lego_attention_dq_f16_d128_kernel<false, false>);
+}

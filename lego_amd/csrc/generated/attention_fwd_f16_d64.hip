@@ -1,0 +1,395 @@
+// generated by lego_amd (python -m lego_amd.build) -- do not edit; edit the generator
+//
+// Attention, forward: O = softmax(score(Q K^T)) V over the keys that a query sees, f16, up to 64 head elements.
+// One pass over the keys with a running maximum and sum.  A workgroup of 4 wavefronts owns 128 queries of a head, a wavefront 32 of them, one to a
+// lane of each half: the scores are computed transposed, S^T = K Q^T, so that a query's scores lie in two lanes, its maximum and sum cost one exchange between
+// the halves, and its factors are a lane's own.  P^T is the second operand of O^T = V^T P^T as it lies in the registers.  Tiles of 64 keys go from memory into LDS
+// without passing registers, the next one while the present one is computed.
+// P is rounded to the operands' type for the product with V, as is everything that MFMAs of 16-bit operands take; its sum is of the unrounded values, in fp32.
+// Index expressions printed from LEGO layouts:
+//   LDS tile   OrderBy(GenP((64, 8), row*8 + (chunk ^ key(row)))).TileBy([64, 8])
+//   launch     OrderBy(Col(per_xcd, 8)).TileBy([per_xcd, 8])[Row(per_xcd, 8).inv(wg)]; pid = ((batch, head), block of queries, last first)
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "attention_args.h"
+
+namespace {
+
+typedef _Float16 elt_t;
+typedef elt_t elt2 __attribute__((ext_vector_type(2)));
+typedef elt_t elt8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr unsigned DC = 64;               // head elements that are computed; elements from the head's size on are zeros
+constexpr unsigned KS = DC / 16, DB = DC / 32;   // MFMA steps along the head, blocks of 32 head elements
+constexpr unsigned PITCH = 64;           // elements between the rows of a tile in LDS
+constexpr unsigned ROWS = 64;                   // rows of a tile in LDS
+constexpr unsigned TILE = ROWS * PITCH * 2;     // bytes
+constexpr unsigned WAVES = 4;
+constexpr unsigned COPIES = TILE / 1024 / WAVES; // memory->LDS instructions of a wave for a tile
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float16v mfma(elt8 a, elt8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ float16v zeros()
+{
+  float16v z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+  return z;
+}
+
+// Two fp32 values as a pair of the operands' type, rounded to nearest.
+__device__ __forceinline__ unsigned pack(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector(float2v{a, b}, elt2)); }
+
+// The sixteen values that a lane holds of a 32 x 32 accumulator block (column lane % 32; value r is row 8 (r / 4) + 4 (lane / 32) + r % 4)
+// as the second operand of two MFMA steps over the block's rows.  The steps sum over the rows in the order in which a lane holds them:
+// rows 16 s + 4 (lane / 32) + 0..3 and 16 s + 8 + 4 (lane / 32) + 0..3, and the first operand is read in that order (transposed()).
+struct Operands { elt8 step[2]; };
+__device__ __forceinline__ Operands as_operands(const float16v& x)
+{
+  Operands o;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    o.step[s] = __builtin_bit_cast(elt8, u32x4{pack(x[8 * s], x[8 * s + 1]), pack(x[8 * s + 2], x[8 * s + 3]), pack(x[8 * s + 4], x[8 * s + 5]), pack(x[8 * s + 6], x[8 * s + 7])});
+  return o;
+}
+
+// A tile in LDS: OrderBy(GenP((64, 8), row*8 + (chunk ^ key(row)))).TileBy([64, 8])
+// with chunks of 16 bytes; the key makes both kinds of reads, 16 bytes of 16 rows in a row and transposing ones of 64 bytes of four rows, free of bank
+// conflicts.  rows(): the first operand whose rows are the tile's (block of 32 rows, step of 16 head elements); transposed(): the first operand whose rows
+// are 32 head elements (block `db`) and whose sum goes over 16 of the tile's rows, in as_operands()'s order.
+struct Reader {
+  unsigned row_at, tr_at;       // bytes within a tile
+  __device__ __forceinline__ explicit Reader(unsigned lane)
+  {
+    const unsigned l32 = lane % 32, lhi = lane / 32, l16 = lane % 16, lgrp = lane / 16;
+    row_at = 16 * (8*l32 + ((lhi) ^ (((l32)/(4)) % 4 + 4*(((l32)/(2)) % 2))));
+    tr_at = 16 * (32*lhi + ((2*(lgrp % 2) + ((l16 % 4)/(2))) ^ (lhi + 4*((l16)/(8)))) + 8*((l16)/(4))) + 8 * (l16 % 2);
+    (void)lgrp;
+  }
+  __device__ __forceinline__ elt8 rows(const char* tile, unsigned block, unsigned ks) const
+  {
+    return *reinterpret_cast<const elt8*>(tile + (row_at ^ (32 * ks)) + block * (32 * PITCH * 2));
+  }
+  // rows 16 * step .. of the tile
+  __device__ __forceinline__ elt8 transposed(const char* tile, unsigned step, unsigned db) const
+  {
+    const char* const at = tile + step * (16 * PITCH * 2);
+    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + (tr_at ^ (64 * db))));
+    const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + (tr_at ^ (64 * db) ^ 32) + 8 * PITCH * 2));
+    return __builtin_bit_cast(elt8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// Fills a tile from rows of memory: lane l of copy `it` of wave w fetches the 16-byte chunk that belongs into slot 64 (WAVES it + w) + l.  Chunks past
+// the head's size, rows past the last one and rows that `skip` names lie outside the descriptor, for which zeros are written.  Inline assembly, as the compiler orders
+// every LDS read after all outstanding memory->LDS loads it knows of; a scalar write of M0 needs one wait state before the instruction that reads it.
+constexpr unsigned kOutside = 0x80000000u;
+struct Filler {
+  unsigned offset, step, row0, bytes;     // of this lane's first chunk; between copies; its row; a row's extent
+  __device__ __forceinline__ Filler(unsigned lane, unsigned wave, unsigned stride_bytes, unsigned head)
+  {
+    row0 = 8*wave + ((lane)/(8));
+    const unsigned chunk = ((lane % 8) ^ ((2*wave + ((lane)/(32))) % 4 + 4*(((lane)/(16)) % 2)));
+    step = (ROWS / COPIES) * stride_bytes;
+    bytes = 2 * head;
+    offset = 8 * chunk < head ? row0 * stride_bytes + 16 * chunk : kOutside;
+  }
+  // `rows` rows of the tile exist, at least one
+  template <class Skip>
+  __device__ __forceinline__ void operator()(const elt_t* base, size_t first, unsigned stride_bytes, unsigned rows, unsigned lds, const Skip& skip) const
+  {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base) + first * stride_bytes;
+    const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
+                        (unsigned)__builtin_amdgcn_readfirstlane((min(rows, ROWS) - 1) * stride_bytes + bytes), 0x00020000u};
+#pragma unroll
+    for (unsigned it = 0; it < COPIES; ++it) {
+      const unsigned row = row0 + it * (ROWS / COPIES);
+      unsigned off = offset + it * step;
+      if (row >= rows || skip(row)) off = kOutside;
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds + it * (WAVES * 1024)) : "memory", "m0");
+    }
+  }
+};
+__device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Score function, in units of log2 e: what the exponential takes.  CAP: cap * tanh(scale q.k / cap) as cap (1 - 2 / (e^(2x) + 1)); its derivative by
+// scale q.k is 1 - tanh^2.  BIAS: less slope * |distance|.
+template <bool CAP>
+__device__ __forceinline__ float score(float qk, const Scores& f)
+{
+  if (!CAP) return f.scale_log2 * qk;
+  const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
+  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+}
+
+// The same and the derivative of the score by scale * q.k.
+template <bool CAP>
+__device__ __forceinline__ float score(float qk, const Scores& f, float& slope)
+{
+  slope = 1.0f;
+  if (!CAP) return f.scale_log2 * qk;
+  const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
+  slope = 4.0f * r * (1.0f - r);
+  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+}
+
+// What of the keys the queries of a block see.  Query i stands at position i + shift; it sees keys below limit(i), of its own document.
+struct Seen {
+  int keys, shift, prefix;      // prefix: -1 where queries see all keys
+  __device__ __forceinline__ int limit(int i) const { return prefix < 0 ? keys : min(keys, max(max(i + shift + 1, prefix), 0)); }
+};
+
+// Documents of a tile of 64 positions: the lowest and highest number (negative: padding).  Tiles that share no document with the others need no look at all; where
+// both hold one and the same document, nothing has to be compared.
+__device__ __forceinline__ bool apart(int2 a, int2 b) { return a.y < 0 || b.y < 0 || a.y < b.x || b.y < a.x; }
+__device__ __forceinline__ bool same(int2 a, int2 b) { return a.x == a.y && b.x == b.y && a.x == b.x; }
+
+// The tiles that a workgroup goes through, in order: 64 at a time are looked at, a lane each.
+template <class Look>
+struct Walk {
+  const Look& look;             // (tile) -> bit 0: needed, bit 1: documents have to be compared
+  unsigned lane, base, end;
+  unsigned long long need = 0, compare = 0;
+  __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin_, unsigned end_) : look(look_), lane(lane_), base(begin_), end(end_) { fetch(); }
+  __device__ __forceinline__ void fetch()
+  {
+    const unsigned tile = base + lane;
+    const unsigned bits = tile < end ? look(tile) : 0u;
+    need = __builtin_amdgcn_ballot_w64((bits & 1u) != 0);
+    compare = __builtin_amdgcn_ballot_w64((bits & 2u) != 0);
+  }
+  // the next tile, with bit 31 where documents have to be compared, or ~0u
+  __device__ __forceinline__ unsigned next()
+  {
+    while (need == 0) {
+      if (base + 64 >= end) return ~0u;
+      base += 64;
+      fetch();
+    }
+    const unsigned at = (unsigned)__builtin_ctzll(need);
+    need &= need - 1;
+    return (base + at) | ((unsigned)(compare >> at) & 1u) << 31;
+  }
+};
+
+// a value and the other half of the wavefront's, joined
+typedef unsigned pair_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float across_max(float x)
+{
+  const pair_t p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+}
+__device__ __forceinline__ float across_sum(float x)
+{
+  const pair_t p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(p.x) + __uint_as_float(p.y);
+}
+
+// Stores the columns of a wave's transposed result, blocks of 32 head elements: lane l holds element 8 (r / 4) + 4 (l / 32) + r % 4 of column l % 32.  Neighbouring
+// groups of four change places between the halves, so that a lane stores 16 bytes at a time.
+template <unsigned BLOCKS>
+__device__ __forceinline__ void store_columns(const float16v (&acc)[BLOCKS], elt_t* row, unsigned lane, unsigned head, float factor)
+{
+  const unsigned lhi = lane / 32;
+#pragma unroll
+  for (unsigned db = 0; db < BLOCKS; ++db)
+#pragma unroll
+    for (unsigned g = 0; g < 2; ++g) {
+      u32x2 w[2];
+#pragma unroll
+      for (unsigned e = 0; e < 2; ++e) {
+        const unsigned lo = pack(factor * acc[db][8 * g + 2 * e], factor * acc[db][8 * g + 2 * e + 1]);
+        const unsigned hi = pack(factor * acc[db][8 * g + 4 + 2 * e], factor * acc[db][8 * g + 4 + 2 * e + 1]);
+        const pair_t both = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+        w[0][e] = both.x;
+        w[1][e] = both.y;
+      }
+      const unsigned d = 32 * db + 16 * g + 8 * lhi;
+      if (row && d < head) *reinterpret_cast<u32x4*>(row + d) = u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+    }
+}
+
+}  // namespace
+
+namespace {
+
+// A maximum rises by less than this (in units of log2) without the sums being scaled down: P stays below 2^8, which changes no relative rounding.
+constexpr float kLazy = 8.0f;
+
+template <bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kernel(AttentionArgs a, unsigned per_xcd)
+{
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];      // K and V, twice
+  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
+  const unsigned blocks = (a.queries + 32 * WAVES - 1) / (32 * WAVES);
+  const unsigned wg = blockIdx.x;
+  const unsigned pid = per_xcd*(wg % 8) + ((wg)/(8));
+  if (pid >= blocks * a.heads * a.batch) return;
+  const unsigned block = blocks - 1 - pid % blocks, h = pid / blocks % a.heads, b = pid / blocks / a.heads;
+  const unsigned hk = h / (a.heads / a.key_heads);
+  const int q0 = (int)(32 * WAVES * block), q_last = min(q0 + 32 * (int)WAVES, a.queries) - 1;
+  const int w0 = q0 + 32 * (int)wave;                      // the wavefront's first query
+  const int i = w0 + (int)l32;                              // the lane's query
+  const Seen seen{a.keys, a.keys - a.queries, a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : -1};
+  const int limit = seen.limit(i), limit_w0 = seen.limit(w0), limit_w1 = seen.limit(min(w0 + 31, q_last));
+  const int* const documents = a.documents ? a.documents + (size_t)b * a.keys : nullptr;
+  const int2* const tiles = documents ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
+
+  // a lane's query as the second operand; queries past the last one are computed as the last one is
+  elt8 qv[KS];
+  {
+    const elt_t* const row = static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch + (size_t)min(i, a.queries - 1) * a.sq.token + (size_t)h * a.sq.head;
+#pragma unroll
+    for (unsigned ks = 0; ks < KS; ++ks) {
+      const unsigned d = 16 * ks + 8 * lhi;
+      qv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(row + d) : elt8{};
+    }
+  }
+  const int own_document = documents ? documents[min(i, a.queries - 1) + seen.shift] : 0;
+  int2 own_tiles = {0, 0};
+  if (documents) {
+    own_tiles = tiles[(q0 + seen.shift) / 64];
+    for (int t = (q0 + seen.shift) / 64 + 1; t <= (q_last + seen.shift) / 64; ++t) own_tiles = {min(own_tiles.x, tiles[t].x), max(own_tiles.y, tiles[t].y)};
+  }
+  const float slope = BIAS ? kLog2e * a.slopes[h] : 0.0f;
+
+  const elt_t* const kb = static_cast<const elt_t*>(a.k) + (size_t)b * a.sk.batch + (size_t)hk * a.sk.head;
+  const elt_t* const vb = static_cast<const elt_t*>(a.v) + (size_t)b * a.sv.batch + (size_t)hk * a.sv.head;
+  const unsigned k_stride = 2 * (unsigned)a.sk.token, v_stride = 2 * (unsigned)a.sv.token;
+  const Filler fill_k(lane, wave, k_stride, a.head), fill_v(lane, wave, v_stride, a.head);
+  const Reader read(lane);
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
+  const auto fill = [&](unsigned tile, unsigned buffer) {
+    const unsigned first = 64 * (tile & 0x7fffffffu), rows = a.keys - first;
+    const unsigned at = lds_at + buffer * (2 * TILE);
+    if (tile >> 31) {      // padding among the keys is read as zeros, whatever it holds
+      const auto skip = [&](unsigned row) { return documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
+      fill_k(kb, first, k_stride, rows, at, skip);
+      fill_v(vb, first, v_stride, rows, at + TILE, skip);
+    } else {
+      const auto skip = [](unsigned) { return false; };
+      fill_k(kb, first, k_stride, rows, at, skip);
+      fill_v(vb, first, v_stride, rows, at + TILE, skip);
+    }
+  };
+  const auto look = [&](unsigned tile) -> unsigned {
+    if (!documents) return 1u;
+    const int2 t = tiles[tile];
+    return apart(t, own_tiles) ? 0u : same(t, own_tiles) ? 1u : 3u;
+  };
+
+  float16v acc[DB];
+#pragma unroll
+  for (unsigned db = 0; db < DB; ++db) acc[db] = zeros();
+  float most = -INFINITY, sum = 0.0f;      // of the lane's own keys; the halves agree on `most`
+  Walk<decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
+  unsigned now = walk.next(), buffer = 0;
+  if (now != ~0u) fill(now, 0);
+  while (now != ~0u) {
+    const unsigned next = walk.next();
+    wait_for_copies();
+    __syncthreads();                       // the tile is there, and the other buffer is read no more
+    if (next != ~0u) fill(next, buffer ^ 1);
+    const char* const kt = lds + buffer * (2 * TILE);
+    const char* const vt = kt + TILE;
+    const int first = (int)(64 * (now & 0x7fffffffu));
+    const bool compare = now >> 31;
+    if (first < limit_w1) {
+      float16v s[2] = {zeros(), zeros()};
+#pragma unroll
+      for (unsigned ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (unsigned kb2 = 0; kb2 < 2; ++kb2) s[kb2] = mfma(read.rows(kt, kb2, ks), qv[ks], s[kb2]);
+      // scores of keys first + 32 kb2 + 8 (r / 4) + 4 lhi + r % 4
+      const float distance0 = (float)(i + seen.shift - first - 4 * (int)lhi);
+#pragma unroll
+      for (unsigned kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float x = score<CAP>(s[kb2][r], a.scores);
+          if (BIAS) x -= slope * fabsf(distance0 - (float)(32 * kb2 + 8 * (r / 4) + r % 4));
+          s[kb2][r] = x;
+        }
+      if (first + 64 > limit_w0) {
+        const int end = limit - first - 4 * (int)lhi;
+#pragma unroll
+        for (unsigned kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb2][r] = (int)(32 * kb2 + 8 * (r / 4) + r % 4) < end ? s[kb2][r] : -INFINITY;
+      }
+      if (compare) {
+#pragma unroll
+        for (unsigned kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = first + (int)(32 * kb2 + 8 * (r / 4) + 4 * lhi + r % 4);
+            s[kb2][r] = own_document >= 0 && documents[min(key, a.keys - 1)] == own_document ? s[kb2][r] : -INFINITY;
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (unsigned kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb2][r]);
+      top = across_max(top);
+      if (__builtin_amdgcn_ballot_w64(top > most + kLazy) != 0) {
+        // (-inf - -inf where a query has seen nothing yet: its sums are zeros, whatever they are multiplied by but not by NaN)
+        const float risen = fmaxf(most, top), factor = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most - risen);
+        most = risen;
+        sum *= factor;
+#pragma unroll
+        for (unsigned db = 0; db < DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= factor;
+      }
+      const float base = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+      for (unsigned kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[kb2][r] = __builtin_amdgcn_exp2f(s[kb2][r] - base);
+          sum += s[kb2][r];
+        }
+#pragma unroll
+      for (unsigned kb2 = 0; kb2 < 2; ++kb2) {
+        const Operands p = as_operands(s[kb2]);
+#pragma unroll
+        for (unsigned st = 0; st < 2; ++st)
+#pragma unroll
+          for (unsigned db = 0; db < DB; ++db) acc[db] = mfma(read.transposed(vt, 2 * kb2 + st, db), p.step[st], acc[db]);
+      }
+    }
+    now = next;
+    buffer ^= 1;
+  }
+  sum = across_sum(sum);
+  elt_t* const row = i < a.queries ? static_cast<elt_t*>(a.o) + (size_t)b * a.so.batch + (size_t)i * a.so.token + (size_t)h * a.so.head : nullptr;
+  store_columns<DB>(acc, row, lane, a.head, sum == 0.0f ? 0.0f : 1.0f / sum);
+  if (i < a.queries && lhi == 0) a.lse[((size_t)b * a.heads + h) * a.queries + i] = sum == 0.0f ? -INFINITY : kLn2 * (most + __builtin_amdgcn_logf(sum));
+}
+
+}  // namespace
+
+hipError_t lego_attention_fwd_f16_d64_launch(const AttentionArgs& a, hipStream_t stream)
+{
+  const unsigned blocks = (unsigned)((a.queries + 32 * WAVES - 1) / (32 * WAVES)) * (unsigned)a.heads * (unsigned)a.batch;
+  const unsigned per_xcd = (blocks + 8 - 1) / 8;
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(per_xcd * 8), dim3(64 * WAVES), 0, stream, a, per_xcd);
+    return hipGetLastError();
+  };
+  if (a.capped) return a.slopes ? launch(lego_attention_fwd_f16_d64_kernel<true, true>) : launch(lego_attention_fwd_f16_d64_kernel<true, false>);
+  return a.slopes ? launch(lego_attention_fwd_f16_d64_kernel<false, true>) : launch(lego_attention_fwd_f16_d64_kernel<false, false>);
+}

@@ -1,0 +1,127 @@
+// generated by lego_amd (python -m lego_amd.build) -- do not edit; edit the generator
+//
+// The passes over rows beside the attention kernels: the lowest and highest document of every 64 positions; sum of out * dout of every query, with
+// the power of two that brings the largest dout of 64 queries to 1..2; and the sum of the parts of dk and dv.  Each reads its input once.
+// Index expressions printed from LEGO layouts:
+//   statistics   OrderBy(Row(batch, heads, queries)).TileBy([batch, heads, queries])[b, h, i]
+//   parts        OrderBy(Row(parts, 2, batch, key heads, keys, head))
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "attention_args.h"
+
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+// One wavefront a tile.
+__global__ void __launch_bounds__(256) lego_attention_tiles_kernel(const int* __restrict__ documents, int2* __restrict__ tiles, unsigned batch, unsigned keys)
+{
+  const unsigned per = (keys + 63) / 64, at = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
+  if (at >= batch * per) return;
+  const unsigned b = at / per, key = min(64 * (at % per) + lane, keys - 1);
+  int low = documents[(size_t)b * keys + key], high = low;
+#pragma unroll
+  for (int d = 32; d; d /= 2) {
+    low = min(low, __shfl_xor(low, d));
+    high = max(high, __shfl_xor(high, d));
+  }
+  if (lane == 0) tiles[at] = int2{low, high};
+}
+
+// 64 queries of a head a workgroup, 16 lanes a query.
+template <class E>
+__global__ void __launch_bounds__(256) lego_attention_delta_kernel(AttentionArgs a, unsigned tiles)
+{
+  typedef E elt8 __attribute__((ext_vector_type(8)));
+  __shared__ float largest_s[4];
+  const unsigned tile = blockIdx.x % tiles, h = blockIdx.x / tiles % a.heads, b = blockIdx.x / tiles / a.heads;
+  const unsigned lane = threadIdx.x % 16, team = threadIdx.x / 16;
+  const E* const out = static_cast<const E*>(a.out) + (size_t)b * a.so.batch + (size_t)h * a.so.head;
+  const E* const dout = static_cast<const E*>(a.dout) + (size_t)b * a.sdo.batch + (size_t)h * a.sdo.head;
+  float largest = 0.0f;
+#pragma unroll
+  for (unsigned it = 0; it < 4; ++it) {
+    const unsigned i = 64 * tile + 16 * it + team;
+    const bool inside = i < (unsigned)a.queries;
+    float sum = 0.0f;
+    const size_t stat = a.heads*a.queries*(size_t)b + a.queries*h + i;
+    const bool empty = !inside || a.lse[stat] == -INFINITY;      // a query that sees nothing gives no gradient, whatever its dout holds
+    if (!empty && 8 * lane < (unsigned)a.head) {
+      const elt8 x = *reinterpret_cast<const elt8*>(out + (size_t)i * a.so.token + 8 * lane), y = *reinterpret_cast<const elt8*>(dout + (size_t)i * a.sdo.token + 8 * lane);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sum += (float)x[e] * (float)y[e];
+        largest = fmaxf(largest, fabsf((float)y[e]));
+      }
+    }
+#pragma unroll
+    for (int d = 8; d; d /= 2) sum += __shfl_xor(sum, d);
+    if (lane == 0 && inside) a.delta[stat] = sum;
+  }
+#pragma unroll
+  for (int d = 32; d; d /= 2) largest = fmaxf(largest, __shfl_xor(largest, d));
+  if (threadIdx.x % 64 == 0) largest_s[threadIdx.x / 64] = largest;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    largest = fmaxf(fmaxf(largest_s[0], largest_s[1]), fmaxf(largest_s[2], largest_s[3]));
+    a.ups[((size_t)b * a.heads + h) * tiles + tile] = largest > 0.0f && largest < INFINITY ? ldexpf(1.0f, 1 - __builtin_amdgcn_frexp_expf(largest)) : 1.0f;
+  }
+}
+
+// Eight elements of dk or dv a lane, the parts summed in their order.
+template <class E>
+__global__ void __launch_bounds__(256) lego_attention_join_kernel(AttentionArgs a, unsigned parts)
+{
+  typedef E elt8 __attribute__((ext_vector_type(8)));
+  const size_t chunks = (size_t)a.batch * a.key_heads * a.keys * (a.head / 8), at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= 2 * chunks) return;
+  const unsigned which = at >= chunks;
+  const size_t chunk = at - which * chunks;
+  const unsigned per_row = a.head / 8, c = chunk % per_row;
+  const size_t row = chunk / per_row;
+  float4v lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+  for (unsigned part = 0; part < parts; ++part) {
+    const float* const from = a.parts + ((2 * part + which) * chunks + chunk) * 8;
+    lo += *reinterpret_cast<const float4v*>(from);
+    hi += *reinterpret_cast<const float4v*>(from + 4);
+  }
+  const unsigned key = row % a.keys, hk = row / a.keys % a.key_heads, b = row / a.keys / a.key_heads;
+  const Strides& s = which ? a.sdv : a.sdk;
+  elt8 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = static_cast<E>(lo[e]);
+    v[4 + e] = static_cast<E>(hi[e]);
+  }
+  *reinterpret_cast<elt8*>(static_cast<E*>(which ? a.dv : a.dk) + (size_t)b * s.batch + (size_t)key * s.token + (size_t)hk * s.head + 8 * c) = v;
+}
+
+}  // namespace
+
+hipError_t lego_attention_tiles_launch(const int* documents, int2* tiles, int batch, int keys, hipStream_t stream)
+{
+  const unsigned count = (unsigned)batch * (((unsigned)keys + 63) / 64);
+  hipLaunchKernelGGL(lego_attention_tiles_kernel, dim3((count + 3) / 4), dim3(256), 0, stream, documents, tiles, (unsigned)batch, (unsigned)keys);
+  return hipGetLastError();
+}
+
+hipError_t lego_attention_delta_launch(const AttentionArgs& a, int element, hipStream_t stream)
+{
+  const unsigned tiles = ((unsigned)a.queries + 63) / 64;
+  const dim3 grid(tiles * (unsigned)a.heads * (unsigned)a.batch);
+  if (element == 0) hipLaunchKernelGGL(lego_attention_delta_kernel<_Float16>, grid, dim3(256), 0, stream, a, tiles);
+  else hipLaunchKernelGGL(lego_attention_delta_kernel<__bf16>, grid, dim3(256), 0, stream, a, tiles);
+  return hipGetLastError();
+}
+
+hipError_t lego_attention_join_launch(const AttentionArgs& a, int element, hipStream_t stream)
+{
+  const unsigned parts = (unsigned)(a.heads / a.key_heads / a.heads_per_part);
+  const unsigned long long chunks = 2ull * a.batch * a.key_heads * a.keys * (a.head / 8);
+  const dim3 grid((unsigned)((chunks + 255) / 256));
+  if (element == 0) hipLaunchKernelGGL(lego_attention_join_kernel<_Float16>, grid, dim3(256), 0, stream, a, parts);
+  else hipLaunchKernelGGL(lego_attention_join_kernel<__bf16>, grid, dim3(256), 0, stream, a, parts);
+  return hipGetLastError();
+}

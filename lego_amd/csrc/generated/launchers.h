@@ -330,3 +330,24 @@ hipError_t lego_stencil_f32_plan(int, int, int, int, int*);
 hipError_t lego_lud_f32_launch(float*, int, hipStream_t);
 hipError_t lego_lud_f32_plan(int, int*, int, int*);
 #define LEGO_LUD_BLOCK 64
+
+struct AttentionArgs;
+struct RotaryArgs;
+hipError_t lego_attention_fwd_f16_d64_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_fwd_f16_d96_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_fwd_f16_d128_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_fwd_bf16_d64_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_fwd_bf16_d96_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_fwd_bf16_d128_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_bwd_f16_d64_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_bwd_f16_d96_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_bwd_f16_d128_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_bwd_bf16_d64_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_bwd_bf16_d96_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_bwd_bf16_d128_launch(const AttentionArgs&, hipStream_t);
+hipError_t lego_attention_tiles_launch(const int*, int2*, int, int, hipStream_t);
+hipError_t lego_attention_delta_launch(const AttentionArgs&, int, hipStream_t);
+hipError_t lego_attention_join_launch(const AttentionArgs&, int, hipStream_t);
+hipError_t lego_rotary_launch(const RotaryArgs&, int, int, int, int, hipStream_t);
+#define LEGO_ATTENTION_MAX_HEAD 128
+#define LEGO_ROTARY_MAX_PART 256

@@ -1,0 +1,193 @@
+// C-ABI entry points of the attention operators (declared in include/lego_hip.h).  Written by hand, as lego_hip_abi.hip is: an entry point checks what
+// the generated kernels assume and enqueues them on the caller's stream.  It allocates nothing and never synchronises.
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "attention_args.h"
+#include "generated/launchers.h"
+#include "lego_hip.h"
+
+namespace {
+
+constexpr int kInvalid = static_cast<int>(hipErrorInvalidValue);
+constexpr long long kMostTokens = 1ll << 28;
+// bytes between tokens: a tile of 64 lies within a descriptor's 2 GiB
+constexpr long long kMostPitch = (1ll << 31) / 2 / 64 - LEGO_ATTENTION_MAX_HEAD;
+
+inline bool aligned16(const void* p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+inline hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
+inline size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+// strides of one tensor: whole 16-byte chunks
+inline bool take(Strides& s, const long long* three)
+{
+  s = {three[0], three[1], three[2]};
+  for (int i = 0; i < 3; ++i)
+    if (three[i] < 0 || three[i] % 8) return false;
+  return s.token <= kMostPitch;
+}
+
+inline bool take_sizes(AttentionArgs& a, const long long* sizes)
+{
+  if (!sizes) return false;
+  for (int i = 0; i < 6; ++i)
+    if (sizes[i] < 1 || sizes[i] > kMostTokens) return false;
+  a.batch = (int)sizes[0], a.queries = (int)sizes[1], a.keys = (int)sizes[2], a.heads = (int)sizes[3], a.key_heads = (int)sizes[4], a.head = (int)sizes[5];
+  if (a.heads % a.key_heads || a.head % 8 || a.head > LEGO_ATTENTION_MAX_HEAD) return false;
+  // workgroups of a launch, the finest being 64 queries of a head
+  const unsigned __int128 tiles = ((unsigned __int128)(a.queries > a.keys ? a.queries : a.keys) + 63) / 64;
+  return tiles * a.heads * a.batch < (1u << 30) && (unsigned __int128)a.batch * a.key_heads * a.keys * a.head < ((unsigned __int128)1 << 38);
+}
+
+inline bool take_mask(AttentionArgs& a, float scale, float softcap, const float* slopes, const int* documents, const int* prefix, int causal)
+{
+  if (!(fabsf(scale) < INFINITY) || !(softcap >= 0.0f && softcap < INFINITY) || (causal != 0 && causal != 1)) return false;
+  if (!aligned4(slopes) || !aligned4(documents) || !aligned4(prefix) || (prefix && !causal) || (documents && a.keys < a.queries)) return false;
+  const float log2e = 1.4426950408889634f;
+  a.scores = {scale, scale * log2e, softcap > 0.0f ? 2.0f * scale * log2e / softcap : 0.0f, softcap * log2e};
+  a.capped = softcap > 0.0f;
+  a.slopes = slopes, a.documents = documents, a.prefix = prefix, a.causal = causal;
+  return true;
+}
+
+inline size_t tiles_bytes(const AttentionArgs& a) { return up16((size_t)a.batch * ((a.keys + 63) / 64) * sizeof(int2)); }
+
+// Query heads of a group whose dk and dv one workgroup sums.  All of them where that leaves enough workgroups; else fewer, whose sums go through memory.
+inline int heads_per_part(const AttentionArgs& a)
+{
+  const int group = a.heads / a.key_heads;
+  const long long blocks = (long long)((a.keys + 127) / 128) * a.key_heads * a.batch;
+  for (int parts = 1; parts <= group; ++parts)
+    if (group % parts == 0 && blocks * parts >= 1024) return group / parts;
+  return 1;
+}
+
+struct Room { size_t tiles, delta, ups, parts, all; };
+inline Room room_of(const AttentionArgs& a, bool documents, bool backward)
+{
+  Room r = {0, 0, 0, 0, 0};
+  r.delta = documents ? tiles_bytes(a) : 0;
+  r.ups = r.delta;
+  r.parts = r.ups;
+  r.all = r.parts;
+  if (!backward) return r;
+  const size_t rows = (size_t)a.batch * a.heads;
+  r.ups = r.delta + up16(rows * a.queries * sizeof(float));
+  r.parts = r.ups + up16(rows * ((a.queries + 63) / 64) * sizeof(float));
+  const int per = heads_per_part(a), parts = a.heads / a.key_heads / per;
+  r.all = r.parts + (parts > 1 ? (size_t)parts * 2 * a.batch * a.key_heads * a.keys * a.head * sizeof(float) : 0);
+  return r;
+}
+
+inline hipError_t forward(const AttentionArgs& a, int element, hipStream_t stream)
+{
+  const int which = a.head <= 64 ? 0 : a.head <= 96 ? 1 : 2;
+  static hipError_t (*const launch[2][3])(const AttentionArgs&, hipStream_t) = {
+    {lego_attention_fwd_f16_d64_launch, lego_attention_fwd_f16_d96_launch, lego_attention_fwd_f16_d128_launch},
+    {lego_attention_fwd_bf16_d64_launch, lego_attention_fwd_bf16_d96_launch, lego_attention_fwd_bf16_d128_launch}};
+  return launch[element][which](a, stream);
+}
+
+inline hipError_t backward(const AttentionArgs& a, int element, hipStream_t stream)
+{
+  const int which = a.head <= 64 ? 0 : a.head <= 96 ? 1 : 2;
+  static hipError_t (*const launch[2][3])(const AttentionArgs&, hipStream_t) = {
+    {lego_attention_bwd_f16_d64_launch, lego_attention_bwd_f16_d96_launch, lego_attention_bwd_f16_d128_launch},
+    {lego_attention_bwd_bf16_d64_launch, lego_attention_bwd_bf16_d96_launch, lego_attention_bwd_bf16_d128_launch}};
+  return launch[element][which](a, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int lego_hip_attention_workspace_bytes(const long long* sizes, int documents, int backward, unsigned long long* bytes)
+{
+  AttentionArgs a = {};
+  if (!bytes || !take_sizes(a, sizes)) return kInvalid;
+  *bytes = room_of(a, documents != 0, backward != 0).all;
+  return 0;
+}
+
+int lego_hip_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const long long* sizes, const long long* strides, float scale,
+                           float softcap, const float* slopes, const int* documents, const int* prefix, int causal, int element, void* workspace,
+                           unsigned long long workspace_bytes, void* stream)
+{
+  AttentionArgs a = {};
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !lse || !aligned4(lse) || !strides || element < 0 || element > 1) return kInvalid;
+  if (!take_sizes(a, sizes) || !take(a.sq, strides) || !take(a.sk, strides + 3) || !take(a.sv, strides + 6) || !take(a.so, strides + 9)) return kInvalid;
+  if (!take_mask(a, scale, softcap, slopes, documents, prefix, causal)) return kInvalid;
+  if (documents && (!aligned16(workspace) || workspace_bytes < room_of(a, true, false).all)) return kInvalid;
+  a.q = q, a.k = k, a.v = v, a.o = out, a.lse = lse;
+  if (documents) {
+    a.tiles = static_cast<int2*>(workspace);
+    const hipError_t e = lego_attention_tiles_launch(documents, a.tiles, a.batch, a.keys, as_stream(stream));
+    if (e != hipSuccess) return (int)e;
+  }
+  return (int)forward(a, element, as_stream(stream));
+}
+
+int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                           const long long* sizes, const long long* strides, float scale, float softcap, const float* slopes, const int* documents, const int* prefix,
+                           int causal, int element, void* workspace, unsigned long long workspace_bytes, void* stream)
+{
+  AttentionArgs a = {};
+  for (const void* p : {dout, q, k, v, out, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (!aligned16(p)) return kInvalid;
+  if (!lse || !aligned4(lse) || !strides || element < 0 || element > 1 || !take_sizes(a, sizes)) return kInvalid;
+  Strides* const into[8] = {&a.sq, &a.sk, &a.sv, &a.so, &a.sdo, &a.sdq, &a.sdk, &a.sdv};
+  for (int t = 0; t < 8; ++t)
+    if (!take(*into[t], strides + 3 * t)) return kInvalid;
+  if (!take_mask(a, scale, softcap, slopes, documents, prefix, causal)) return kInvalid;
+  const Room room = room_of(a, documents != nullptr, true);
+  if (!aligned16(workspace) || workspace_bytes < room.all) return kInvalid;
+  char* const at = static_cast<char*>(workspace);
+  a.q = q, a.k = k, a.v = v, a.out = out, a.dout = dout, a.lse = const_cast<float*>(lse), a.dq = dq, a.dk = dk, a.dv = dv;
+  a.tiles = reinterpret_cast<int2*>(at), a.delta = reinterpret_cast<float*>(at + room.delta), a.ups = reinterpret_cast<float*>(at + room.ups);
+  a.parts = room.all > room.parts ? reinterpret_cast<float*>(at + room.parts) : nullptr;
+  a.heads_per_part = heads_per_part(a);
+  hipError_t e = documents ? lego_attention_tiles_launch(documents, a.tiles, a.batch, a.keys, as_stream(stream)) : hipSuccess;
+  if (e == hipSuccess) e = lego_attention_delta_launch(a, element, as_stream(stream));
+  if (e == hipSuccess) e = backward(a, element, as_stream(stream));
+  if (e == hipSuccess && a.parts) e = lego_attention_join_launch(a, element, as_stream(stream));
+  return (int)e;
+}
+
+int lego_hip_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions, const double* frequencies, const long long* sizes,
+                    const long long* strides, int interleaved, float magnitude, int inverse, int element, int wide_positions, void* stream)
+{
+  if (!q || !q_out || !positions || !frequencies || !sizes || !strides || element < 0 || element > 2 || (interleaved | inverse | wide_positions) & ~1) return kInvalid;
+  const long long key_heads = sizes[3], head = sizes[4], part = sizes[5];
+  if (key_heads < 0 || (key_heads > 0) != (k != nullptr) || (k != nullptr) != (k_out != nullptr)) return kInvalid;
+  for (int i : {0, 1, 2, 4, 5})
+    if (sizes[i] < 1) return kInvalid;
+  for (int i = 0; i < 5; ++i)
+    if (sizes[i] > kMostTokens) return kInvalid;
+  if (part % 2 || part > head || part > LEGO_ROTARY_MAX_PART) return kInvalid;
+  for (int i = 0; i < 14; ++i)
+    if (strides[i] < 0) return kInvalid;
+  // tokens are workgroups; a token's elements are counted in 32 bits
+  if ((unsigned __int128)sizes[0] * sizes[1] > (1u << 30) || (unsigned __int128)(sizes[2] + key_heads) * head > (1u << 30)) return kInvalid;
+  const unsigned bytes = element == 2 ? 4 : 2, n = 16 / bytes;
+  const auto at = [](const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1u)) == 0; };
+  bool vectors = head % n == 0 && (interleaved ? part : part / 2) % n == 0;
+  for (const void* p : {q, k, (const void*)q_out, (const void*)k_out}) {
+    if (!at(p, bytes)) return kInvalid;
+    vectors = vectors && at(p, 16);
+  }
+  if (!at(positions, wide_positions ? 8 : 4) || !at(frequencies, 8)) return kInvalid;
+  for (int i = 0; i < 12; ++i) vectors = vectors && (strides[i] % n == 0 || (!k && (i / 3) % 2));
+  RotaryArgs a = {};
+  a.q = q, a.k = k, a.qo = q_out, a.ko = k_out, a.positions = positions, a.frequencies = frequencies;
+  Strides* const into[4] = {&a.sq, &a.sk, &a.sqo, &a.sko};
+  for (int t = 0; t < 4; ++t) *into[t] = {strides[3 * t], strides[3 * t + 1], strides[3 * t + 2]};
+  a.position_batch = strides[12], a.position_token = strides[13];
+  a.batch = (unsigned)sizes[0], a.tokens = (unsigned)sizes[1], a.heads = (unsigned)sizes[2], a.key_heads = (unsigned)key_heads, a.head = (unsigned)head, a.part = (unsigned)part;
+  a.magnitude = magnitude, a.inverse = inverse;
+  return (int)lego_rotary_launch(a, interleaved, vectors, wide_positions, element, as_stream(stream));
+}
+
+}  // extern "C"

@@ -7,13 +7,18 @@
 ``transpose(x)``                     the generated transpose programs have no callable
                                      (mlir_generated/transpose/transpose_smem_4096.mlir:2)
 
+and, beside them, what stands between the projections of a transformer block: ``rotary``, ``attention`` and
+``tree_attention``, which the reference has no counterpart of.
+
 As in the reference, inputs are borrowed, outputs are allocated here with ``torch.empty``
 and the kernel is enqueued on the current stream without synchronisation.  Tensors are
 only carriers of device pointers: every call goes through the C ABI of liblego_hip.so.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 import warnings
 
 import torch
@@ -451,3 +456,275 @@ def lud(m: torch.Tensor) -> torch.Tensor:
         raise ValueError("m must be square")
     runtime.call("lego_hip_lud_f32", _ptr(m), m.shape[0], _stream())
     return m
+
+
+# Attention.  Tensors are [batch, token, head, element]; a query head reads key head h // (query heads / key heads).
+
+_ATTENTION_ELEMENT = {torch.float16: 0, torch.bfloat16: 1}
+MAX_HEAD = 128      # head elements that the attention kernels take, in whole eights
+_MOST_PITCH = (1 << 24) - 256      # elements between tokens: a tile of 64 within 2 GiB
+
+
+def _on(t):
+    """The device of ``t`` as the current one: streams and launches are the current device's."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _strides(t):
+    """Elements between batches, tokens and heads; 0 where there is one of them."""
+    return [st if n > 1 else 0 for st, n in zip(t.stride(), t.shape[:3])]
+
+
+def _in_chunks(t):
+    """``t`` as the attention kernels read it: whole 16-byte chunks.  Slices of a fused projection are; other layouts are copied."""
+    if (t.shape[3] == 1 or t.stride(3) == 1) and t.data_ptr() % 16 == 0:
+        st = _strides(t)
+        if not (st[0] % 8 or st[1] % 8 or st[2] % 8) and st[1] <= _MOST_PITCH:
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_qkv(q, k, v):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.is_cuda:
+            raise ValueError(f"{name} must live on the GPU")
+        if t.dtype not in _ATTENTION_ELEMENT:
+            raise ValueError(f"{name} must be float16 or bfloat16, got {t.dtype}")
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [batch, token, head, element]")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("q, k and v must have the same dtype and device")
+    if k.shape != v.shape:
+        raise ValueError("k and v must have the same shape")
+    if k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError("q and k must have the same batch and head size")
+    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError("the query heads must be a multiple of the key heads")
+    if q.shape[3] % 8 or not 8 <= q.shape[3] <= MAX_HEAD:
+        raise ValueError(f"heads of 8, 16, ... {MAX_HEAD} elements, got {q.shape[3]}")
+
+
+def _vector(t, name, dtype, shape, device):
+    """A small tensor beside the operands, contiguous, or None."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {dtype} of shape {list(shape)} on {device}")
+    if t.requires_grad:
+        raise ValueError(f"{name} has no gradient here")
+    return t.contiguous()
+
+
+def _check_mask(q, k, causal, scale, softcap, slopes, documents, prefix):
+    """``(slopes, documents, prefix, scale, softcap)`` as the entry points take them."""
+    scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
+    softcap = float(softcap or 0.0)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if not (0.0 <= softcap < math.inf):
+        raise ValueError("softcap must be positive, or 0 for none")
+    if prefix is not None and not causal:
+        raise ValueError("a prefix goes with a causal mask")
+    if documents is not None and q.shape[1] > k.shape[1]:
+        raise ValueError("documents are the keys', which the queries are the last of")
+    return (_vector(slopes, "slopes", torch.float32, (q.shape[2],), q.device),
+            _vector(documents, "documents", torch.int32, (k.shape[0], k.shape[1]), q.device),
+            _vector(prefix, "prefix", torch.int32, (q.shape[0],), q.device), scale, softcap)
+
+
+def _longs(values):
+    return (ctypes.c_longlong * len(values))(*values)
+
+
+def _optional(t):
+    return None if t is None else t.data_ptr()
+
+
+def _attention_room(sizes, documents, backward, device):
+    size = ctypes.c_ulonglong(0)
+    runtime.call("lego_hip_attention_workspace_bytes", sizes, documents, backward, ctypes.byref(size))
+    return (torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None), size.value
+
+
+def attention_fwd(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None):
+    """Attention without its gradient; returns ``(out, lse)``, with the fp32 logarithm of every query's sum of exponentials,
+    ``[batch, head, query]`` (-inf for a query that sees no key).  Arguments as ``attention`` has them."""
+    _check_qkv(q, k, v)
+    slopes, documents, prefix, scale, softcap = _check_mask(q, k, causal, scale, softcap, slopes, documents, prefix)
+    batch, queries, heads, head = q.shape
+    out = torch.empty((batch, queries, heads, head), dtype=q.dtype, device=q.device)
+    lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=q.device)
+    if out.numel() == 0:
+        return out, lse
+    if k.shape[1] == 0:
+        return out.zero_(), lse.fill_(-math.inf)
+    with _on(q):
+        q, k, v = _in_chunks(q), _in_chunks(k), _in_chunks(v)
+        sizes = _longs((batch, queries, k.shape[1], heads, k.shape[2], head))
+        workspace, room = _attention_room(sizes, 1, 0, q.device) if documents is not None else (None, 0)
+        runtime.call("lego_hip_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), sizes,
+                     _longs(_strides(q) + _strides(k) + _strides(v) + _strides(out)), scale, softcap, _optional(slopes), _optional(documents),
+                     _optional(prefix), 1 if causal else 0, _ATTENTION_ELEMENT[q.dtype], _optional(workspace), room, _stream())
+    return out, lse
+
+
+def attention_bwd(dout, q, k, v, out, lse, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None):
+    """The gradients ``(dq, dk, dv)`` from that of ``out``, with ``out`` and ``lse`` of ``attention_fwd`` and its arguments.  Sums are in
+    fp32 and in a fixed order: the same inputs give the same bits."""
+    _check_qkv(q, k, v)
+    slopes, documents, prefix, scale, softcap = _check_mask(q, k, causal, scale, softcap, slopes, documents, prefix)
+    batch, queries, heads, head = q.shape
+    for name, t in (("dout", dout), ("out", out)):
+        if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{name} must have the shape, dtype and device of q")
+    if tuple(lse.shape) != (batch, heads, queries) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        raise ValueError("lse must be attention_fwd's")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    if q.numel() == 0 or k.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    with _on(q):
+        dout, q, k, v, out = (_in_chunks(t) for t in (dout, q, k, v, out))
+        sizes = _longs((batch, queries, k.shape[1], heads, k.shape[2], head))
+        workspace, room = _attention_room(sizes, documents is not None, 1, q.device)
+        strides = [st for t in (q, k, v, out, dout, dq, dk, dv) for st in _strides(t)]
+        runtime.call("lego_hip_attention_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), sizes,
+                     _longs(strides), scale, softcap, _optional(slopes), _optional(documents), _optional(prefix), 1 if causal else 0,
+                     _ATTENTION_ELEMENT[q.dtype], _optional(workspace), room, _stream())
+    return dq, dk, dv
+
+
+class LEGOAttention(torch.autograd.Function):
+    """The node of ``attention``."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, causal, scale, softcap, slopes, documents, prefix):
+        out, lse = attention_fwd(q, k, v, causal, scale, softcap, slopes, documents, prefix)
+        ctx.save_for_backward(q, k, v, out, lse, slopes, documents, prefix)
+        ctx.how = (causal, scale, softcap)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, slopes, documents, prefix = ctx.saved_tensors
+        return attention_bwd(dout, q, k, v, out, lse, *ctx.how, slopes, documents, prefix) + (None,) * 6
+
+
+def attention(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None):
+    """``softmax(s) v`` with gradients of q, k and v; fp16 or bf16, fp32 softmax and sums.
+
+    q is ``[batch, queries, heads, element]``, k and v ``[batch, keys, key heads, element]`` (the heads a multiple of the key heads, each
+    shared by its group; a head of 8, 16, ... 128 elements); slices of a fused projection are read where they lie.
+    ``s = scale * q.k`` (default ``1/sqrt(element)``), then ``softcap * tanh(s / softcap)``, then less ``slopes[head] * |distance|`` (fp32, no gradient).
+    Query i stands at position ``i + keys - queries``.  It sees the keys that are no later where ``causal``, and the first
+    ``prefix[batch]`` (int32) whatever their place; of those the ones of its own document, ``documents`` (int32 ``[batch, keys]``; a negative
+    number is padding, which sees and is seen by nothing, whatever it holds).  A query that sees nothing gives zeros, and takes and gives no gradient.
+    A NaN or infinity in a key or value reaches the queries that see it, and may reach others within 64 positions of those.
+
+    Inside a captured graph call ``attention_fwd`` and ``attention_bwd``: autograd's own bookkeeping of leaves is not made for it."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return LEGOAttention.apply(q, k, v, causal, scale, softcap, slopes, documents, prefix)
+    return attention_fwd(q, k, v, causal, scale, softcap, slopes, documents, prefix)[0]
+
+
+_ROTARY_ELEMENT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+MAX_ROTARY_PART = 256
+
+
+def rotary_frequencies(part, base=10000.0, stretch=1.0, original=None, slow=1.0, fast=32.0, device="cuda"):
+    """What ``rotary`` multiplies positions with: ``base ** (-2 i / part)`` radians a position for the ``part / 2`` pairs of a head, in float64.
+
+    For contexts ``stretch`` times as long as the ``original`` positions that a model was trained on: frequencies that make fewer than ``slow`` turns over the
+    original length are divided by ``stretch``, those of more than ``fast`` turns are kept, and between the two the division comes in
+    linearly with the turns.  Without ``original`` all are divided."""
+    if part < 2 or part % 2 or part > MAX_ROTARY_PART:
+        raise ValueError(f"part must be even, from 2 to {MAX_ROTARY_PART}")
+    if not (base > 0 and stretch > 0):
+        raise ValueError("base and stretch must be positive")
+    radians = float(base) ** (-torch.arange(0, part, 2, dtype=torch.float64) / part)
+    if stretch != 1.0:
+        keep = torch.zeros_like(radians)
+        if original is not None:
+            if not fast > slow:
+                raise ValueError("fast must be above slow")
+            keep = ((original * radians / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        radians = radians * (keep + (1.0 - keep) / stretch)
+    return radians.to(device)
+
+
+def _rotary(q, k, positions, frequencies, interleaved, magnitude, inverse):
+    """Checked tensors through the kernel; ``k`` may be None."""
+    batch, tokens, heads, head = q.shape
+    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    key_heads = 0 if k is None else k.shape[2]
+    if key_heads == 0 or outs[1].numel() == 0:
+        if q.numel() == 0:
+            return outs
+        k, key_heads = None, 0
+    elif q.numel() == 0:      # the keys alone, in the queries' place
+        outs[1] = _rotary(k, None, positions, frequencies, interleaved, magnitude, inverse)[0]
+        return outs
+    with _on(q):
+        ts = [t if t is None or head == 1 or t.stride(3) == 1 else t.contiguous() for t in (q, k)]
+        strides = []
+        for t in (ts[0], ts[1], outs[0], outs[1] if k is not None else None):
+            strides += [0, 0, 0] if t is None else _strides(t)
+        strides += [st if n > 1 else 0 for st, n in zip(positions.stride(), positions.shape)]
+        runtime.call("lego_hip_rotary", _ptr(ts[0]), None if k is None else _ptr(ts[1]), _ptr(outs[0]), None if k is None else _ptr(outs[1]), _ptr(positions),
+                     _ptr(frequencies), _longs((batch, tokens, heads, key_heads, head, 2 * frequencies.shape[0])), _longs(strides), 1 if interleaved else 0,
+                     magnitude, inverse, _ROTARY_ELEMENT[q.dtype], 1 if positions.dtype == torch.int64 else 0, _stream())
+    return outs
+
+
+class LEGORotary(torch.autograd.Function):
+    """The node of ``rotary``: its gradient is the turn back."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, interleaved, magnitude):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = (interleaved, magnitude)
+        ctx.set_materialize_grads(False)
+        return tuple(_rotary(q, k, positions, frequencies, interleaved, magnitude, 0))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        positions, frequencies = ctx.saved_tensors
+        if dq is None or dk is None:
+            one = dk if dq is None else dq
+            got = None if one is None else _rotary(one, None, positions, frequencies, *ctx.how, 1)[0]
+            return (None, got, None, None, None, None) if dq is None else (got, None, None, None, None, None)
+        return (*_rotary(dq, dk, positions, frequencies, *ctx.how, 1), None, None, None, None)
+
+
+def rotary(q, k, positions, frequencies, interleaved=False, magnitude=1.0):
+    """Queries and keys turned by their positions, ``(q', k')``, with gradients; ``k`` may be None.  fp16, bf16 or fp32, any head size and strides.
+
+    q and k are ``[batch, token, head, element]``, positions (int32 or int64) ``[batch, token]`` or ``[token]``.  The first ``part = 2 * len(frequencies)`` elements
+    of a head are turned: pair i by ``positions * frequencies[i]`` radians (float64, as ``rotary_frequencies`` makes them) and times ``magnitude``; pair i is elements
+    ``(i, i + part/2)``, or ``(2i, 2i + 1)`` where ``interleaved``.  The others stay."""
+    for name, t in (("q", q), ("k", k)):
+        if t is None and name == "k":
+            continue
+        if not t.is_cuda or t.dtype not in _ROTARY_ELEMENT or t.dim() != 4:
+            raise ValueError(f"{name} must be a [batch, token, head, element] GPU tensor of float16, bfloat16 or float32")
+        if t.dtype != q.dtype or t.device != q.device or t.shape[:2] != q.shape[:2] or t.shape[3] != q.shape[3]:
+            raise ValueError("q and k must have the same batch, tokens, head size, dtype and device")
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or frequencies.device != q.device or frequencies.requires_grad:
+        raise ValueError("frequencies must be a float64 vector on the device of q, without gradient")
+    if not 1 <= frequencies.shape[0] <= min(q.shape[3], MAX_ROTARY_PART) // 2:
+        raise ValueError(f"frequencies must be those of at most {MAX_ROTARY_PART} elements of a head")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+        raise ValueError("positions must be int32 or int64 on the device of q")
+    if tuple(positions.shape) not in ((q.shape[1],), tuple(q.shape[:2])):
+        raise ValueError("positions must be [token] or [batch, token]")
+    if not math.isfinite(magnitude):
+        raise ValueError("magnitude must be finite")
+    if positions.dim() == 1:
+        positions = positions.expand(q.shape[0], -1)
+    frequencies, magnitude = frequencies.contiguous(), float(magnitude)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return LEGORotary.apply(q, k, positions, frequencies, interleaved, magnitude)
+    return tuple(_rotary(q, k, positions, frequencies, interleaved, magnitude, 0))

@@ -16,6 +16,7 @@ CALLS_PATH = LIB_PATH.with_name("host_calls.so")
 _c_int, _c_void_p, _c_float = ctypes.c_int, ctypes.c_void_p, ctypes.c_float
 _PTR_ARRAY = ctypes.POINTER(ctypes.c_void_p)
 _INT_ARRAY = ctypes.POINTER(ctypes.c_int)
+_LONG_ARRAY = ctypes.POINTER(ctypes.c_longlong)
 
 # name -> argument types, exactly the prototypes of include/lego_hip.h
 SIGNATURES = {
@@ -90,6 +91,12 @@ SIGNATURES = {
     "lego_hip_mfma_probe": [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p],
     "lego_hip_grouped_gemm_f16_stamps": [_PTR_ARRAY, _PTR_ARRAY, _PTR_ARRAY, _INT_ARRAY, _c_int, _c_void_p],
     "lego_hip_gemm_stamps_read": [_c_void_p, _c_int],
+    "lego_hip_attention_workspace_bytes": [_LONG_ARRAY, _c_int, _c_int, ctypes.POINTER(ctypes.c_ulonglong)],
+    "lego_hip_attention_fwd": [_c_void_p] * 5 + [_LONG_ARRAY, _LONG_ARRAY, _c_float, _c_float, _c_void_p, _c_void_p, _c_void_p,
+                               _c_int, _c_int, _c_void_p, ctypes.c_ulonglong, _c_void_p],
+    "lego_hip_attention_bwd": [_c_void_p] * 9 + [_LONG_ARRAY, _LONG_ARRAY, _c_float, _c_float, _c_void_p, _c_void_p, _c_void_p,
+                               _c_int, _c_int, _c_void_p, ctypes.c_ulonglong, _c_void_p],
+    "lego_hip_rotary": [_c_void_p] * 6 + [_LONG_ARRAY, _LONG_ARRAY, _c_int, _c_float, _c_int, _c_int, _c_int, _c_void_p],
 }
 
 _lib = None
