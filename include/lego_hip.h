@@ -401,6 +401,19 @@ int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const
 int lego_hip_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions, const double* frequencies, const long long* sizes,
                     const long long* strides, int interleaved, float magnitude, int inverse, int element, int wide_positions, void* stream);
 
+/* Attention of drafted tokens over a paged cache: out[b][t][h] = softmax(s) v over the lengths[b] cached keys of sequence b and over those of its drafts j with
+ * tree[b][t][j] (one byte each; null: j <= t); k and v null: over the cache alone.  s as in lego_hip_attention_fwd, the distance of slopes being that of positions: a cached key's
+ * is its number, a draft's positions[b][j] (int32 [batch][drafts]; null: lengths[b] + j).  Cached key i of sequence b is row i % page of page pages[b][i / page] of the caches
+ * ([page][row][key head][element]; int32 [batch][width]).  A page number that is none of the cache's, and what of a length is past the table, stands for no key; a row that sees no key
+ * gives zeros.
+ * sizes: batch, drafts, query heads, key heads, head elements, rows of a page, pages of the cache, width of the table.
+ * strides (elements): of q, k, v (batch, token, head), k_cache, v_cache (page, row, head), out, three each, then of tree the one between batches.  Each of k, v and the caches spans
+ * less than 64 GiB.  workspace (16-byte aligned): what the first function says, null where that is 0. */
+int lego_hip_tree_attention_workspace_bytes(const long long* sizes, unsigned long long* bytes);
+int lego_hip_tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out, const int* pages, const int* lengths,
+                            const unsigned char* tree, const float* slopes, const int* positions, const long long* sizes, const long long* strides, float scale,
+                            float softcap, int element, void* workspace, unsigned long long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -310,7 +310,9 @@ def collect():
           f"#define LEGO_STENCIL_BRICK {mst['B']}", f"#define LEGO_STENCIL_MAX_RADIUS {mst['MAX_RADIUS']}",
           f"#define LEGO_STENCIL_STAR_MAX_RADIUS {mst['STAR_MAX_RADIUS']}", "",
           "hipError_t lego_lud_f32_launch(float*, int, hipStream_t);", "hipError_t lego_lud_f32_plan(int, int*, int, int*);", f"#define LEGO_LUD_BLOCK {mlu['B']}", ""]
-    h += ["struct AttentionArgs;", "struct RotaryArgs;"]
+    h += ["struct AttentionArgs;", "struct RotaryArgs;", "struct TreeArgs;"]
+    h += [f"hipError_t lego_tree_{d}_d{head}_launch(const TreeArgs&, int, hipStream_t);" for d in mat["ELEMENTS"] for head in mat["HEADS"]]
+    h += [f"#define LEGO_TREE_LEAST {mat['TREE_LEAST']}"]
     h += [f"hipError_t lego_attention_{way}_{d}_d{head}_launch(const AttentionArgs&, hipStream_t);"
           for way in ("fwd", "bwd") for d in mat["ELEMENTS"] for head in mat["HEADS"]]
     h += ["hipError_t lego_attention_tiles_launch(const int*, int2*, int, int, hipStream_t);",

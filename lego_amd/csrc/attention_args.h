@@ -41,3 +41,38 @@ struct RotaryArgs {
   float magnitude;
   int inverse;
 };
+
+// Attention of drafted tokens over a paged cache.
+struct TreeArgs {
+  const void *q, *k, *v;        // the drafts; k and v may be null
+  const void *k_cache, *v_cache;
+  void* o;
+  const int* pages;             // [batch][width]
+  const int* lengths;           // [batch]
+  const unsigned char* tree;    // [batch][draft][draft], or null: a draft sees itself and the earlier ones
+  const float* slopes;          // [head], or null
+  const int* positions;         // [batch][draft], or null: length + draft
+  float* sums;                  // of parts of rows: [slot][row][head element]
+  float2* stats;                // [slot][row]: maximum (log2) and sum
+  Strides sq, sk, sv, so, skc, svc;      // of the caches: between pages, slots of a page and heads
+  long long tree_batch;
+  Scores scores;
+  int batch, drafts, heads, key_heads, head, page, count, width;
+  int capped, whole;            // whole: a workgroup goes through all keys of its rows
+  unsigned row_blocks;          // of a key head's rows, drafts * (heads / key_heads)
+  unsigned workgroups;
+};
+
+// Where a cached key lies: the page that holds it, or -1 where the sequence is shorter or its table names no page of the cache.
+static inline
+#ifdef __HIPCC__
+__host__ __device__
+#endif
+int page_of(const int* pages, unsigned width, unsigned page, unsigned count, unsigned length, unsigned key)
+{
+  if (key >= length) return -1;
+  const unsigned at = key / page;
+  if (at >= width) return -1;
+  const int p = pages[at];
+  return p >= 0 && (unsigned)p < count ? p : -1;
+}

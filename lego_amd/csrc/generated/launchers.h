@@ -333,6 +333,14 @@ hipError_t lego_lud_f32_plan(int, int*, int, int*);
 
 struct AttentionArgs;
 struct RotaryArgs;
+struct TreeArgs;
+hipError_t lego_tree_f16_d64_launch(const TreeArgs&, int, hipStream_t);
+hipError_t lego_tree_f16_d96_launch(const TreeArgs&, int, hipStream_t);
+hipError_t lego_tree_f16_d128_launch(const TreeArgs&, int, hipStream_t);
+hipError_t lego_tree_bf16_d64_launch(const TreeArgs&, int, hipStream_t);
+hipError_t lego_tree_bf16_d96_launch(const TreeArgs&, int, hipStream_t);
+hipError_t lego_tree_bf16_d128_launch(const TreeArgs&, int, hipStream_t);
+#define LEGO_TREE_LEAST 2
 hipError_t lego_attention_fwd_f16_d64_launch(const AttentionArgs&, hipStream_t);
 hipError_t lego_attention_fwd_f16_d96_launch(const AttentionArgs&, hipStream_t);
 hipError_t lego_attention_fwd_f16_d128_launch(const AttentionArgs&, hipStream_t);

@@ -100,9 +100,86 @@ inline hipError_t backward(const AttentionArgs& a, int element, hipStream_t stre
   return launch[element][which](a, stream);
 }
 
+// Launch of attention over a cache: wavefronts of 32 rows that share a tile, and what a launch in runs needs.
+struct TreePlan { int row_waves; size_t stats, all; };
+inline bool plan_of(TreeArgs& a, const long long* sizes, TreePlan& plan)
+{
+  if (!sizes) return false;
+  for (int i = 0; i < 8; ++i)
+    if (sizes[i] < 1 || sizes[i] > kMostTokens) return false;
+  a.batch = (int)sizes[0], a.drafts = (int)sizes[1], a.heads = (int)sizes[2], a.key_heads = (int)sizes[3], a.head = (int)sizes[4];
+  a.page = (int)sizes[5], a.count = (int)sizes[6], a.width = (int)sizes[7];
+  if (a.heads % a.key_heads || a.head % 8 || a.head > LEGO_ATTENTION_MAX_HEAD) return false;
+  const unsigned __int128 keys = (unsigned __int128)a.page * a.width + a.drafts, all_rows = (unsigned __int128)a.batch * a.heads * a.drafts;
+  if (keys > (unsigned)kMostTokens || all_rows > (1u << 30)) return false;
+  const unsigned rows = (unsigned)a.drafts * (unsigned)(a.heads / a.key_heads);
+  plan.row_waves = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  const unsigned block = 32 * plan.row_waves;
+  a.row_blocks = (rows + block - 1) / block;
+  const unsigned long long items = (unsigned long long)a.batch * a.key_heads * a.row_blocks;
+  const unsigned long long most = ((unsigned long long)a.page * a.width + 63) / 64 + ((unsigned)a.drafts + 63) / 64;
+  if (items * most >= (1ull << 31)) return false;
+  // An item of few tiles is one workgroup's; else the tiles are dealt in equal runs to as many workgroups as the chip holds at a time, but no run is shorter than LEGO_TREE_LEAST.
+  a.whole = most <= 2 * LEGO_TREE_LEAST;
+  const unsigned long long held = a.head <= 64 ? 1024 : 512, runs = (items * most + LEGO_TREE_LEAST - 1) / LEGO_TREE_LEAST;
+  a.workgroups = (unsigned)(runs < held ? runs : held);
+  plan.stats = plan.all = 0;
+  if (a.whole) return true;
+  const unsigned pitch = a.head <= 64 ? 64 : a.head <= 96 ? 96 : 128;
+  const size_t slots = (size_t)a.workgroups + items;
+  plan.stats = slots * block * pitch * sizeof(float);
+  plan.all = plan.stats + slots * block * sizeof(float2);
+  return true;
+}
+
 }  // namespace
 
 extern "C" {
+
+int lego_hip_tree_attention_workspace_bytes(const long long* sizes, unsigned long long* bytes)
+{
+  TreeArgs a = {};
+  TreePlan plan;
+  if (!bytes || !plan_of(a, sizes, plan)) return kInvalid;
+  *bytes = plan.all;
+  return 0;
+}
+
+int lego_hip_tree_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* out, const int* pages, const int* lengths,
+                            const unsigned char* tree, const float* slopes, const int* positions, const long long* sizes, const long long* strides, float scale,
+                            float softcap, int element, void* workspace, unsigned long long workspace_bytes, void* stream)
+{
+  TreeArgs a = {};
+  TreePlan plan;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !pages || !lengths || !strides || element < 0 || element > 1) return kInvalid;
+  if ((k == nullptr) != (v == nullptr) || (k && (!aligned16(k) || !aligned16(v))) || (!k && tree)) return kInvalid;
+  if (!aligned4(pages) || !aligned4(lengths) || !aligned4(slopes) || !aligned4(positions) || (positions && !slopes) || !plan_of(a, sizes, plan)) return kInvalid;
+  if (!(fabsf(scale) < INFINITY) || !(softcap >= 0.0f && softcap < INFINITY)) return kInvalid;
+  Strides* const into[6] = {&a.sq, &a.sk, &a.sv, &a.skc, &a.svc, &a.so};
+  const long long count[6][3] = {{a.batch, a.drafts, a.heads}, {a.batch, a.drafts, a.key_heads}, {a.batch, a.drafts, a.key_heads}, {a.count, a.page, a.key_heads},
+                                 {a.count, a.page, a.key_heads}, {a.batch, a.drafts, a.heads}};
+  for (int t = 0; t < 6; ++t) {
+    *into[t] = {strides[3 * t], strides[3 * t + 1], strides[3 * t + 2]};
+    unsigned __int128 extent = 0;
+    for (int i = 0; i < 3; ++i) {
+      if (strides[3 * t + i] < 0 || strides[3 * t + i] % 8) return kInvalid;
+      extent += (unsigned __int128)strides[3 * t + i] * (count[t][i] - 1);
+    }
+    if (extent / 8 + LEGO_ATTENTION_MAX_HEAD / 8 >= 0xffffffffu && t > 0 && t < 5) return kInvalid;      // rows are told apart by 32 bits of 16-byte chunks
+  }
+  a.tree_batch = strides[18];
+  if (a.tree_batch < 0) return kInvalid;
+  if (plan.all && (!aligned16(workspace) || workspace_bytes < plan.all)) return kInvalid;
+  const float log2e = 1.4426950408889634f;
+  a.scores = {scale, scale * log2e, softcap > 0.0f ? 2.0f * scale * log2e / softcap : 0.0f, softcap * log2e};
+  a.capped = softcap > 0.0f;
+  a.q = q, a.k = k, a.v = v, a.k_cache = k_cache, a.v_cache = v_cache, a.o = out, a.pages = pages, a.lengths = lengths, a.tree = tree, a.slopes = slopes, a.positions = positions;
+  a.sums = static_cast<float*>(workspace);
+  a.stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + plan.stats);
+  static hipError_t (*const launch[2][3])(const TreeArgs&, int, hipStream_t) = {{lego_tree_f16_d64_launch, lego_tree_f16_d96_launch, lego_tree_f16_d128_launch},
+                                                                               {lego_tree_bf16_d64_launch, lego_tree_bf16_d96_launch, lego_tree_bf16_d128_launch}};
+  return (int)launch[element][a.head <= 64 ? 0 : a.head <= 96 ? 1 : 2](a, plan.row_waves, as_stream(stream));
+}
 
 int lego_hip_attention_workspace_bytes(const long long* sizes, int documents, int backward, unsigned long long* bytes)
 {

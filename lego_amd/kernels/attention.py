@@ -22,6 +22,7 @@ MAX_HEAD = HEADS[-1]
 ROWS = 64
 WAVES = 4
 LAZY = 8
+TREE_LEAST = 2      # tiles of a run at least
 
 
 def tile_layout(rows, chunks):
@@ -63,6 +64,7 @@ def _tile_params(head, waves):
     assert all(unit == (x * 16 * pitch * 2 + y * 8 * pitch * 2, (32 * y) ^ (64 * z)) for (x, y, z), unit in tr_units.items())
     # memory -> LDS: copy `it` of wave w fills slots 64 (waves it + w) .. + 63; a lane's chunk is the same for all copies, its rows are a
     # whole number of rows apart
+    g = idx("g")      # number of a copy among all waves'
     slot = 64 * (waves * it + wave) + lane
     copies = ROWS * pitch * 2 // 1024 // waves
     row_e, chunk_e = (tidy(e, {lane: (0, 64), wave: (0, waves), it: (0, copies)}) for e in lds.inv(slot))
@@ -74,6 +76,8 @@ def _tile_params(head, waves):
     return dict(DC=head, PITCH=pitch, WAVES=waves, LAZY=LAZY, XCDS=XCDS,
                 lds_layout=f"OrderBy(GenP(({ROWS}, {chunks}), row*{chunks} + (chunk ^ key(row)))).TileBy([{ROWS}, {chunks}])",
                 row_lane=code(tidy(row_lane / 16, rng)), tr_lane=code(tidy(tr_lane / 16, rng)),
+                any_row=code(tidy(lds.inv(64 * g + lane)[0], {lane: (0, 64), g: (0, ROWS * pitch // 512)})),
+                any_chunk=code(tidy(lds.inv(64 * g + lane)[1], {lane: (0, 64), g: (0, ROWS * pitch // 512)})),
                 fill_row=code(tidy(row_e.subs(it, 0), rng)), fill_chunk=code(tidy(chunk_e.subs(it, 0), rng)))
 
 
@@ -87,6 +91,8 @@ def emit():
         for head in HEADS:
             params = dict(_tile_params(head, WAVES), banner=BANNER, elt=elt, dt=dt, tag=f"{dt}_d{head}", pid=pid, launch_layout=launch,
                           PSHIFT=8 if dt == "f16" else 0)
+            params["LEAST"] = TREE_LEAST
+            units.append(Emitted(f"tree_attention_{dt}_d{head}.hip", template("tree_attention.hip.j2").render(**params), [f"lego_tree_{dt}_d{head}_launch"]))
             for way in ("fwd", "bwd"):
                 name = f"attention_{way}_{dt}_d{head}"
                 units.append(Emitted(f"{name}.hip", template(f"attention_{way}.hip.j2").render(**params), [f"lego_{name}_launch"]))
@@ -99,4 +105,4 @@ def emit():
         banner=BANNER, stat=stat, stat_layout="OrderBy(Row(batch, heads, queries)).TileBy([batch, heads, queries])[b, h, i]",
         parts_layout="OrderBy(Row(parts, 2, batch, key heads, keys, head))"),
         ["lego_attention_tiles_launch", "lego_attention_delta_launch", "lego_attention_join_launch"]))
-    return units, dict(HEADS=HEADS, MAX_HEAD=MAX_HEAD, ELEMENTS=tuple(ELEMENTS))
+    return units, dict(HEADS=HEADS, TREE_LEAST=TREE_LEAST, MAX_HEAD=MAX_HEAD, ELEMENTS=tuple(ELEMENTS))

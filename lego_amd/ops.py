@@ -486,7 +486,15 @@ def _in_chunks(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _check_qkv(q, k, v):
+def _cache_in_chunks(t):
+    """A cache is never copied: it is what the program lays out once."""
+    st = _strides(t)
+    if t.stride(3) != 1 or t.data_ptr() % 16 or st[0] % 8 or st[1] % 8 or st[2] % 8:
+        raise ValueError("the caches must have elements one apart, and bases and strides in whole 16 bytes")
+    return t
+
+
+def _check_qkv(q, k, v, cache=False):
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not t.is_cuda:
             raise ValueError(f"{name} must live on the GPU")
@@ -498,7 +506,7 @@ def _check_qkv(q, k, v):
             raise ValueError("q, k and v must have the same dtype and device")
     if k.shape != v.shape:
         raise ValueError("k and v must have the same shape")
-    if k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+    if (k.shape[0] != q.shape[0] and not cache) or k.shape[3] != q.shape[3]:
         raise ValueError("q and k must have the same batch and head size")
     if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError("the query heads must be a multiple of the key heads")
@@ -627,6 +635,69 @@ def attention(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, docum
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return LEGOAttention.apply(q, k, v, causal, scale, softcap, slopes, documents, prefix)
     return attention_fwd(q, k, v, causal, scale, softcap, slopes, documents, prefix)[0]
+
+
+def tree_attention(q, k, v, k_cache, v_cache, pages, lengths, tree=None, scale=None, softcap=0.0, slopes=None, positions=None):
+    """Attention of drafted tokens over a paged cache, without gradients: one drafted token a sequence is a step of ordinary decoding, more are a chain
+    or a tree to be verified.  fp16 or bf16, fp32 softmax and sums; any lengths side by side.
+
+    q is ``[batch, draft, heads, element]``, k and v, the drafts' own, ``[batch, draft, key heads, element]``; the caches are
+    ``[page, row, key heads, element]``, pages of any number of rows.  Key i of sequence b lies in row ``i % rows`` of page ``pages[b, i // rows]`` (int32
+    ``[batch, width]``; a number that is no page's stands for keys that are not there), for i below ``lengths[b]`` (int32 ``[batch]``, at most ``width * rows``).
+    A draft sees all cached keys of its sequence and the drafts that ``tree`` (bool ``[draft, draft]`` or ``[batch, draft, draft]``: which one, a row, sees which) shows it; without
+    ``tree`` itself and the earlier ones.  With k and v None it sees the cache alone.  Scores are ``attention``'s; the distances of ``slopes`` go by ``positions`` (int32
+    ``[batch, draft]``, a cached key's being its number; default ``lengths[b] + draft``).  A draft that sees nothing gives zeros."""
+    if (k is None) != (v is None):
+        raise ValueError("k and v go together")
+    _check_qkv(q, *((k_cache, v_cache) if k is None else (k, v)), cache=k is None)
+    if k is not None:
+        if k.shape[1] != q.shape[1]:
+            raise ValueError("q, k and v must have the same drafts")
+        if k_cache.shape != v_cache.shape or k_cache.dim() != 4 or k_cache.shape[2:] != k.shape[2:] or any(t.dtype != q.dtype or t.device != q.device for t in (k_cache, v_cache)):
+            raise ValueError("the caches must be [page, row, key head, element] of k's heads, dtype and device")
+    batch, drafts, heads, head = q.shape
+    count, page, key_heads = k_cache.shape[:3]
+    scale = 1.0 / math.sqrt(head) if scale is None else float(scale)
+    softcap = float(softcap or 0.0)
+    if not math.isfinite(scale) or not 0.0 <= softcap < math.inf:
+        raise ValueError("scale must be finite, and softcap positive, or 0 for none")
+    if pages.dim() != 2:
+        raise ValueError("pages must be [batch, width]")
+    width = pages.shape[1]
+    pages = _vector(pages, "pages", torch.int32, (batch, width), q.device)
+    lengths = _vector(lengths, "lengths", torch.int32, (batch,), q.device)
+    slopes = _vector(slopes, "slopes", torch.float32, (heads,), q.device)
+    if positions is not None and slopes is None:
+        raise ValueError("positions are what slopes go by")
+    positions = _vector(positions, "positions", torch.int32, (batch, drafts), q.device)
+    if tree is not None:
+        if k is None:
+            raise ValueError("a tree is of drafts: it takes k and v")
+        tree = _vector(tree, "tree", torch.bool, (drafts, drafts) if tree.dim() == 2 else (batch, drafts, drafts), q.device)
+        if slopes is not None and positions is None:
+            raise ValueError("in a tree, slopes take the drafts' positions")
+    out = torch.empty((batch, drafts, heads, head), dtype=q.dtype, device=q.device)
+    if out.numel() == 0:
+        return out
+    if count * page * width == 0:      # no cache: the drafts among themselves
+        if k is None:
+            return out.zero_()
+        k, v = _in_chunks(k), _in_chunks(v)
+        k_cache, v_cache, pages, count, page, width = k, v, torch.full((batch, 1), -1, dtype=torch.int32, device=q.device), 1, 1, 1
+    with _on(q):
+        q, k_cache, v_cache = _in_chunks(q), _cache_in_chunks(k_cache), _cache_in_chunks(v_cache)
+        if k is not None:
+            k, v = _in_chunks(k), _in_chunks(v)
+        sizes = _longs((batch, drafts, heads, key_heads, head, page, count, width))
+        size = ctypes.c_ulonglong(0)
+        runtime.call("lego_hip_tree_attention_workspace_bytes", sizes, ctypes.byref(size))
+        workspace = torch.empty(size.value, dtype=torch.uint8, device=q.device) if size.value else None
+        none = [0, 0, 0]
+        strides = _longs(_strides(q) + (none if k is None else _strides(k)) + (none if v is None else _strides(v)) + _strides(k_cache) + _strides(v_cache) + _strides(out)
+                         + [0 if tree is None or tree.dim() == 2 else drafts * drafts])
+        runtime.call("lego_hip_tree_attention", _ptr(q), _optional(k), _optional(v), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(pages), _ptr(lengths), _optional(tree),
+                     _optional(slopes), _optional(positions), sizes, strides, scale, softcap, _ATTENTION_ELEMENT[q.dtype], _optional(workspace), size.value, _stream())
+    return out
 
 
 _ROTARY_ELEMENT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
