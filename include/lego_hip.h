@@ -380,15 +380,15 @@ int lego_hip_attention_workspace_bytes(const long long* sizes, int documents, in
  * Query i stands at position i + keys - queries.  It sees key j if
  *   causal is 0, or j is no later, or j < prefix[batch] (int32, given with causal 1 only), and
  *   documents (int32 [batch][keys], given for queries <= keys only) is null, or holds the same number, not negative, at both positions.
- * Keys of a negative document are never read, whatever they hold.  strides: of q, k, v and out, three each.
+ * Keys of a negative document are never read, whatever they hold.  rest, laid out as out, or null: what rounding took from out.  strides: of q, k, v and out, three each.
  * workspace (16-byte aligned): what lego_hip_attention_workspace_bytes says, null where that is 0. */
-int lego_hip_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const long long* sizes, const long long* strides, float scale,
+int lego_hip_attention_fwd(const void* q, const void* k, const void* v, void* out, void* rest, float* lse, const long long* sizes, const long long* strides, float scale,
                            float softcap, const float* slopes, const int* documents, const int* prefix, int causal, int element, void* workspace,
                            unsigned long long workspace_bytes, void* stream);
 
-/* Gradients of q, k and v from that of out; out and lse as the forward pass left them.  Queries that see no key give and get none.
+/* Gradients of q, k and v from that of out; out, rest (or null) and lse as the forward pass left them: the row sums of out * dout take what rounding took from out with rest.  Queries that see no key give and get none.
  * strides: of q, k, v, out, dout, dq, dk and dv, three each.  The result does not depend on the order in which workgroups run. */
-int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const void* rest, const float* lse, void* dq, void* dk, void* dv,
                            const long long* sizes, const long long* strides, float scale, float softcap, const float* slopes, const int* documents, const int* prefix,
                            int causal, int element, void* workspace, unsigned long long workspace_bytes, void* stream);
 

@@ -13,8 +13,8 @@ struct Scores {
 };
 
 struct AttentionArgs {
-  const void *q, *k, *v, *out, *dout;
-  void *o, *dq, *dk, *dv;
+  const void *q, *k, *v, *out, *rest, *dout;
+  void *o, *o_rest, *dq, *dk, *dv;      // rest: what rounding took from out, laid out as out, or null
   float* lse;                   // [batch][head][query], natural logarithm
   float* delta;                 // the same, of the backward pass: sum of out * dout
   float* ups;                   // [batch][head][tile of 64 queries]: power of two that brings the tile's largest dout to 1..2

@@ -27,6 +27,7 @@ typedef __attribute__((address_space(3))) short4v lds_short4;
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -122,6 +123,14 @@ struct Filler {
     }
   }
 };
+// 64 words, a statistic or a number of each row, into LDS by one wavefront; rows past the last one read as zeros
+__device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsigned lane, unsigned lds)
+{
+  const uintptr_t at = reinterpret_cast<uintptr_t>(base);
+  const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
+                      (unsigned)__builtin_amdgcn_readfirstlane(4 * min(rows, ROWS)), 0x00020000u};
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(4 * lane), "s"(rsrc), "s"(lds) : "memory", "m0");
+}
 __device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Score function, in units of log2 e: what the exponential takes.  CAP: cap * tanh(scale q.k / cap) as cap (1 - 2 / (e^(2x) + 1)); its derivative by
@@ -156,31 +165,40 @@ struct Seen {
 __device__ __forceinline__ bool apart(int2 a, int2 b) { return a.y < 0 || b.y < 0 || a.y < b.x || b.y < a.x; }
 __device__ __forceinline__ bool same(int2 a, int2 b) { return a.x == a.y && b.x == b.y && a.x == b.x; }
 
+// What a look at the documents of a tile (t) tells beside those of the workgroup's own rows.
+constexpr unsigned kNeeded = 1, kCompare = 2, kPadded = 4;
+__device__ __forceinline__ unsigned look_at(int2 t, int2 own) { return apart(t, own) ? 0u : same(t, own) ? kNeeded : kNeeded | kCompare | (t.x < 0 ? kPadded : 0u); }
+
 // The tiles that a workgroup goes through, in order: 64 at a time are looked at, a lane each.
+struct Step {
+  unsigned tile;                // ~0u: none is left
+  bool compare, padded;         // documents have to be compared; some rows of the tile are padding
+  __device__ __forceinline__ bool there() const { return tile != ~0u; }
+};
 template <class Look>
 struct Walk {
-  const Look& look;             // (tile) -> bit 0: needed, bit 1: documents have to be compared
+  const Look& look;             // (tile) -> kNeeded, kCompare, kPadded
   unsigned lane, base, end;
-  unsigned long long need = 0, compare = 0;
+  unsigned long long need = 0, compare = 0, padded = 0;
   __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin_, unsigned end_) : look(look_), lane(lane_), base(begin_), end(end_) { fetch(); }
   __device__ __forceinline__ void fetch()
   {
     const unsigned tile = base + lane;
     const unsigned bits = tile < end ? look(tile) : 0u;
-    need = __builtin_amdgcn_ballot_w64((bits & 1u) != 0);
-    compare = __builtin_amdgcn_ballot_w64((bits & 2u) != 0);
+    need = __builtin_amdgcn_ballot_w64((bits & kNeeded) != 0);
+    compare = __builtin_amdgcn_ballot_w64((bits & kCompare) != 0);
+    padded = __builtin_amdgcn_ballot_w64((bits & kPadded) != 0);
   }
-  // the next tile, with bit 31 where documents have to be compared, or ~0u
-  __device__ __forceinline__ unsigned next()
+  __device__ __forceinline__ Step next()
   {
     while (need == 0) {
-      if (base + 64 >= end) return ~0u;
+      if (base + 64 >= end) return {~0u, false, false};
       base += 64;
       fetch();
     }
     const unsigned at = (unsigned)__builtin_ctzll(need);
     need &= need - 1;
-    return (base + at) | ((unsigned)(compare >> at) & 1u) << 31;
+    return {base + at, (compare >> at & 1) != 0, (padded >> at & 1) != 0};
   }
 };
 
@@ -228,19 +246,10 @@ namespace {
 constexpr float kShift = 0.0f;        // P is held as 2^kShift P
 constexpr float kUnshift = 1.0f / (1 << 0);
 
-// 64 floats of a row-wise statistic into LDS, by one wavefront; rows past the last one read as zeros
-__device__ __forceinline__ void fill_rows(const float* base, unsigned rows, unsigned lane, unsigned lds)
-{
-  const uintptr_t at = reinterpret_cast<uintptr_t>(base);
-  const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
-                      (unsigned)__builtin_amdgcn_readfirstlane(4 * min(rows, ROWS)), 0x00020000u};
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(4 * lane), "s"(rsrc), "s"(lds) : "memory", "m0");
-}
-
 template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_kernel(AttentionArgs a, unsigned per_xcd)
 {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 1024];      // Q and dO, twice; lse and delta, twice
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 2 * 768];      // Q and dO, twice; lse, delta and documents, twice
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
   const unsigned blocks = (a.keys + 32 * WAVES - 1) / (32 * WAVES), group = a.heads / a.key_heads, parts = group / a.heads_per_part;
   const unsigned wg = blockIdx.x;
@@ -279,14 +288,16 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
   const Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_base = (unsigned)(uintptr_t)(lds_ptr)lds, lds_at = lds_base + wave * 1024;
-  const auto fill = [&](unsigned h, unsigned tile, unsigned buffer) {
-    const unsigned first = 64 * (tile & 0x7fffffffu), rows = a.queries - first;
+  const auto fill = [&](unsigned h, const Step& step, unsigned buffer) {
+    const unsigned first = 64 * step.tile, rows = a.queries - first;
     const elt_t* const qb = static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch + (size_t)h * a.sq.head;
     const elt_t* const dob = static_cast<const elt_t*>(a.dout) + (size_t)b * a.sdo.batch + (size_t)h * a.sdo.head;
     const size_t row = ((size_t)b * a.heads + h) * a.queries + first;
-    const unsigned at = lds_at + buffer * (2 * TILE);
-    if (wave < 2) fill_rows((wave ? a.delta : a.lse) + row, rows, lane, lds_base + 4 * TILE + buffer * 512 + wave * 256);
-    if (tile >> 31) {      // rows that see no key are read as zeros, whatever they hold
+    const unsigned at = lds_at + buffer * (2 * TILE), words = lds_base + 4 * TILE + buffer * 768;
+    if (wave == 0) fill_words(a.lse + row, rows, lane, words);
+    if (wave == 1) fill_words(a.delta + row, rows, lane, words + 256);
+    if (wave == 2 && step.compare) fill_words(documents + first + shift, rows, lane, words + 512);
+    if (step.padded) {      // rows that see no key are read as zeros, whatever they hold
       const auto skip = [&](unsigned r) { return a.lse[row + min(r, rows - 1)] == -INFINITY; };
       fill_q(qb, first, q_stride, rows, at, skip);
       fill_do(dob, first, do_stride, rows, at + TILE, skip);
@@ -298,11 +309,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
   };
   const auto look = [&](unsigned tile) -> unsigned {
     const int first = (int)(64 * tile);
-    const unsigned empty = first + shift < 0 && a.causal ? 2u : 0u;      // rows before the first key
-    if (!documents) return 1u | empty;
+    if (!documents) return first + shift < 0 && a.causal ? kNeeded | kPadded : kNeeded;      // rows before the first key
     const int t0 = (first + shift) / 64, t1 = (min(first + 63, a.queries - 1) + shift) / 64;
-    const int2 t = t0 == t1 ? tiles[t0] : int2{min(tiles[t0].x, tiles[t1].x), max(tiles[t0].y, tiles[t1].y)};
-    return apart(t, own_tiles) ? 0u : same(t, own_tiles) ? 1u : 3u;
+    return look_at(t0 == t1 ? tiles[t0] : int2{min(tiles[t0].x, tiles[t1].x), max(tiles[t0].y, tiles[t1].y)}, own_tiles);
   };
 
   float16v dk[DB], dv[DB];
@@ -315,28 +324,28 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
   Queries walk(look, lane, begin, end);
   unsigned h = h0;
   const auto advance = [&](unsigned& head) {      // the next tile of the heads in turn
-    unsigned tile = walk.next();
-    while (tile == ~0u && head + 1 < h1) {
+    Step step = walk.next();
+    while (!step.there() && head + 1 < h1) {
       ++head;
       walk.base = begin;
       walk.fetch();
-      tile = walk.next();
+      step = walk.next();
     }
-    return tile;
+    return step;
   };
-  unsigned now = advance(h), buffer = 0;
-  if (now != ~0u) fill(h, now, 0);
-  while (now != ~0u) {
+  Step now = advance(h);
+  unsigned buffer = 0;
+  if (now.there()) fill(h, now, 0);
+  while (now.there()) {
     unsigned next_h = h;
-    const unsigned next = advance(next_h);
+    const Step next = advance(next_h);
     wait_for_copies();
     __syncthreads();
-    if (next != ~0u) fill(next_h, next, buffer ^ 1);
+    if (next.there()) fill(next_h, next, buffer ^ 1);
     const char* const qt = lds + buffer * (2 * TILE);
     const char* const dot = qt + TILE;
-    const float* const lse_s = reinterpret_cast<const float*>(lds + 4 * TILE + buffer * 512);
-    const int first = (int)(64 * (now & 0x7fffffffu));
-    const bool compare = documents && now >> 31;
+    const float* const lse_s = reinterpret_cast<const float*>(lds + 4 * TILE + buffer * 768);
+    const int first = (int)(64 * now.tile);
     const float slope = BIAS ? kLog2e * a.slopes[h] : 0.0f;
     if (first + 63 >= from_w0) {
 #pragma unroll
@@ -349,7 +358,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
         }
         // rows first + 32 qb + 8 (r / 4) + 4 lhi + r % 4
         const int row0 = first + 32 * (int)qb + 4 * (int)lhi;
-        const bool edge = first + 32 * (int)qb < from_w1;
+        const bool edge = first + 32 * (int)qb < from_w1 || first + 32 * (int)qb + 32 > a.queries;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4v lse = *reinterpret_cast<const float4v*>(lse_s + 32 * qb + 8 * g + 4 * lhi);
@@ -363,10 +372,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
             float p = __builtin_amdgcn_exp2f(x - (kLog2e * lse[e] - kShift));
             float ds = p * (dp[r] - delta[e]);
             if (CAP) ds *= bend;
-            if (edge && row < from_key) p = ds = 0.0f;
-            if (compare && !(own_document >= 0 && row < a.queries && documents[min(row, a.queries - 1) + shift] == own_document)) p = ds = 0.0f;
+            if (edge && (row < from_key || row >= a.queries)) p = ds = 0.0f;
             s[r] = p;
             dp[r] = ds;
+          }
+        }
+        if (now.compare) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4v d = *reinterpret_cast<const int4v*>(reinterpret_cast<const int*>(lse_s) + 128 + 32 * qb + 8 * g + 4 * lhi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(own_document >= 0 && d[e] == own_document)) s[4 * g + e] = dp[4 * g + e] = 0.0f;
           }
         }
         const Operands p = as_operands(s), ds = as_operands(dp);
@@ -408,7 +425,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
 template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kernel(AttentionArgs a, unsigned per_xcd)
 {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];      // K and V, twice
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 512];      // K and V, twice; the keys' documents, twice
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
   const unsigned blocks = (a.queries + 32 * WAVES - 1) / (32 * WAVES);
   const unsigned wg = blockIdx.x;
@@ -451,10 +468,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kern
   const Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
-  const auto fill = [&](unsigned tile, unsigned buffer) {
-    const unsigned first = 64 * (tile & 0x7fffffffu), rows = a.keys - first;
+  const auto fill = [&](const Step& step, unsigned buffer) {
+    const unsigned first = 64 * step.tile, rows = a.keys - first;
     const unsigned at = lds_at + buffer * (2 * TILE);
-    if (tile >> 31) {      // padding among the keys is read as zeros, whatever it holds
+    if (step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + 4 * TILE + buffer * 256);
+    if (step.padded) {      // padding among the keys is read as zeros, whatever it holds
       const auto skip = [&](unsigned row) { return documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
       fill_k(kb, first, k_stride, rows, at, skip);
       fill_v(vb, first, v_stride, rows, at + TILE, skip);
@@ -464,27 +482,24 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kern
       fill_v(vb, first, v_stride, rows, at + TILE, skip);
     }
   };
-  const auto look = [&](unsigned tile) -> unsigned {
-    if (!documents) return 1u;
-    const int2 t = tiles[tile];
-    return apart(t, own_tiles) ? 0u : same(t, own_tiles) ? 1u : 3u;
-  };
+  const auto look = [&](unsigned tile) { return documents ? look_at(tiles[tile], own_tiles) : kNeeded; };
 
   float16v dq[DB];
 #pragma unroll
   for (unsigned db = 0; db < DB; ++db) dq[db] = zeros();
   Walk<decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
-  unsigned now = walk.next(), buffer = 0;
-  if (now != ~0u) fill(now, 0);
-  while (now != ~0u) {
-    const unsigned next = walk.next();
+  Step now = walk.next();
+  unsigned buffer = 0;
+  if (now.there()) fill(now, 0);
+  while (now.there()) {
+    const Step next = walk.next();
     wait_for_copies();
     __syncthreads();
-    if (next != ~0u) fill(next, buffer ^ 1);
+    if (next.there()) fill(next, buffer ^ 1);
     const char* const kt = lds + buffer * (2 * TILE);
     const char* const vt = kt + TILE;
-    const int first = (int)(64 * (now & 0x7fffffffu));
-    const bool compare = now >> 31;
+    const int first = (int)(64 * now.tile);
+    const int* const document_s = reinterpret_cast<const int*>(lds + 4 * TILE + buffer * 256);
     if (first < limit_w1) {
 #pragma unroll
       for (unsigned kb2 = 0; kb2 < 2; ++kb2) {
@@ -507,8 +522,15 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kern
           float ds = p * (dp[r] - delta);
           if (CAP) ds *= bend;
           if (edge && key >= limit) ds = 0.0f;
-          if (compare && !(own_document >= 0 && documents[min(key, a.keys - 1)] == own_document)) ds = 0.0f;
           dp[r] = ds;
+        }
+        if (now.compare) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4v d = *reinterpret_cast<const int4v*>(document_s + 32 * kb2 + 8 * g + 4 * lhi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * g + e] = own_document >= 0 && d[e] == own_document ? dp[4 * g + e] : 0.0f;
+          }
         }
         const Operands ds = as_operands(dp);
 #pragma unroll

@@ -26,6 +26,7 @@ typedef __attribute__((address_space(3))) short4v lds_short4;
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -121,6 +122,14 @@ struct Filler {
     }
   }
 };
+// 64 words, a statistic or a number of each row, into LDS by one wavefront; rows past the last one read as zeros
+__device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsigned lane, unsigned lds)
+{
+  const uintptr_t at = reinterpret_cast<uintptr_t>(base);
+  const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
+                      (unsigned)__builtin_amdgcn_readfirstlane(4 * min(rows, ROWS)), 0x00020000u};
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(4 * lane), "s"(rsrc), "s"(lds) : "memory", "m0");
+}
 __device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Score function, in units of log2 e: what the exponential takes.  CAP: cap * tanh(scale q.k / cap) as cap (1 - 2 / (e^(2x) + 1)); its derivative by
@@ -155,31 +164,40 @@ struct Seen {
 __device__ __forceinline__ bool apart(int2 a, int2 b) { return a.y < 0 || b.y < 0 || a.y < b.x || b.y < a.x; }
 __device__ __forceinline__ bool same(int2 a, int2 b) { return a.x == a.y && b.x == b.y && a.x == b.x; }
 
+// What a look at the documents of a tile (t) tells beside those of the workgroup's own rows.
+constexpr unsigned kNeeded = 1, kCompare = 2, kPadded = 4;
+__device__ __forceinline__ unsigned look_at(int2 t, int2 own) { return apart(t, own) ? 0u : same(t, own) ? kNeeded : kNeeded | kCompare | (t.x < 0 ? kPadded : 0u); }
+
 // The tiles that a workgroup goes through, in order: 64 at a time are looked at, a lane each.
+struct Step {
+  unsigned tile;                // ~0u: none is left
+  bool compare, padded;         // documents have to be compared; some rows of the tile are padding
+  __device__ __forceinline__ bool there() const { return tile != ~0u; }
+};
 template <class Look>
 struct Walk {
-  const Look& look;             // (tile) -> bit 0: needed, bit 1: documents have to be compared
+  const Look& look;             // (tile) -> kNeeded, kCompare, kPadded
   unsigned lane, base, end;
-  unsigned long long need = 0, compare = 0;
+  unsigned long long need = 0, compare = 0, padded = 0;
   __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin_, unsigned end_) : look(look_), lane(lane_), base(begin_), end(end_) { fetch(); }
   __device__ __forceinline__ void fetch()
   {
     const unsigned tile = base + lane;
     const unsigned bits = tile < end ? look(tile) : 0u;
-    need = __builtin_amdgcn_ballot_w64((bits & 1u) != 0);
-    compare = __builtin_amdgcn_ballot_w64((bits & 2u) != 0);
+    need = __builtin_amdgcn_ballot_w64((bits & kNeeded) != 0);
+    compare = __builtin_amdgcn_ballot_w64((bits & kCompare) != 0);
+    padded = __builtin_amdgcn_ballot_w64((bits & kPadded) != 0);
   }
-  // the next tile, with bit 31 where documents have to be compared, or ~0u
-  __device__ __forceinline__ unsigned next()
+  __device__ __forceinline__ Step next()
   {
     while (need == 0) {
-      if (base + 64 >= end) return ~0u;
+      if (base + 64 >= end) return {~0u, false, false};
       base += 64;
       fetch();
     }
     const unsigned at = (unsigned)__builtin_ctzll(need);
     need &= need - 1;
-    return (base + at) | ((unsigned)(compare >> at) & 1u) << 31;
+    return {base + at, (compare >> at & 1) != 0, (padded >> at & 1) != 0};
   }
 };
 
@@ -230,7 +248,7 @@ constexpr float kLazy = 8.0f;
 template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d64_kernel(AttentionArgs a, unsigned per_xcd)
 {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];      // K and V, twice
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 512];      // K and V, twice; the keys' documents, twice
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
   const unsigned blocks = (a.queries + 32 * WAVES - 1) / (32 * WAVES);
   const unsigned wg = blockIdx.x;
@@ -271,10 +289,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d64_ker
   const Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
-  const auto fill = [&](unsigned tile, unsigned buffer) {
-    const unsigned first = 64 * (tile & 0x7fffffffu), rows = a.keys - first;
+  const auto fill = [&](const Step& step, unsigned buffer) {
+    const unsigned first = 64 * step.tile, rows = a.keys - first;
     const unsigned at = lds_at + buffer * (2 * TILE);
-    if (tile >> 31) {      // padding among the keys is read as zeros, whatever it holds
+    if (step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + 4 * TILE + buffer * 256);
+    if (step.padded) {      // padding among the keys is read as zeros, whatever it holds
       const auto skip = [&](unsigned row) { return documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
       fill_k(kb, first, k_stride, rows, at, skip);
       fill_v(vb, first, v_stride, rows, at + TILE, skip);
@@ -284,28 +303,25 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d64_ker
       fill_v(vb, first, v_stride, rows, at + TILE, skip);
     }
   };
-  const auto look = [&](unsigned tile) -> unsigned {
-    if (!documents) return 1u;
-    const int2 t = tiles[tile];
-    return apart(t, own_tiles) ? 0u : same(t, own_tiles) ? 1u : 3u;
-  };
+  const auto look = [&](unsigned tile) { return documents ? look_at(tiles[tile], own_tiles) : kNeeded; };
 
   float16v acc[DB];
 #pragma unroll
   for (unsigned db = 0; db < DB; ++db) acc[db] = zeros();
   float most = -INFINITY, sum = 0.0f;      // of the lane's own keys; the halves agree on `most`
   Walk<decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
-  unsigned now = walk.next(), buffer = 0;
-  if (now != ~0u) fill(now, 0);
-  while (now != ~0u) {
-    const unsigned next = walk.next();
+  Step now = walk.next();
+  unsigned buffer = 0;
+  if (now.there()) fill(now, 0);
+  while (now.there()) {
+    const Step next = walk.next();
     wait_for_copies();
     __syncthreads();                       // the tile is there, and the other buffer is read no more
-    if (next != ~0u) fill(next, buffer ^ 1);
+    if (next.there()) fill(next, buffer ^ 1);
     const char* const kt = lds + buffer * (2 * TILE);
     const char* const vt = kt + TILE;
-    const int first = (int)(64 * (now & 0x7fffffffu));
-    const bool compare = now >> 31;
+    const int first = (int)(64 * now.tile);
+    const int* const document_s = reinterpret_cast<const int*>(lds + 4 * TILE + buffer * 256);
     if (first < limit_w1) {
       float16v s[2] = {zeros(), zeros()};
 #pragma unroll
@@ -329,13 +345,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d64_ker
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[kb2][r] = (int)(32 * kb2 + 8 * (r / 4) + r % 4) < end ? s[kb2][r] : -INFINITY;
       }
-      if (compare) {
+      if (now.compare) {
 #pragma unroll
         for (unsigned kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = first + (int)(32 * kb2 + 8 * (r / 4) + 4 * lhi + r % 4);
-            s[kb2][r] = own_document >= 0 && documents[min(key, a.keys - 1)] == own_document ? s[kb2][r] : -INFINITY;
+          for (int g = 0; g < 4; ++g) {
+            const int4v d = *reinterpret_cast<const int4v*>(document_s + 32 * kb2 + 8 * g + 4 * lhi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[kb2][4 * g + e] = own_document >= 0 && d[e] == own_document ? s[kb2][4 * g + e] : -INFINITY;
           }
       }
       float top = s[0][0];
@@ -375,8 +392,20 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d64_ker
     buffer ^= 1;
   }
   sum = across_sum(sum);
-  elt_t* const row = i < a.queries ? static_cast<elt_t*>(a.o) + (size_t)b * a.so.batch + (size_t)i * a.so.token + (size_t)h * a.so.head : nullptr;
-  store_columns<DB>(acc, row, lane, a.head, sum == 0.0f ? 0.0f : 1.0f / sum);
+  const size_t row_at = (size_t)b * a.so.batch + (size_t)min(i, a.queries - 1) * a.so.token + (size_t)h * a.so.head;
+  const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (unsigned db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[db][r] *= factor;
+  store_columns<DB>(acc, i < a.queries ? static_cast<elt_t*>(a.o) + row_at : nullptr, lane, a.head, 1.0f);
+  if (a.o_rest) {
+#pragma unroll
+    for (unsigned db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] -= static_cast<float>(static_cast<elt_t>(acc[db][r]));
+    store_columns<DB>(acc, i < a.queries ? static_cast<elt_t*>(a.o_rest) + row_at : nullptr, lane, a.head, 1.0f);
+  }
   if (i < a.queries && lhi == 0) a.lse[((size_t)b * a.heads + h) * a.queries + i] = sum == 0.0f ? -INFINITY : kLn2 * (most + __builtin_amdgcn_logf(sum));
 }
 

@@ -39,6 +39,7 @@ __global__ void __launch_bounds__(256) lego_attention_delta_kernel(AttentionArgs
   const unsigned tile = blockIdx.x % tiles, h = blockIdx.x / tiles % a.heads, b = blockIdx.x / tiles / a.heads;
   const unsigned lane = threadIdx.x % 16, team = threadIdx.x / 16;
   const E* const out = static_cast<const E*>(a.out) + (size_t)b * a.so.batch + (size_t)h * a.so.head;
+  const E* const rest = a.rest ? static_cast<const E*>(a.rest) + (size_t)b * a.so.batch + (size_t)h * a.so.head : nullptr;
   const E* const dout = static_cast<const E*>(a.dout) + (size_t)b * a.sdo.batch + (size_t)h * a.sdo.head;
   float largest = 0.0f;
 #pragma unroll
@@ -50,9 +51,10 @@ __global__ void __launch_bounds__(256) lego_attention_delta_kernel(AttentionArgs
     const bool empty = !inside || a.lse[stat] == -INFINITY;      // a query that sees nothing gives no gradient, whatever its dout holds
     if (!empty && 8 * lane < (unsigned)a.head) {
       const elt8 x = *reinterpret_cast<const elt8*>(out + (size_t)i * a.so.token + 8 * lane), y = *reinterpret_cast<const elt8*>(dout + (size_t)i * a.sdo.token + 8 * lane);
+      const elt8 less = rest ? *reinterpret_cast<const elt8*>(rest + (size_t)i * a.so.token + 8 * lane) : elt8{};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        sum += (float)x[e] * (float)y[e];
+        sum += ((float)x[e] + (float)less[e]) * (float)y[e];
         largest = fmaxf(largest, fabsf((float)y[e]));
       }
     }

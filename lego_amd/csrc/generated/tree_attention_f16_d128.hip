@@ -27,6 +27,7 @@ typedef __attribute__((address_space(3))) short4v lds_short4;
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -122,6 +123,14 @@ struct Filler {
     }
   }
 };
+// 64 words, a statistic or a number of each row, into LDS by one wavefront; rows past the last one read as zeros
+__device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsigned lane, unsigned lds)
+{
+  const uintptr_t at = reinterpret_cast<uintptr_t>(base);
+  const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
+                      (unsigned)__builtin_amdgcn_readfirstlane(4 * min(rows, ROWS)), 0x00020000u};
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(4 * lane), "s"(rsrc), "s"(lds) : "memory", "m0");
+}
 __device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Score function, in units of log2 e: what the exponential takes.  CAP: cap * tanh(scale q.k / cap) as cap (1 - 2 / (e^(2x) + 1)); its derivative by
@@ -156,31 +165,40 @@ struct Seen {
 __device__ __forceinline__ bool apart(int2 a, int2 b) { return a.y < 0 || b.y < 0 || a.y < b.x || b.y < a.x; }
 __device__ __forceinline__ bool same(int2 a, int2 b) { return a.x == a.y && b.x == b.y && a.x == b.x; }
 
+// What a look at the documents of a tile (t) tells beside those of the workgroup's own rows.
+constexpr unsigned kNeeded = 1, kCompare = 2, kPadded = 4;
+__device__ __forceinline__ unsigned look_at(int2 t, int2 own) { return apart(t, own) ? 0u : same(t, own) ? kNeeded : kNeeded | kCompare | (t.x < 0 ? kPadded : 0u); }
+
 // The tiles that a workgroup goes through, in order: 64 at a time are looked at, a lane each.
+struct Step {
+  unsigned tile;                // ~0u: none is left
+  bool compare, padded;         // documents have to be compared; some rows of the tile are padding
+  __device__ __forceinline__ bool there() const { return tile != ~0u; }
+};
 template <class Look>
 struct Walk {
-  const Look& look;             // (tile) -> bit 0: needed, bit 1: documents have to be compared
+  const Look& look;             // (tile) -> kNeeded, kCompare, kPadded
   unsigned lane, base, end;
-  unsigned long long need = 0, compare = 0;
+  unsigned long long need = 0, compare = 0, padded = 0;
   __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin_, unsigned end_) : look(look_), lane(lane_), base(begin_), end(end_) { fetch(); }
   __device__ __forceinline__ void fetch()
   {
     const unsigned tile = base + lane;
     const unsigned bits = tile < end ? look(tile) : 0u;
-    need = __builtin_amdgcn_ballot_w64((bits & 1u) != 0);
-    compare = __builtin_amdgcn_ballot_w64((bits & 2u) != 0);
+    need = __builtin_amdgcn_ballot_w64((bits & kNeeded) != 0);
+    compare = __builtin_amdgcn_ballot_w64((bits & kCompare) != 0);
+    padded = __builtin_amdgcn_ballot_w64((bits & kPadded) != 0);
   }
-  // the next tile, with bit 31 where documents have to be compared, or ~0u
-  __device__ __forceinline__ unsigned next()
+  __device__ __forceinline__ Step next()
   {
     while (need == 0) {
-      if (base + 64 >= end) return ~0u;
+      if (base + 64 >= end) return {~0u, false, false};
       base += 64;
       fetch();
     }
     const unsigned at = (unsigned)__builtin_ctzll(need);
     need &= need - 1;
-    return (base + at) | ((unsigned)(compare >> at) & 1u) << 31;
+    return {base + at, (compare >> at & 1) != 0, (padded >> at & 1) != 0};
   }
 };
 
@@ -523,42 +541,56 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
   } while (true);
 }
 
-// The rows of items in several runs, and of those that have no tile: a lane has two elements of a row.
+// The rows of items in several runs, and of those that have no tile: a workgroup a row, DC / 4 lanes a part of its sums, the parts in turn.
 __global__ void __launch_bounds__(256) lego_tree_join_f16_d128_kernel(TreeArgs a, unsigned block_rows)
 {
-  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  constexpr unsigned LANES = DC / 4 > 16 ? 32 : 16, TEAMS = 256 / LANES;
+  __shared__ float4v sums_s[TEAMS][LANES];
+  __shared__ float2 stats_s[4];
+  const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = threadIdx.x % LANES, team = threadIdx.x / LANES;
   const unsigned group = a.heads / a.key_heads, rows = group * a.drafts, items = a.key_heads * a.row_blocks;
-  const unsigned at = blockIdx.x * 4 + wave;      // (sequence, key head, row)
-  const unsigned b = at / (a.key_heads * rows), hk = at / rows % a.key_heads, r = at % rows;
-  if (b >= (unsigned)a.batch) return;
+  const unsigned b = blockIdx.x / (a.key_heads * rows), hk = blockIdx.x / rows % a.key_heads, r = blockIdx.x % rows;
   const unsigned total = total_tiles(a, lane, items), run = run_of(a, total);
   const unsigned item = hk * a.row_blocks + r / block_rows;
   const unsigned tiles = sequence_of(a, b).tiles, first = tiles_before(a, lane, items, b) + item * tiles;
   const unsigned t = r / group, h = hk * group + r % group;
   elt_t* const row = static_cast<elt_t*>(a.o) + (size_t)b * a.so.batch + (size_t)t * a.so.token + (size_t)h * a.so.head;
-  const unsigned d = 2 * lane;
   if (tiles == 0) {
-    if (d < (unsigned)a.head) *reinterpret_cast<unsigned*>(row + d) = 0u;
+    if (threadIdx.x < (unsigned)a.head / 8) *reinterpret_cast<u32x4*>(row + 8 * threadIdx.x) = u32x4{0u, 0u, 0u, 0u};
     return;
   }
-  const unsigned w0 = first / run, w1 = (first + tiles - 1) / run;
-  if (w0 == w1) return;
-  const auto place = [&](unsigned w) { return ((size_t)w + (size_t)b * items + item) * block_rows + r % block_rows; };
+  const unsigned w0 = first / run, parts = (first + tiles - 1) / run - w0 + 1;
+  if (parts == 1) return;
+  const size_t place0 = ((size_t)w0 + (size_t)b * items + item) * block_rows + r % block_rows;      // parts are block_rows apart
   float most = -INFINITY;
-  for (unsigned w = w0; w <= w1; ++w) most = fmaxf(most, a.stats[place(w)].x);
-  float sum = 0.0f, x = 0.0f, y = 0.0f;
-  for (unsigned w = w0; w <= w1; ++w) {
-    const float2 stat = a.stats[place(w)];
+  for (unsigned p = threadIdx.x; p < parts; p += 256) most = fmaxf(most, a.stats[place0 + (size_t)p * block_rows].x);
+#pragma unroll
+  for (int d = 32; d; d /= 2) most = fmaxf(most, __shfl_xor(most, d));
+  if (lane == 0) stats_s[wave].x = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(stats_s[0].x, stats_s[1].x), fmaxf(stats_s[2].x, stats_s[3].x));
+  float sum = 0.0f;      // the same in every lane of a team
+  float4v x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (unsigned p = team; p < parts; p += TEAMS) {
+    const size_t place = place0 + (size_t)p * block_rows;
+    const float2 stat = a.stats[place];
     const float f = stat.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat.x - most);
     sum += f * stat.y;
-    if (d < (unsigned)a.head) {
-      const float2 v = *reinterpret_cast<const float2*>(a.sums + place(w) * DC + d);
-      x += f * v.x;
-      y += f * v.y;
-    }
+    if (4 * c < DC) x += f * *reinterpret_cast<const float4v*>(a.sums + place * DC + 4 * c);
+  }
+  sums_s[team][c] = x;
+  __shared__ float sum_s[TEAMS];
+  if (c == 0) sum_s[team] = sum;
+  __syncthreads();
+  if (team) return;
+#pragma unroll
+  for (unsigned i = 1; i < TEAMS; ++i) {
+    x += sums_s[i][c];
+    sum += sum_s[i];
   }
   const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (d < (unsigned)a.head) *reinterpret_cast<unsigned*>(row + d) = pack(factor * x, factor * y);
+  if (4 * c < (unsigned)a.head) *reinterpret_cast<u32x2*>(row + 4 * c) = u32x2{pack(factor * x[0], factor * x[1]), pack(factor * x[2], factor * x[3])};
 }
 
 template <unsigned RW>
@@ -573,7 +605,7 @@ hipError_t launch_rows(const TreeArgs& a, hipStream_t stream)
   else e = a.slopes ? launch(lego_tree_f16_d128_kernel<false, true, RW>) : launch(lego_tree_f16_d128_kernel<false, false, RW>);
   if (e != hipSuccess || a.whole) return e;
   const unsigned all = (unsigned)(a.batch * a.heads * a.drafts);
-  hipLaunchKernelGGL(lego_tree_join_f16_d128_kernel, dim3((all + 3) / 4), dim3(256), 0, stream, a, 32 * RW);
+  hipLaunchKernelGGL(lego_tree_join_f16_d128_kernel, dim3(all), dim3(256), 0, stream, a, 32 * RW);
   return hipGetLastError();
 }
 

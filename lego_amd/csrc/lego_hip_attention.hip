@@ -189,16 +189,16 @@ int lego_hip_attention_workspace_bytes(const long long* sizes, int documents, in
   return 0;
 }
 
-int lego_hip_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const long long* sizes, const long long* strides, float scale,
+int lego_hip_attention_fwd(const void* q, const void* k, const void* v, void* out, void* rest, float* lse, const long long* sizes, const long long* strides, float scale,
                            float softcap, const float* slopes, const int* documents, const int* prefix, int causal, int element, void* workspace,
                            unsigned long long workspace_bytes, void* stream)
 {
   AttentionArgs a = {};
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !lse || !aligned4(lse) || !strides || element < 0 || element > 1) return kInvalid;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (rest && !aligned16(rest)) || !lse || !aligned4(lse) || !strides || element < 0 || element > 1) return kInvalid;
   if (!take_sizes(a, sizes) || !take(a.sq, strides) || !take(a.sk, strides + 3) || !take(a.sv, strides + 6) || !take(a.so, strides + 9)) return kInvalid;
   if (!take_mask(a, scale, softcap, slopes, documents, prefix, causal)) return kInvalid;
   if (documents && (!aligned16(workspace) || workspace_bytes < room_of(a, true, false).all)) return kInvalid;
-  a.q = q, a.k = k, a.v = v, a.o = out, a.lse = lse;
+  a.q = q, a.k = k, a.v = v, a.o = out, a.o_rest = rest, a.lse = lse;
   if (documents) {
     a.tiles = static_cast<int2*>(workspace);
     const hipError_t e = lego_attention_tiles_launch(documents, a.tiles, a.batch, a.keys, as_stream(stream));
@@ -207,14 +207,14 @@ int lego_hip_attention_fwd(const void* q, const void* k, const void* v, void* ou
   return (int)forward(a, element, as_stream(stream));
 }
 
-int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, void* dq, void* dk, void* dv,
+int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const void* rest, const float* lse, void* dq, void* dk, void* dv,
                            const long long* sizes, const long long* strides, float scale, float softcap, const float* slopes, const int* documents, const int* prefix,
                            int causal, int element, void* workspace, unsigned long long workspace_bytes, void* stream)
 {
   AttentionArgs a = {};
   for (const void* p : {dout, q, k, v, out, (const void*)dq, (const void*)dk, (const void*)dv})
     if (!aligned16(p)) return kInvalid;
-  if (!lse || !aligned4(lse) || !strides || element < 0 || element > 1 || !take_sizes(a, sizes)) return kInvalid;
+  if ((rest && !aligned16(rest)) || !lse || !aligned4(lse) || !strides || element < 0 || element > 1 || !take_sizes(a, sizes)) return kInvalid;
   Strides* const into[8] = {&a.sq, &a.sk, &a.sv, &a.so, &a.sdo, &a.sdq, &a.sdk, &a.sdv};
   for (int t = 0; t < 8; ++t)
     if (!take(*into[t], strides + 3 * t)) return kInvalid;
@@ -222,7 +222,7 @@ int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const
   const Room room = room_of(a, documents != nullptr, true);
   if (!aligned16(workspace) || workspace_bytes < room.all) return kInvalid;
   char* const at = static_cast<char*>(workspace);
-  a.q = q, a.k = k, a.v = v, a.out = out, a.dout = dout, a.lse = const_cast<float*>(lse), a.dq = dq, a.dk = dk, a.dv = dv;
+  a.q = q, a.k = k, a.v = v, a.out = out, a.rest = rest, a.dout = dout, a.lse = const_cast<float*>(lse), a.dq = dq, a.dk = dk, a.dv = dv;
   a.tiles = reinterpret_cast<int2*>(at), a.delta = reinterpret_cast<float*>(at + room.delta), a.ups = reinterpret_cast<float*>(at + room.ups);
   a.parts = room.all > room.parts ? reinterpret_cast<float*>(at + room.parts) : nullptr;
   a.heads_per_part = heads_per_part(a);

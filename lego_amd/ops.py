@@ -56,7 +56,7 @@ def _check(t, dtype, name, ndim=2):
 class _InPython:
     """In place of the module in C++: every call is Python's."""
 
-    transpose = softmax = stencil = matmul = group = staticmethod(lambda *args: None)
+    transpose = softmax = stencil = matmul = group = attention = tree = rotary = staticmethod(lambda *args: None)
 
 
 _calls = None
@@ -556,35 +556,41 @@ def _attention_room(sizes, documents, backward, device):
     return (torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None), size.value
 
 
-def attention_fwd(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None):
+def attention_fwd(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None, with_rest=False):
     """Attention without its gradient; returns ``(out, lse)``, with the fp32 logarithm of every query's sum of exponentials,
-    ``[batch, head, query]`` (-inf for a query that sees no key).  Arguments as ``attention`` has them."""
+    ``[batch, head, query]`` (-inf for a query that sees no key), and ``with_rest`` what rounding took from ``out`` too, in a tensor like it.  Arguments as
+    ``attention`` has them."""
     _check_qkv(q, k, v)
     slopes, documents, prefix, scale, softcap = _check_mask(q, k, causal, scale, softcap, slopes, documents, prefix)
     batch, queries, heads, head = q.shape
     out = torch.empty((batch, queries, heads, head), dtype=q.dtype, device=q.device)
     lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=q.device)
+    rest = torch.empty_like(out) if with_rest else None
+    back = (out, lse, rest) if with_rest else (out, lse)
     if out.numel() == 0:
-        return out, lse
+        return back
     if k.shape[1] == 0:
-        return out.zero_(), lse.fill_(-math.inf)
+        out.zero_(), lse.fill_(-math.inf)
+        if with_rest:
+            rest.zero_()
+        return back
     with _on(q):
         q, k, v = _in_chunks(q), _in_chunks(k), _in_chunks(v)
         sizes = _longs((batch, queries, k.shape[1], heads, k.shape[2], head))
         workspace, room = _attention_room(sizes, 1, 0, q.device) if documents is not None else (None, 0)
-        runtime.call("lego_hip_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), sizes,
+        runtime.call("lego_hip_attention_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(out), _optional(rest), _ptr(lse), sizes,
                      _longs(_strides(q) + _strides(k) + _strides(v) + _strides(out)), scale, softcap, _optional(slopes), _optional(documents),
                      _optional(prefix), 1 if causal else 0, _ATTENTION_ELEMENT[q.dtype], _optional(workspace), room, _stream())
-    return out, lse
+    return back
 
 
-def attention_bwd(dout, q, k, v, out, lse, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None):
-    """The gradients ``(dq, dk, dv)`` from that of ``out``, with ``out`` and ``lse`` of ``attention_fwd`` and its arguments.  Sums are in
-    fp32 and in a fixed order: the same inputs give the same bits."""
+def attention_bwd(dout, q, k, v, out, lse, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None, rest=None):
+    """The gradients ``(dq, dk, dv)`` from that of ``out``, with ``out`` and ``lse`` of ``attention_fwd`` and its arguments; with ``rest`` the rounding of
+    ``out`` is no part of their error.  Sums are in fp32 and in a fixed order: the same inputs give the same bits."""
     _check_qkv(q, k, v)
     slopes, documents, prefix, scale, softcap = _check_mask(q, k, causal, scale, softcap, slopes, documents, prefix)
     batch, queries, heads, head = q.shape
-    for name, t in (("dout", dout), ("out", out)):
+    for name, t in (("dout", dout), ("out", out), ("rest", out if rest is None else rest)):
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
             raise ValueError(f"{name} must have the shape, dtype and device of q")
     if tuple(lse.shape) != (batch, heads, queries) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
@@ -593,11 +599,12 @@ def attention_bwd(dout, q, k, v, out, lse, causal=False, scale=None, softcap=0.0
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     with _on(q):
-        dout, q, k, v, out = (_in_chunks(t) for t in (dout, q, k, v, out))
+        dout, q, k, v = (_in_chunks(t) for t in (dout, q, k, v))
+        out, rest = _in_chunks(out.contiguous()), None if rest is None else _in_chunks(rest.contiguous())
         sizes = _longs((batch, queries, k.shape[1], heads, k.shape[2], head))
         workspace, room = _attention_room(sizes, documents is not None, 1, q.device)
         strides = [st for t in (q, k, v, out, dout, dq, dk, dv) for st in _strides(t)]
-        runtime.call("lego_hip_attention_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), sizes,
+        runtime.call("lego_hip_attention_bwd", _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _optional(rest), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), sizes,
                      _longs(strides), scale, softcap, _optional(slopes), _optional(documents), _optional(prefix), 1 if causal else 0,
                      _ATTENTION_ELEMENT[q.dtype], _optional(workspace), room, _stream())
     return dq, dk, dv
@@ -608,16 +615,16 @@ class LEGOAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, causal, scale, softcap, slopes, documents, prefix):
-        out, lse = attention_fwd(q, k, v, causal, scale, softcap, slopes, documents, prefix)
-        ctx.save_for_backward(q, k, v, out, lse, slopes, documents, prefix)
+        out, lse, rest = attention_fwd(q, k, v, causal, scale, softcap, slopes, documents, prefix, with_rest=True)
+        ctx.save_for_backward(q, k, v, out, lse, slopes, documents, prefix, rest)
         ctx.how = (causal, scale, softcap)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, slopes, documents, prefix = ctx.saved_tensors
-        return attention_bwd(dout, q, k, v, out, lse, *ctx.how, slopes, documents, prefix) + (None,) * 6
+        q, k, v, out, lse, slopes, documents, prefix, rest = ctx.saved_tensors
+        return attention_bwd(dout, q, k, v, out, lse, *ctx.how, slopes, documents, prefix, rest) + (None,) * 6
 
 
 def attention(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None):
@@ -632,6 +639,9 @@ def attention(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, docum
     A NaN or infinity in a key or value reaches the queries that see it, and may reach others within 64 positions of those.
 
     Inside a captured graph call ``attention_fwd`` and ``attention_bwd``: autograd's own bookkeeping of leaves is not made for it."""
+    out = _host().attention(q, k, v, causal, scale, softcap, slopes, documents, prefix)
+    if out is not None:
+        return out
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return LEGOAttention.apply(q, k, v, causal, scale, softcap, slopes, documents, prefix)
     return attention_fwd(q, k, v, causal, scale, softcap, slopes, documents, prefix)[0]
@@ -647,6 +657,9 @@ def tree_attention(q, k, v, k_cache, v_cache, pages, lengths, tree=None, scale=N
     A draft sees all cached keys of its sequence and the drafts that ``tree`` (bool ``[draft, draft]`` or ``[batch, draft, draft]``: which one, a row, sees which) shows it; without
     ``tree`` itself and the earlier ones.  With k and v None it sees the cache alone.  Scores are ``attention``'s; the distances of ``slopes`` go by ``positions`` (int32
     ``[batch, draft]``, a cached key's being its number; default ``lengths[b] + draft``).  A draft that sees nothing gives zeros."""
+    out = _host().tree(q, k, v, k_cache, v_cache, pages, lengths, tree, scale, softcap, slopes, positions)
+    if out is not None:
+        return out
     if (k is None) != (v is None):
         raise ValueError("k and v go together")
     _check_qkv(q, *((k_cache, v_cache) if k is None else (k, v)), cache=k is None)
@@ -776,6 +789,9 @@ def rotary(q, k, positions, frequencies, interleaved=False, magnitude=1.0):
     q and k are ``[batch, token, head, element]``, positions (int32 or int64) ``[batch, token]`` or ``[token]``.  The first ``part = 2 * len(frequencies)`` elements
     of a head are turned: pair i by ``positions * frequencies[i]`` radians (float64, as ``rotary_frequencies`` makes them) and times ``magnitude``; pair i is elements
     ``(i, i + part/2)``, or ``(2i, 2i + 1)`` where ``interleaved``.  The others stay."""
+    out = _host().rotary(q, k, positions, frequencies, interleaved, magnitude)
+    if out is not None:
+        return out
     for name, t in (("q", q), ("k", k)):
         if t is None and name == "k":
             continue

@@ -92,9 +92,9 @@ SIGNATURES = {
     "lego_hip_grouped_gemm_f16_stamps": [_PTR_ARRAY, _PTR_ARRAY, _PTR_ARRAY, _INT_ARRAY, _c_int, _c_void_p],
     "lego_hip_gemm_stamps_read": [_c_void_p, _c_int],
     "lego_hip_attention_workspace_bytes": [_LONG_ARRAY, _c_int, _c_int, ctypes.POINTER(ctypes.c_ulonglong)],
-    "lego_hip_attention_fwd": [_c_void_p] * 5 + [_LONG_ARRAY, _LONG_ARRAY, _c_float, _c_float, _c_void_p, _c_void_p, _c_void_p,
+    "lego_hip_attention_fwd": [_c_void_p] * 6 + [_LONG_ARRAY, _LONG_ARRAY, _c_float, _c_float, _c_void_p, _c_void_p, _c_void_p,
                                _c_int, _c_int, _c_void_p, ctypes.c_ulonglong, _c_void_p],
-    "lego_hip_attention_bwd": [_c_void_p] * 9 + [_LONG_ARRAY, _LONG_ARRAY, _c_float, _c_float, _c_void_p, _c_void_p, _c_void_p,
+    "lego_hip_attention_bwd": [_c_void_p] * 10 + [_LONG_ARRAY, _LONG_ARRAY, _c_float, _c_float, _c_void_p, _c_void_p, _c_void_p,
                                _c_int, _c_int, _c_void_p, ctypes.c_ulonglong, _c_void_p],
     "lego_hip_rotary": [_c_void_p] * 6 + [_LONG_ARRAY, _LONG_ARRAY, _c_int, _c_float, _c_int, _c_int, _c_int, _c_void_p],
     "lego_hip_tree_attention_workspace_bytes": [_LONG_ARRAY, ctypes.POINTER(ctypes.c_ulonglong)],

@@ -116,14 +116,20 @@ def make(batch, queries, keys, heads, key_heads, dim, dtype, seed=0, layout="own
 
 
 def both(q, k, v, dout, **how):
-    out, lse = ops.attention_fwd(q, k, v, **how)
-    grads = ops.attention_bwd(dout, q, k, v, out, lse, **how)
+    out, lse, rest = ops.attention_fwd(q, k, v, **how, with_rest=True)
+    grads = ops.attention_bwd(dout, q, k, v, out, lse, **how, rest=rest)
     return (out, lse, *grads)
 
 
 def check(q, k, v, dout, **how):
     got = both(q, k, v, dout, **how)
-    close(got, *oracle(q, k, v, dout, **how))
+    want = oracle(q, k, v, dout, **how)
+    close(got, *want)
+    out, _, rest = ops.attention_fwd(q, k, v, **how, with_rest=True)      # what rounding took is at most a rounding
+    assert (rest.float().abs() <= U[out.dtype] * out.float().abs() + 2.0 ** -24).all()
+    without = ops.attention_fwd(q, k, v, **how)
+    assert torch.equal(without[0], got[0]) and torch.equal(without[1], got[1])
+    close(without + ops.attention_bwd(dout, q, k, v, *without, **how), *want)
     return got
 
 
@@ -240,8 +246,10 @@ def test_autograd_gradients_and_repeats():
         now = (out.detach(), *grads)
         first = first or now
         assert all(torch.equal(a, b) for a, b in zip(first, now))
-    got = both(q.detach(), k.detach(), v.detach(), dout, causal=True)
-    assert torch.equal(got[0], first[0]) and all(torch.equal(a, b) for a, b in zip(got[2:], first[1:]))
+    q0, k0, v0 = (t.detach() for t in (q, k, v))
+    out, lse, rest = ops.attention_fwd(q0, k0, v0, causal=True, with_rest=True)
+    got = ops.attention_bwd(dout, q0, k0, v0, out, lse, causal=True, rest=rest)
+    assert torch.equal(out, first[0]) and all(torch.equal(a, b) for a, b in zip(got, first[1:]))
     # shared keys through expand: autograd sums what the kernel gives for each
     k1 = torch.randn(1, 200, 1, 64, device="cuda").bfloat16().requires_grad_()
     out = ops.attention(q.detach(), k1.expand(2, -1, 2, -1), v.detach(), causal=True)
@@ -346,12 +354,12 @@ def test_refusals_of_the_entry_points():
     at = lambda i: p(4096 * (i + 1))      # noqa: E731
 
     def fwd(ptrs=None, sizes=good, st=None, scale=0.1, cap=0.0, slopes=None, docs=None, prefix=None, causal=1, element=1, ws=None, room=0):
-        return lib.lego_hip_attention_fwd(*(ptrs or [at(i) for i in range(5)]), longs(*sizes), st or strides(4), scale, cap, slopes, docs, prefix, causal, element, ws, room, None)
+        return lib.lego_hip_attention_fwd(*(ptrs or [at(i) for i in range(6)]), longs(*sizes), st or strides(4), scale, cap, slopes, docs, prefix, causal, element, ws, room, None)
 
-    for i in range(5):
-        ptrs = [at(j) for j in range(5)]
+    for i in range(6):
+        ptrs = [at(j) for j in range(6)]
         ptrs[i] = None
-        assert fwd(ptrs) == 1
+        assert i == 4 or fwd(ptrs) == 1      # (rest may be null)
         ptrs[i] = p(4096 + 2)
         assert fwd(ptrs) == 1
     assert fwd(scale=math.nan) == 1 and fwd(scale=math.inf) == 1 and fwd(cap=-1.0) == 1 and fwd(cap=math.nan) == 1 and fwd(element=2) == 1 and fwd(causal=2) == 1
@@ -360,9 +368,9 @@ def test_refusals_of_the_entry_points():
     assert fwd(sizes=(2, 101, 100, 4, 2, 64), docs=at(9), ws=at(10), room=1 << 20) == 1
     assert fwd(st=strides(4, s=(25600, 256, 60) * 4)) == 1 and fwd(st=strides(4, s=(25600, 1 << 25, 64) * 4)) == 1 and fwd(st=strides(4, s=(-8, 256, 64) * 4)) == 1
     bwd = lambda ptrs, ws, room: lib.lego_hip_attention_bwd(*ptrs, longs(*good), strides(8), 0.1, 0.0, None, None, None, 1, 1, ws, room, None)      # noqa: E731
-    ptrs = [at(i) for i in range(9)]
+    ptrs = [at(i) for i in range(10)]
     assert bwd(ptrs, None, 0) == 1 and bwd(ptrs, at(20), 16) == 1 and bwd(ptrs, p(4097), 1 << 30) == 1
-    for i in range(9):
+    for i in (0, 1, 2, 3, 4, 6, 7, 8, 9):
         assert bwd([None if j == i else x for j, x in enumerate(ptrs)], at(20), 1 << 30) == 1
 
 
