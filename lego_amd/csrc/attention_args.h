@@ -9,6 +9,7 @@ struct Strides { long long batch, token, head; };
 // the score function's constants
 struct Scores {
   float scale, scale_log2;      // of q.k; times log2 e
+  float unscale;                // 1 / scale_log2
   float cap_in, cap_log2;       // 2 scale log2(e) / cap; cap log2(e)
 };
 
@@ -16,7 +17,8 @@ struct AttentionArgs {
   const void *q, *k, *v, *out, *rest, *dout;
   void *o, *o_rest, *dq, *dk, *dv;      // rest: what rounding took from out, laid out as out, or null
   float* lse;                   // [batch][head][query], natural logarithm
-  float* delta;                 // the same, of the backward pass: sum of out * dout
+  float* delta;                 // the same, of the backward pass: - sum of out * dout
+  float* less;                  // what the backward pass adds to a score: a power's exponent less log2(e) lse; with a cap that too, without one over scale_log2, as a sum starts at it
   float* ups;                   // [batch][head][tile of 64 queries]: power of two that brings the tile's largest dout to 1..2
   const float* slopes;          // [head], or null
   const int* documents;         // [batch][key], or null

@@ -9,7 +9,7 @@
 // P and dS are rounded to the operands' type, which their products take; the sums are fp32.
 // Index expressions printed from LEGO layouts:
 //   LDS tile   OrderBy(GenP((64, 16), row*16 + (chunk ^ key(row)))).TileBy([64, 16])
-//   launch     OrderBy(Col(per_xcd, 8)).TileBy([per_xcd, 8])[Row(per_xcd, 8).inv(wg)]; pid = ((batch, head), block of queries, last first)
+//   launch     Row(blocks, heads).inv(wg) = block, turn; head = OrderBy(Col(per_xcd, 8)).TileBy([per_xcd, 8])[Row(per_xcd, 8).inv(turn)]
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -94,35 +94,33 @@ struct Reader {
 };
 
 // Fills a tile from rows of memory: lane l of copy `it` of wave w fetches the 16-byte chunk that belongs into slot 64 (WAVES it + w) + l.  Chunks past
-// the head's size, rows past the last one and rows that `skip` names lie outside the descriptor, for which zeros are written.  Inline assembly, as the compiler orders
+// the head's size, rows past the last one and rows that `skip` names lie outside the descriptor, for which zeros are written (rows that share their memory with others, tokens
+// no elements apart, are read as those).  Inline assembly, as the compiler orders
 // every LDS read after all outstanding memory->LDS loads it knows of; a scalar write of M0 needs one wait state before the instruction that reads it.
 constexpr unsigned kOutside = 0x80000000u;
 struct Filler {
-  unsigned offset, step, row0, bytes;     // of this lane's first chunk; between copies; its row; a row's extent
-  __device__ __forceinline__ Filler(unsigned lane, unsigned wave, unsigned stride_bytes, unsigned head)
-  {
-    row0 = 4*wave + ((lane)/(16));
-    const unsigned chunk = ((lane % 16) ^ (wave + 4*((lane)/(16))));
-    step = (ROWS / COPIES) * stride_bytes;
-    bytes = 2 * head;
-    offset = 8 * chunk < head ? row0 * stride_bytes + 16 * chunk : kOutside;
-  }
-  // `rows` rows of the tile exist, at least one
+  const char* base;
+  unsigned stride, bytes;       // of a row
+  __device__ __forceinline__ Filler(const elt_t* base_, long long token, unsigned head)
+      : base(reinterpret_cast<const char*>(base_)), stride(2 * (unsigned)token), bytes(2 * head) {}
+  // from row `first` on, `rows` of which there are, at least one
   template <class Skip>
-  __device__ __forceinline__ void operator()(const elt_t* base, size_t first, unsigned stride_bytes, unsigned rows, unsigned lds, const Skip& skip) const
+  __device__ __forceinline__ void operator()(unsigned lane, unsigned wave, unsigned first, unsigned rows, unsigned lds, const Skip& skip) const
   {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(base) + first * stride_bytes;
-    const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
-                        (unsigned)__builtin_amdgcn_readfirstlane((min(rows, ROWS) - 1) * stride_bytes + bytes), 0x00020000u};
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base) + (size_t)first * stride;
+    const u32x4 rsrc = {(unsigned)at, (unsigned)(at >> 32), (min(rows, ROWS) - 1) * stride + bytes, 0x00020000u};
+    asm volatile("" : "+v"(lane));      // what follows from it is a few operations, and not to be kept in registers from tile to tile
+    const unsigned row0 = 4*wave + ((lane)/(16)), chunk = ((lane % 16) ^ (wave + 4*((lane)/(16))));
+    const unsigned offset = 16 * chunk < bytes ? row0 * stride + 16 * chunk : kOutside;
 #pragma unroll
     for (unsigned it = 0; it < COPIES; ++it) {
-      const unsigned row = row0 + it * (ROWS / COPIES);
-      unsigned off = offset + it * step;
-      if (row >= rows || skip(row)) off = kOutside;
+      unsigned off = offset + it * ((ROWS / COPIES) * stride);
+      if (skip(row0 + it * (ROWS / COPIES))) off = kOutside;
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds + it * (WAVES * 1024)) : "memory", "m0");
     }
   }
 };
+
 // 64 words, a statistic or a number of each row, into LDS by one wavefront; rows past the last one read as zeros
 __device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsigned lane, unsigned lds)
 {
@@ -131,6 +129,11 @@ __device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsi
                       (unsigned)__builtin_amdgcn_readfirstlane(4 * min(rows, ROWS)), 0x00020000u};
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(4 * lane), "s"(rsrc), "s"(lds) : "memory", "m0");
 }
+// The scheduler's next instructions of a kind: it would read an operand from LDS only when the one before is used, and wait for each.
+#define LEGO_MFMAS(N) __builtin_amdgcn_sched_group_barrier(0x008, N, 0)
+#define LEGO_READS(N) __builtin_amdgcn_sched_group_barrier(0x100, N, 0)
+#define LEGO_ARITHMETIC(N) __builtin_amdgcn_sched_group_barrier(0x402, N, 0)
+
 __device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Score function, in units of log2 e: what the exponential takes.  CAP: cap * tanh(scale q.k / cap) as cap (1 - 2 / (e^(2x) + 1)); its derivative by
@@ -140,18 +143,23 @@ __device__ __forceinline__ float score(float qk, const Scores& f)
 {
   if (!CAP) return f.scale_log2 * qk;
   const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
-  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+  return __builtin_fmaf(-2.0f * f.cap_log2, r, f.cap_log2);
 }
 
-// The same and the derivative of the score by scale * q.k.
+// For the backward pass with a cap: the score with `less`, which holds the cap too, added, and a quarter of its derivative by scale q.k.
 template <bool CAP>
-__device__ __forceinline__ float score(float qk, const Scores& f, float& slope)
+__device__ __forceinline__ float score(float qk, const Scores& f, float less, float& bend)
 {
-  slope = 1.0f;
-  if (!CAP) return f.scale_log2 * qk;
   const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
-  slope = 4.0f * r * (1.0f - r);
-  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+  bend = __builtin_fmaf(-r, r, r);
+  return __builtin_fmaf(-2.0f * f.cap_log2, r, less);
+}
+
+// The head of a workgroup's turn among `all`: turns go round the XCDs, heads stay on one where that comes out even.
+__device__ __forceinline__ unsigned place(unsigned turn, unsigned all)
+{
+  const unsigned per_xcd = all / 8;
+  return all % 8 ? turn : per_xcd*(turn % 8) + ((turn)/(8));
 }
 
 // What of the keys the queries of a block see.  Query i stands at position i + shift; it sees keys below limit(i), of its own document.
@@ -169,18 +177,23 @@ __device__ __forceinline__ bool same(int2 a, int2 b) { return a.x == a.y && b.x 
 constexpr unsigned kNeeded = 1, kCompare = 2, kPadded = 4;
 __device__ __forceinline__ unsigned look_at(int2 t, int2 own) { return apart(t, own) ? 0u : same(t, own) ? kNeeded : kNeeded | kCompare | (t.x < 0 ? kPadded : 0u); }
 
-// The tiles that a workgroup goes through, in order: 64 at a time are looked at, a lane each.
+// The tiles that a workgroup goes through, in order.  With documents 64 of them are looked at at a time, a lane each.
 struct Step {
   unsigned tile;                // ~0u: none is left
   bool compare, padded;         // documents have to be compared; some rows of the tile are padding
   __device__ __forceinline__ bool there() const { return tile != ~0u; }
 };
-template <class Look>
+template <bool DOCS, class Look>
 struct Walk {
   const Look& look;             // (tile) -> kNeeded, kCompare, kPadded
-  unsigned lane, base, end;
+  unsigned lane, base, end;     // base: the next tile, or the first of the 64
   unsigned long long need = 0, compare = 0, padded = 0;
-  __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin_, unsigned end_) : look(look_), lane(lane_), base(begin_), end(end_) { fetch(); }
+  __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin, unsigned end_) : look(look_), lane(lane_), end(end_) { restart(begin); }
+  __device__ __forceinline__ void restart(unsigned begin)
+  {
+    base = begin;
+    if (DOCS) fetch();
+  }
   __device__ __forceinline__ void fetch()
   {
     const unsigned tile = base + lane;
@@ -191,6 +204,7 @@ struct Walk {
   }
   __device__ __forceinline__ Step next()
   {
+    if (!DOCS) return {base < end ? base++ : ~0u, false, false};
     while (need == 0) {
       if (base + 64 >= end) return {~0u, false, false};
       base += 64;
@@ -243,74 +257,67 @@ __device__ __forceinline__ void store_columns(const float16v (&acc)[BLOCKS], elt
 
 namespace {
 
-constexpr float kShift = 0.0f;        // P is held as 2^kShift P
-constexpr float kUnshift = 1.0f / (1 << 0);
+constexpr float kUnshift = 1.0f / (1 << 0);      // P is held as P / kUnshift
+template <unsigned V> struct Constant { static constexpr unsigned value = V; };
+constexpr unsigned RING = 4;      // operands read ahead
 
-template <bool CAP, bool BIAS>
-__global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_kernel(AttentionArgs a, unsigned per_xcd)
+template <bool CAP, bool BIAS, bool DOCS>
+__global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_kernel(AttentionArgs a)
 {
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 2 * 768];      // Q and dO, twice; lse, delta and documents, twice
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
   const unsigned blocks = (a.keys + 32 * WAVES - 1) / (32 * WAVES), group = a.heads / a.key_heads, parts = group / a.heads_per_part;
-  const unsigned wg = blockIdx.x;
-  const unsigned pid = per_xcd*(wg % 8) + ((wg)/(8));
-  if (pid >= blocks * parts * a.key_heads * a.batch) return;
-  const unsigned block = pid % blocks, part = pid / blocks % parts, hk = pid / blocks / parts % a.key_heads, b = pid / blocks / parts / a.key_heads;
-  const int k0 = (int)(32 * WAVES * block), k_last = min(k0 + 32 * (int)WAVES, a.keys) - 1;
-  const int w0 = k0 + 32 * (int)wave, key = w0 + (int)l32;
+  const unsigned all_parts = parts * a.key_heads * a.batch, turn = blockIdx.x % all_parts, block = blockIdx.x / all_parts;      // earlier keys may be seen by more queries
+  const unsigned at_part = place(turn, all_parts), part = at_part % parts, hk = at_part / parts % a.key_heads, b = at_part / parts / a.key_heads;
+  const int k0 = (int)(32 * WAVES * block), k_last = min(k0 + (int)(32 * WAVES), a.keys) - 1;
+  const int w0 = k0 + (int)(32 * wave), key = w0 + (int)l32;
   const int shift = a.keys - a.queries, prefix = a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : a.keys;
+  const int first_row = a.causal && prefix == 0 ? -shift : 0;      // that sees a key
   // a query sees a key from this row on
-  const auto from = [&](int j) { return j < prefix ? INT32_MIN : j - shift; };
+  const auto from = [&](int j) { return j < prefix ? -(1 << 30) : j - shift; };
   const int from_key = from(key), from_w0 = from(w0), from_w1 = from(min(w0 + 31, a.keys - 1));
-  const int* const documents = a.documents ? a.documents + (size_t)b * a.keys : nullptr;
-  const int2* const tiles = documents ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
+  const int* const documents = DOCS ? a.documents + (size_t)b * a.keys : nullptr;
+  const int2* const tiles = DOCS ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
 
-  elt8 kv[KS], vv[KS];
+  const int own_document = DOCS ? documents[min(key, a.keys - 1)] : 0;
+  elt8 kv[KS], vv[KS];      // a key of padding is zeros, whatever it holds
   {
-    const elt_t* const krow = static_cast<const elt_t*>(a.k) + (size_t)b * a.sk.batch + (size_t)min(key, a.keys - 1) * a.sk.token + (size_t)hk * a.sk.head;
-    const elt_t* const vrow = static_cast<const elt_t*>(a.v) + (size_t)b * a.sv.batch + (size_t)min(key, a.keys - 1) * a.sv.token + (size_t)hk * a.sv.head;
+    const int j = min(key, a.keys - 1);
+    const elt_t* const krow = static_cast<const elt_t*>(a.k) + (size_t)b * a.sk.batch + (size_t)j * a.sk.token + (size_t)hk * a.sk.head;
+    const elt_t* const vrow = static_cast<const elt_t*>(a.v) + (size_t)b * a.sv.batch + (size_t)j * a.sv.token + (size_t)hk * a.sv.head;
 #pragma unroll
     for (unsigned ks = 0; ks < KS; ++ks) {
       const unsigned d = 16 * ks + 8 * lhi;
-      kv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(krow + d) : elt8{};
-      vv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(vrow + d) : elt8{};
+      kv[ks] = d < (unsigned)a.head && own_document >= 0 ? *reinterpret_cast<const elt8*>(krow + d) : elt8{};
+      vv[ks] = d < (unsigned)a.head && own_document >= 0 ? *reinterpret_cast<const elt8*>(vrow + d) : elt8{};
     }
   }
-  const int own_document = documents ? documents[min(key, a.keys - 1)] : 0;
   int2 own_tiles = {0, 0};
-  if (documents) {
+  if (DOCS) {
     own_tiles = tiles[k0 / 64];
     for (int t = k0 / 64 + 1; t <= k_last / 64; ++t) own_tiles = {min(own_tiles.x, tiles[t].x), max(own_tiles.y, tiles[t].y)};
   }
 
-  const unsigned q_stride = 2 * (unsigned)a.sq.token, do_stride = 2 * (unsigned)a.sdo.token;
-  const Filler fill_q(lane, wave, q_stride, a.head), fill_do(lane, wave, do_stride, a.head);
-  const Reader read(lane);
+  Filler fill_q(static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch, a.sq.token, a.head), fill_do(static_cast<const elt_t*>(a.dout) + (size_t)b * a.sdo.batch, a.sdo.token, a.head);
+  Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_base = (unsigned)(uintptr_t)(lds_ptr)lds, lds_at = lds_base + wave * 1024;
   const auto fill = [&](unsigned h, const Step& step, unsigned buffer) {
     const unsigned first = 64 * step.tile, rows = a.queries - first;
-    const elt_t* const qb = static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch + (size_t)h * a.sq.head;
-    const elt_t* const dob = static_cast<const elt_t*>(a.dout) + (size_t)b * a.sdo.batch + (size_t)h * a.sdo.head;
+    fill_q.base = reinterpret_cast<const char*>(static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch + (size_t)h * a.sq.head);
+    fill_do.base = reinterpret_cast<const char*>(static_cast<const elt_t*>(a.dout) + (size_t)b * a.sdo.batch + (size_t)h * a.sdo.head);
     const size_t row = ((size_t)b * a.heads + h) * a.queries + first;
     const unsigned at = lds_at + buffer * (2 * TILE), words = lds_base + 4 * TILE + buffer * 768;
-    if (wave == 0) fill_words(a.lse + row, rows, lane, words);
+    if (wave == 0) fill_words(a.less + row, rows, lane, words);
     if (wave == 1) fill_words(a.delta + row, rows, lane, words + 256);
-    if (wave == 2 && step.compare) fill_words(documents + first + shift, rows, lane, words + 512);
-    if (step.padded) {      // rows that see no key are read as zeros, whatever they hold
-      const auto skip = [&](unsigned r) { return a.lse[row + min(r, rows - 1)] == -INFINITY; };
-      fill_q(qb, first, q_stride, rows, at, skip);
-      fill_do(dob, first, do_stride, rows, at + TILE, skip);
-    } else {
-      const auto skip = [](unsigned) { return false; };
-      fill_q(qb, first, q_stride, rows, at, skip);
-      fill_do(dob, first, do_stride, rows, at + TILE, skip);
-    }
+    if (DOCS && wave == 2 && step.compare) fill_words(documents + first + shift, rows, lane, words + 512);
+    // rows that see no key, padding and those before the first key, are read as zeros, whatever they hold
+    const auto skip = [&](unsigned r) { return DOCS ? step.padded && a.lse[row + min(r, rows - 1)] == -INFINITY : (int)(first + r) < first_row; };
+    fill_q(lane, wave, first, rows, at, skip);
+    fill_do(lane, wave, first, rows, at + TILE, skip);
   };
   const auto look = [&](unsigned tile) -> unsigned {
-    const int first = (int)(64 * tile);
-    if (!documents) return first + shift < 0 && a.causal ? kNeeded | kPadded : kNeeded;      // rows before the first key
-    const int t0 = (first + shift) / 64, t1 = (min(first + 63, a.queries - 1) + shift) / 64;
+    const int first = (int)(64 * tile), t0 = (first + shift) / 64, t1 = (min(first + 63, a.queries - 1) + shift) / 64;
     return look_at(t0 == t1 ? tiles[t0] : int2{min(tiles[t0].x, tiles[t1].x), max(tiles[t0].y, tiles[t1].y)}, own_tiles);
   };
 
@@ -320,15 +327,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
   float up = 0.0f;                 // the power of two that dk carries (fp16)
   const unsigned h0 = hk * group + part * a.heads_per_part, h1 = h0 + a.heads_per_part;
   const unsigned begin = k0 < prefix ? 0u : (unsigned)max(k0 - shift, 0) / 64, end = (unsigned)(a.queries + 63) / 64;
-  typedef Walk<decltype(look)> Queries;
+  typedef Walk<DOCS, decltype(look)> Queries;
   Queries walk(look, lane, begin, end);
   unsigned h = h0;
   const auto advance = [&](unsigned& head) {      // the next tile of the heads in turn
     Step step = walk.next();
     while (!step.there() && head + 1 < h1) {
       ++head;
-      walk.base = begin;
-      walk.fetch();
+      walk.restart(begin);
       step = walk.next();
     }
     return step;
@@ -344,103 +350,165 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
     if (next.there()) fill(next_h, next, buffer ^ 1);
     const char* const qt = lds + buffer * (2 * TILE);
     const char* const dot = qt + TILE;
-    const float* const lse_s = reinterpret_cast<const float*>(lds + 4 * TILE + buffer * 768);
+    const float* const less_s = reinterpret_cast<const float*>(lds + 4 * TILE + buffer * 768);
     const int first = (int)(64 * now.tile);
-    const float slope = BIAS ? kLog2e * a.slopes[h] : 0.0f;
+    const float slope = BIAS ? (CAP ? kLog2e : kLog2e * a.scores.unscale) * a.slopes[h] : 0.0f;
     if (first + 63 >= from_w0) {
-#pragma unroll
+#pragma unroll 1
       for (unsigned qb = 0; qb < 2; ++qb) {
-        float16v s = zeros(), dp = zeros();
-#pragma unroll
-        for (unsigned ks = 0; ks < KS; ++ks) {
-          s = mfma(read.rows(qt, qb, ks), kv[ks], s);
-          dp = mfma(read.rows(dot, qb, ks), vv[ks], dp);
-        }
+        asm volatile("" : "+v"(read.row_at), "+v"(read.tr_at));      // the offsets of a step are one operation from these: they are not to be kept in registers
+        // The operands that the products read from LDS, in their order: rows of Q, of dO, then columns of dO and of Q
+        const auto operand = [&](unsigned j) {
+          if (j < 2 * KS) return read.rows(j < KS ? qt : dot, qb, j % KS);
+          const unsigned i = j - 2 * KS;
+          return read.transposed(i < 2 * DB ? dot : qt, 2 * qb + i / DB % 2, i % DB);
+        };
         // rows first + 32 qb + 8 (r / 4) + 4 lhi + r % 4
         const int row0 = first + 32 * (int)qb + 4 * (int)lhi;
         const bool edge = first + 32 * (int)qb < from_w1 || first + 32 * (int)qb + 32 > a.queries;
+        // The sums start at what is added to them: a score at -lse (and its slope) over the scale, where no cap is in between, and dP at -delta.
+        const auto lessened = [&](int g) { return *reinterpret_cast<const float4v*>(less_s + 32 * qb + 8 * g + 4 * lhi); };
+        float16v s, dp;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float4v lse = *reinterpret_cast<const float4v*>(lse_s + 32 * qb + 8 * g + 4 * lhi);
-          const float4v delta = *reinterpret_cast<const float4v*>(lse_s + 64 + 32 * qb + 8 * g + 4 * lhi);
+          const float4v x = CAP ? float4v{0.0f, 0.0f, 0.0f, 0.0f} : lessened(g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * g + e, row = row0 + 8 * g + e;
-            float bend;
-            float x = score<CAP>(s[r], a.scores, bend);
-            if (BIAS) x -= slope * fabsf((float)(row + shift - key));
-            float p = __builtin_amdgcn_exp2f(x - (kLog2e * lse[e] - kShift));
-            float ds = p * (dp[r] - delta[e]);
-            if (CAP) ds *= bend;
-            if (edge && (row < from_key || row >= a.queries)) p = ds = 0.0f;
-            s[r] = p;
-            dp[r] = ds;
-          }
+          for (int e = 0; e < 4; ++e) s[4 * g + e] = BIAS && !CAP ? x[e] - slope * fabsf((float)(row0 + 8 * g + e + shift - key)) : x[e];
         }
-        if (now.compare) {
+        elt8 ahead[RING];
+#pragma unroll
+        for (unsigned j = 0; j < RING; ++j) ahead[j] = operand(j);
+        __builtin_amdgcn_sched_barrier(0);
+        // every product has its slot, with the operand of the one RING further on and a part of the arithmetic that the products after these need
+#pragma unroll
+        for (unsigned j = 0; j < KS; ++j) {
+          s = mfma(ahead[j % RING], kv[j], s);
+          ahead[j % RING] = operand(j + RING);
+          if (j == KS - 2) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float4v d = *reinterpret_cast<const float4v*>(less_s + 64 + 32 * qb + 8 * g + 4 * lhi);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dp[4 * g + e] = d[e];
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        unsigned p_pairs[8], ds_pairs[8];      // as operands: steps of eight values
+        float4v less = CAP ? lessened(0) : float4v{};
+        float p_even = 0.0f;
+        const auto exponential = [&](int r) {
+          float x = a.scores.scale_log2 * s[r], bend = 1.0f;
+          if (CAP) {
+            x = score<CAP>(s[r], a.scores, less[r % 4], bend);
+            if (BIAS) x -= slope * fabsf((float)(row0 + 8 * (r / 4) + r % 4 + shift - key));
+            if (r % 4 == 3 && r < 15) less = lessened(r / 4 + 1);
+          }
+          const float p = __builtin_amdgcn_exp2f(x);
+          if (r % 2) p_pairs[r / 2] = pack(p_even, p);
+          else p_even = p;
+          s[r] = CAP ? p * bend : p;
+        };
+        const auto hide = [&](int r, bool seen0, bool seen1) {      // of rows r and r + 1
+          p_pairs[r / 2] &= (seen0 ? 0xffffu : 0u) | (seen1 ? 0xffff0000u : 0u);
+          s[r] = seen0 ? s[r] : 0.0f;
+          s[r + 1] = seen1 ? s[r + 1] : 0.0f;
+        };
+        const auto derivative = [&](int r) {
+          dp[r] *= s[r];
+          if (r % 2) ds_pairs[r / 2] = pack(dp[r - 1], dp[r]);
+        };
+        const auto step_of = [](const unsigned (&x)[8], unsigned st) { return __builtin_bit_cast(elt8, u32x4{x[4 * st], x[4 * st + 1], x[4 * st + 2], x[4 * st + 3]}); };
+#pragma unroll
+        for (unsigned j = KS; j < 2 * KS; ++j) {
+          dp = mfma(ahead[j % RING], vv[j - KS], dp);
+          ahead[j % RING] = operand(j + RING);
+#pragma unroll
+          for (int r = (int)(16 * (j - KS) / KS); r < (int)(16 * (j - KS + 1) / KS); ++r) exponential(r);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (edge) {
+          int begin = from_key - row0, end = a.queries - row0;
+          asm volatile("" : "+v"(begin), "+v"(end));      // a branch, and no comparisons ahead of it: most tiles have nothing to hide
+          const auto seen = [&](int r) { return 8 * (r / 4) + r % 4 >= begin && 8 * (r / 4) + r % 4 < end; };
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) hide(r, seen(r), seen(r + 1));
+        }
+        if (DOCS && now.compare) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const int4v d = *reinterpret_cast<const int4v*>(reinterpret_cast<const int*>(lse_s) + 128 + 32 * qb + 8 * g + 4 * lhi);
+            const int4v d = *reinterpret_cast<const int4v*>(reinterpret_cast<const int*>(less_s) + 128 + 32 * qb + 8 * g + 4 * lhi);
+            const auto seen = [&](int e) { return own_document >= 0 && d[e] == own_document; };
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!(own_document >= 0 && d[e] == own_document)) s[4 * g + e] = dp[4 * g + e] = 0.0f;
+            for (int e = 0; e < 4; e += 2) hide(4 * g + e, seen(e), seen(e + 1));
           }
         }
-        const Operands p = as_operands(s), ds = as_operands(dp);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (unsigned st = 0; st < 2; ++st)
+        for (unsigned j = 2 * KS; j < 2 * KS + 2 * DB; ++j) {
+          const unsigned i = j - 2 * KS;
+          dv[i % DB] = mfma(ahead[j % RING], step_of(p_pairs, i / DB), dv[i % DB]);
+          ahead[j % RING] = operand(j + RING);
 #pragma unroll
-          for (unsigned db = 0; db < DB; ++db) {
-            dv[db] = mfma(read.transposed(dot, 2 * qb + st, db), p.step[st], dv[db]);
-            dk[db] = mfma(read.transposed(qt, 2 * qb + st, db), ds.step[st], dk[db]);
-          }
+          for (int r = (int)(16 * i / (2 * DB)); r < (int)(16 * (i + 1) / (2 * DB)); ++r) derivative(r);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (unsigned j = 2 * KS + 2 * DB; j < 2 * KS + 4 * DB; ++j) {
+          const unsigned i = j - 2 * KS - 2 * DB;
+          dk[i % DB] = mfma(ahead[j % RING], step_of(ds_pairs, i / DB), dk[i % DB]);
+          if (j + RING < 2 * KS + 4 * DB) ahead[j % RING] = operand(j + RING);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
     now = next;
     h = next_h;
     buffer ^= 1;
   }
-  const float k_factor = a.scores.scale, v_factor = kUnshift;
-  if (!a.parts) {
-    const bool mine = key < a.keys;
-    store_columns<DB>(dk, mine ? static_cast<elt_t*>(a.dk) + (size_t)b * a.sdk.batch + (size_t)key * a.sdk.token + (size_t)hk * a.sdk.head : nullptr, lane, a.head, k_factor);
-    store_columns<DB>(dv, mine ? static_cast<elt_t*>(a.dv) + (size_t)b * a.sdv.batch + (size_t)key * a.sdv.token + (size_t)hk * a.sdv.head : nullptr, lane, a.head, v_factor);
-    return;
-  }
-  if (key >= a.keys) return;
-  const size_t rows = (size_t)a.batch * a.key_heads * a.keys, row = ((size_t)b * a.key_heads + hk) * a.keys + key;
-  float* const dk_at = a.parts + ((size_t)(2 * part) * rows + row) * a.head;
-  float* const dv_at = dk_at + rows * a.head;
+  const float k_factor = (CAP ? 4.0f : 1.0f) * a.scores.scale, v_factor = kUnshift;
+  {
+    const int j = key;
+    const bool mine = j < a.keys;
+    if (!a.parts) {
+      store_columns<DB>(dk, mine ? static_cast<elt_t*>(a.dk) + (size_t)b * a.sdk.batch + (size_t)j * a.sdk.token + (size_t)hk * a.sdk.head : nullptr, lane, a.head, k_factor);
+      store_columns<DB>(dv, mine ? static_cast<elt_t*>(a.dv) + (size_t)b * a.sdv.batch + (size_t)j * a.sdv.token + (size_t)hk * a.sdv.head : nullptr, lane, a.head, v_factor);
+    } else if (mine) {
+      const size_t rows = (size_t)a.batch * a.key_heads * a.keys, row = ((size_t)b * a.key_heads + hk) * a.keys + j;
+      float* const dk_at = a.parts + ((size_t)(2 * part) * rows + row) * a.head;
+      float* const dv_at = dk_at + rows * a.head;
 #pragma unroll
-  for (unsigned db = 0; db < DB; ++db)
+      for (unsigned db = 0; db < DB; ++db)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const unsigned d = 32 * db + 8 * g + 4 * lhi;
-      if (d >= (unsigned)a.head) continue;
-      *reinterpret_cast<float4v*>(dk_at + d) = float4v{k_factor * dk[db][4 * g], k_factor * dk[db][4 * g + 1], k_factor * dk[db][4 * g + 2], k_factor * dk[db][4 * g + 3]};
-      *reinterpret_cast<float4v*>(dv_at + d) = float4v{v_factor * dv[db][4 * g], v_factor * dv[db][4 * g + 1], v_factor * dv[db][4 * g + 2], v_factor * dv[db][4 * g + 3]};
+        for (int g = 0; g < 4; ++g) {
+          const unsigned d = 32 * db + 8 * g + 4 * lhi;
+          if (d >= (unsigned)a.head) continue;
+          *reinterpret_cast<float4v*>(dk_at + d) = float4v{k_factor * dk[db][4 * g], k_factor * dk[db][4 * g + 1], k_factor * dk[db][4 * g + 2], k_factor * dk[db][4 * g + 3]};
+          *reinterpret_cast<float4v*>(dv_at + d) = float4v{v_factor * dv[db][4 * g], v_factor * dv[db][4 * g + 1], v_factor * dv[db][4 * g + 2], v_factor * dv[db][4 * g + 3]};
+        }
     }
+  }
 }
 
-template <bool CAP, bool BIAS>
-__global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kernel(AttentionArgs a, unsigned per_xcd)
+template <bool CAP, bool BIAS, bool DOCS>
+__global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kernel(AttentionArgs a)
 {
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 512];      // K and V, twice; the keys' documents, twice
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
   const unsigned blocks = (a.queries + 32 * WAVES - 1) / (32 * WAVES);
-  const unsigned wg = blockIdx.x;
-  const unsigned pid = per_xcd*(wg % 8) + ((wg)/(8));
-  if (pid >= blocks * a.heads * a.batch) return;
-  const unsigned block = blocks - 1 - pid % blocks, h = pid / blocks % a.heads, b = pid / blocks / a.heads;
+  const unsigned all_heads = a.heads * a.batch, block = blocks - 1 - blockIdx.x / all_heads;      // later queries may see more keys
+  const unsigned head = place(blockIdx.x % all_heads, all_heads);
+  const unsigned h = head % a.heads, b = head / a.heads;
   const unsigned hk = h / (a.heads / a.key_heads);
   const int q0 = (int)(32 * WAVES * block), q_last = min(q0 + 32 * (int)WAVES, a.queries) - 1;
   const int w0 = q0 + 32 * (int)wave, i = w0 + (int)l32;
   const Seen seen{a.keys, a.keys - a.queries, a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : -1};
   const int limit = seen.limit(i), limit_w0 = seen.limit(w0), limit_w1 = seen.limit(min(w0 + 31, q_last));
-  const int* const documents = a.documents ? a.documents + (size_t)b * a.keys : nullptr;
-  const int2* const tiles = documents ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
+  const int* const documents = DOCS ? a.documents + (size_t)b * a.keys : nullptr;
+  const int2* const tiles = DOCS ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
   const size_t stat = ((size_t)b * a.heads + h) * a.queries + min(i, a.queries - 1);
-  const float lse = a.lse[stat], delta = a.delta[stat];
+  const bool nothing = a.lse[stat] == -INFINITY;      // a query that sees no key is zeros, whatever it holds
+  const float less = nothing ? 0.0f : a.less[stat], delta = nothing ? 0.0f : a.delta[stat];
 
   elt8 qv[KS], dov[KS];
   {
@@ -449,45 +517,39 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kern
 #pragma unroll
     for (unsigned ks = 0; ks < KS; ++ks) {
       const unsigned d = 16 * ks + 8 * lhi;
-      qv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(qrow + d) : elt8{};
-      dov[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(dorow + d) : elt8{};
+      qv[ks] = d < (unsigned)a.head && !nothing ? *reinterpret_cast<const elt8*>(qrow + d) : elt8{};
+      dov[ks] = d < (unsigned)a.head && !nothing ? *reinterpret_cast<const elt8*>(dorow + d) : elt8{};
     }
   }
-  const int own_document = documents ? documents[min(i, a.queries - 1) + seen.shift] : 0;
+  const int own_document = DOCS ? documents[min(i, a.queries - 1) + seen.shift] : 0;
   int2 own_tiles = {0, 0};
-  if (documents) {
+  if (DOCS) {
     own_tiles = tiles[(q0 + seen.shift) / 64];
     for (int t = (q0 + seen.shift) / 64 + 1; t <= (q_last + seen.shift) / 64; ++t) own_tiles = {min(own_tiles.x, tiles[t].x), max(own_tiles.y, tiles[t].y)};
   }
-  const float slope = BIAS ? kLog2e * a.slopes[h] : 0.0f;
+  const float slope = BIAS ? (CAP ? kLog2e : kLog2e * a.scores.unscale) * a.slopes[h] : 0.0f;
 
   const elt_t* const kb = static_cast<const elt_t*>(a.k) + (size_t)b * a.sk.batch + (size_t)hk * a.sk.head;
   const elt_t* const vb = static_cast<const elt_t*>(a.v) + (size_t)b * a.sv.batch + (size_t)hk * a.sv.head;
-  const unsigned k_stride = 2 * (unsigned)a.sk.token, v_stride = 2 * (unsigned)a.sv.token;
-  const Filler fill_k(lane, wave, k_stride, a.head), fill_v(lane, wave, v_stride, a.head);
-  const Reader read(lane);
+  const Filler fill_k(kb, a.sk.token, a.head), fill_v(vb, a.sv.token, a.head);
+  Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
   const auto fill = [&](const Step& step, unsigned buffer) {
     const unsigned first = 64 * step.tile, rows = a.keys - first;
     const unsigned at = lds_at + buffer * (2 * TILE);
-    if (step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + 4 * TILE + buffer * 256);
-    if (step.padded) {      // padding among the keys is read as zeros, whatever it holds
-      const auto skip = [&](unsigned row) { return documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
-      fill_k(kb, first, k_stride, rows, at, skip);
-      fill_v(vb, first, v_stride, rows, at + TILE, skip);
-    } else {
-      const auto skip = [](unsigned) { return false; };
-      fill_k(kb, first, k_stride, rows, at, skip);
-      fill_v(vb, first, v_stride, rows, at + TILE, skip);
-    }
+    if (DOCS && step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + 4 * TILE + buffer * 256);
+    // padding among the keys is read as zeros, whatever it holds
+    const auto skip = [&](unsigned row) { return DOCS && step.padded && documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
+    fill_k(lane, wave, first, rows, at, skip);
+    fill_v(lane, wave, first, rows, at + TILE, skip);
   };
-  const auto look = [&](unsigned tile) { return documents ? look_at(tiles[tile], own_tiles) : kNeeded; };
+  const auto look = [&](unsigned tile) { return look_at(tiles[tile], own_tiles); };
 
   float16v dq[DB];
 #pragma unroll
   for (unsigned db = 0; db < DB; ++db) dq[db] = zeros();
-  Walk<decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
+  Walk<DOCS, decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
   Step now = walk.next();
   unsigned buffer = 0;
   if (now.there()) fill(now, 0);
@@ -501,49 +563,98 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kern
     const int first = (int)(64 * now.tile);
     const int* const document_s = reinterpret_cast<const int*>(lds + 4 * TILE + buffer * 256);
     if (first < limit_w1) {
-#pragma unroll
-      for (unsigned kb2 = 0; kb2 < 2; ++kb2) {
-        float16v s = zeros(), dp = zeros();
-#pragma unroll
-        for (unsigned ks = 0; ks < KS; ++ks) {
-          s = mfma(read.rows(kt, kb2, ks), qv[ks], s);
-          dp = mfma(read.rows(vt, kb2, ks), dov[ks], dp);
-        }
-        const int key0 = first + (int)(32 * kb2 + 4 * lhi);
-        const bool edge = first + 32 * (int)kb2 + 32 > limit_w0;
-        const float distance0 = (float)(i + seen.shift - key0);
+asm volatile("" : "+v"(read.row_at), "+v"(read.tr_at));      // the offsets of a step are one operation from these: they are not to be kept in registers
+      // The operands that the products read from LDS, in their order: rows of K and of V for either half of the keys, then columns of K
+      const auto operand = [&](unsigned j) {
+        if (j < 4 * KS) return read.rows(j / KS % 2 ? vt : kt, j / (2 * KS), j % KS);
+        const unsigned i = j - 4 * KS;
+        return read.transposed(kt, i / DB, i % DB);
+      };
+      float16v s[2], dp[2];      // they start at what is added to them, as in the other kernel
+      const auto start = [&](int kb2, bool scores) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = key0 + 8 * (r / 4) + r % 4;
-          float bend;
-          float x = score<CAP>(s[r], a.scores, bend);
-          if (BIAS) x -= slope * fabsf(distance0 - (float)(8 * (r / 4) + r % 4));
-          const float p = __builtin_amdgcn_exp2f(x - (kLog2e * lse - kShift));
-          float ds = p * (dp[r] - delta);
-          if (CAP) ds *= bend;
-          if (edge && key >= limit) ds = 0.0f;
-          dp[r] = ds;
+          if (!scores) dp[kb2][r] = delta;
+          else s[kb2][r] = CAP ? 0.0f : BIAS ? less - slope * fabsf((float)(i + seen.shift - first - 4 * (int)lhi - (32 * kb2 + 8 * (r / 4) + r % 4))) : less;
         }
-        if (now.compare) {
+      };
+      elt8 ahead[RING];
+#pragma unroll
+      for (unsigned j = 0; j < RING; ++j) ahead[j] = operand(j);
+      __builtin_amdgcn_sched_barrier(0);
+      const auto exponential = [&](int kb2, int r) {
+        float x = a.scores.scale_log2 * s[kb2][r], bend = 1.0f;
+        if (CAP) {
+          x = score<CAP>(s[kb2][r], a.scores, less, bend);
+          if (BIAS) x -= slope * fabsf((float)(i + seen.shift - first - 4 * (int)lhi - (32 * kb2 + 8 * (r / 4) + r % 4)));
+        }
+        s[kb2][r] = __builtin_amdgcn_exp2f(x);
+        if (CAP) s[kb2][r] *= bend;
+      };
+      unsigned ds_pairs[2][8];      // as operands: steps of eight values
+      const auto derivative = [&](int kb2, int r) {
+        dp[kb2][r] *= s[kb2][r];
+        if (r % 2) ds_pairs[kb2][r / 2] = pack(dp[kb2][r - 1], dp[kb2][r]);
+      };
+      const auto step_of = [](const unsigned (&x)[8], unsigned st) { return __builtin_bit_cast(elt8, u32x4{x[4 * st], x[4 * st + 1], x[4 * st + 2], x[4 * st + 3]}); };
+      const auto hide = [&](int kb2) {
+        if (first + 32 * kb2 + 32 > limit_w0) {
+          int end = limit - first - 32 * kb2 - 4 * (int)lhi;
+          asm volatile("" : "+v"(end));      // a branch, and no comparisons ahead of it: most tiles have nothing to hide
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kb2][r] = 8 * (r / 4) + r % 4 < end ? s[kb2][r] : 0.0f;
+        }
+        if (DOCS && now.compare) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int4v d = *reinterpret_cast<const int4v*>(document_s + 32 * kb2 + 8 * g + 4 * lhi);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dp[4 * g + e] = own_document >= 0 && d[e] == own_document ? dp[4 * g + e] : 0.0f;
+            for (int e = 0; e < 4; ++e) s[kb2][4 * g + e] = own_document >= 0 && d[e] == own_document ? s[kb2][4 * g + e] : 0.0f;
           }
         }
-        const Operands ds = as_operands(dp);
+      };
+      // every product has its slot, with the operand of the one RING further on and a part of the arithmetic that the products after these need
+      const auto products = [&](auto which) {      // scores of a half of the keys, or dP of it
+        constexpr unsigned PART = decltype(which)::value, HALF = PART / 2;
+        start(HALF, PART % 2 == 0);
 #pragma unroll
-        for (unsigned st = 0; st < 2; ++st)
+        for (unsigned ks = 0; ks < KS; ++ks) {
+          constexpr unsigned j0 = PART * KS;
+          if (PART % 2 == 0) s[HALF] = mfma(ahead[(j0 + ks) % RING], qv[ks], s[HALF]);
+          else dp[HALF] = mfma(ahead[(j0 + ks) % RING], dov[ks], dp[HALF]);
+          ahead[(j0 + ks) % RING] = operand(j0 + ks + RING);
 #pragma unroll
-          for (unsigned db = 0; db < DB; ++db) dq[db] = mfma(read.transposed(kt, 2 * kb2 + st, db), ds.step[st], dq[db]);
+          for (int r = (int)(16 * ks / KS); r < (int)(16 * (ks + 1) / KS); ++r) {
+            if (PART == 2) derivative(0, r);
+            else if (PART % 2) exponential(HALF, r);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      products(Constant<0>{});
+      products(Constant<1>{});
+      hide(0);
+      products(Constant<2>{});
+      products(Constant<3>{});
+      hide(1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (unsigned j = 4 * KS; j < 4 * KS + 4 * DB; ++j) {
+        const unsigned i = j - 4 * KS;
+        dq[i % DB] = mfma(ahead[j % RING], step_of(ds_pairs[i / (2 * DB)], i / DB % 2), dq[i % DB]);
+        if (j + RING < 4 * KS + 4 * DB) ahead[j % RING] = operand(j + RING);
+        if (i < 2 * DB) {
+#pragma unroll
+          for (int r = (int)(16 * i / (2 * DB)); r < (int)(16 * (i + 1) / (2 * DB)); ++r) derivative(1, r);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     now = next;
     buffer ^= 1;
   }
   elt_t* const row = i < a.queries ? static_cast<elt_t*>(a.dq) + (size_t)b * a.sdq.batch + (size_t)i * a.sdq.token + (size_t)h * a.sdq.head : nullptr;
-  store_columns<DB>(dq, row, lane, a.head, a.scores.scale);
+  store_columns<DB>(dq, row, lane, a.head, (CAP ? 4.0f : 1.0f) * a.scores.scale);
 }
 
 }  // namespace
@@ -551,17 +662,30 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kern
 hipError_t lego_attention_bwd_bf16_d96_launch(const AttentionArgs& a, hipStream_t stream)
 {
   const auto launch = [&](auto kernel, unsigned blocks) {
-    const unsigned per_xcd = (blocks + 8 - 1) / 8;
-    hipLaunchKernelGGL(kernel, dim3(per_xcd * 8), dim3(64 * WAVES), 0, stream, a, per_xcd);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
     return hipGetLastError();
   };
   const auto both = [&](auto dkv, auto dq) {
-    const unsigned keys = (unsigned)(a.keys + 32 * WAVES - 1) / (32 * WAVES), queries = (unsigned)(a.queries + 32 * WAVES - 1) / (32 * WAVES);
-    const hipError_t e = launch(dkv, keys * (unsigned)(a.heads / a.heads_per_part) * (unsigned)a.batch);
+    const unsigned own = 32 * WAVES, keys = ((unsigned)a.keys + own - 1) / own, queries = (unsigned)(a.queries + 32 * WAVES - 1) / (32 * WAVES);
+    const unsigned blocks = keys * (unsigned)(a.heads / a.heads_per_part) * (unsigned)a.batch;
+    const hipError_t e = launch(dkv, blocks);
     return e != hipSuccess ? e : launch(dq, queries * (unsigned)a.heads * (unsigned)a.batch);
   };
-  if (a.capped && a.slopes) return both(lego_attention_dkv_bf16_d96_kernel<true, true>, lego_attention_dq_bf16_d96_kernel<true, true>);
-  if (a.capped) return both(lego_attention_dkv_bf16_d96_kernel<true, false>, lego_attention_dq_bf16_d96_kernel<true, false>);
-  if (a.slopes) return both(lego_attention_dkv_bf16_d96_kernel<false, true>, lego_attention_dq_bf16_d96_kernel<false, true>);
-  return both(lego_attention_dkv_bf16_d96_kernel<false, false>, lego_attention_dq_bf16_d96_kernel<false, false>);
+  if ((a.capped != 0) == true && (a.slopes != nullptr) == true && (a.documents != nullptr) == true)
+    return both(lego_attention_dkv_bf16_d96_kernel<true, true, true>, lego_attention_dq_bf16_d96_kernel<true, true, true>);
+  if ((a.capped != 0) == true && (a.slopes != nullptr) == true && (a.documents != nullptr) == false)
+    return both(lego_attention_dkv_bf16_d96_kernel<true, true, false>, lego_attention_dq_bf16_d96_kernel<true, true, false>);
+  if ((a.capped != 0) == true && (a.slopes != nullptr) == false && (a.documents != nullptr) == true)
+    return both(lego_attention_dkv_bf16_d96_kernel<true, false, true>, lego_attention_dq_bf16_d96_kernel<true, false, true>);
+  if ((a.capped != 0) == true && (a.slopes != nullptr) == false && (a.documents != nullptr) == false)
+    return both(lego_attention_dkv_bf16_d96_kernel<true, false, false>, lego_attention_dq_bf16_d96_kernel<true, false, false>);
+  if ((a.capped != 0) == false && (a.slopes != nullptr) == true && (a.documents != nullptr) == true)
+    return both(lego_attention_dkv_bf16_d96_kernel<false, true, true>, lego_attention_dq_bf16_d96_kernel<false, true, true>);
+  if ((a.capped != 0) == false && (a.slopes != nullptr) == true && (a.documents != nullptr) == false)
+    return both(lego_attention_dkv_bf16_d96_kernel<false, true, false>, lego_attention_dq_bf16_d96_kernel<false, true, false>);
+  if ((a.capped != 0) == false && (a.slopes != nullptr) == false && (a.documents != nullptr) == true)
+    return both(lego_attention_dkv_bf16_d96_kernel<false, false, true>, lego_attention_dq_bf16_d96_kernel<false, false, true>);
+  if ((a.capped != 0) == false && (a.slopes != nullptr) == false && (a.documents != nullptr) == false)
+    return both(lego_attention_dkv_bf16_d96_kernel<false, false, false>, lego_attention_dq_bf16_d96_kernel<false, false, false>);
+  return hipErrorInvalidValue;
 }

@@ -8,7 +8,7 @@
 // P is rounded to the operands' type for the product with V, as is everything that MFMAs of 16-bit operands take; its sum is of the unrounded values, in fp32.
 // Index expressions printed from LEGO layouts:
 //   LDS tile   OrderBy(GenP((64, 8), row*8 + (chunk ^ key(row)))).TileBy([64, 8])
-//   launch     OrderBy(Col(per_xcd, 8)).TileBy([per_xcd, 8])[Row(per_xcd, 8).inv(wg)]; pid = ((batch, head), block of queries, last first)
+//   launch     Row(blocks, heads).inv(wg) = block, turn; head = OrderBy(Col(per_xcd, 8)).TileBy([per_xcd, 8])[Row(per_xcd, 8).inv(turn)]
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -93,35 +93,33 @@ struct Reader {
 };
 
 // Fills a tile from rows of memory: lane l of copy `it` of wave w fetches the 16-byte chunk that belongs into slot 64 (WAVES it + w) + l.  Chunks past
-// the head's size, rows past the last one and rows that `skip` names lie outside the descriptor, for which zeros are written.  Inline assembly, as the compiler orders
+// the head's size, rows past the last one and rows that `skip` names lie outside the descriptor, for which zeros are written (rows that share their memory with others, tokens
+// no elements apart, are read as those).  Inline assembly, as the compiler orders
 // every LDS read after all outstanding memory->LDS loads it knows of; a scalar write of M0 needs one wait state before the instruction that reads it.
 constexpr unsigned kOutside = 0x80000000u;
 struct Filler {
-  unsigned offset, step, row0, bytes;     // of this lane's first chunk; between copies; its row; a row's extent
-  __device__ __forceinline__ Filler(unsigned lane, unsigned wave, unsigned stride_bytes, unsigned head)
-  {
-    row0 = 8*wave + ((lane)/(8));
-    const unsigned chunk = ((lane % 8) ^ ((2*wave + ((lane)/(32))) % 4 + 4*(((lane)/(16)) % 2)));
-    step = (ROWS / COPIES) * stride_bytes;
-    bytes = 2 * head;
-    offset = 8 * chunk < head ? row0 * stride_bytes + 16 * chunk : kOutside;
-  }
-  // `rows` rows of the tile exist, at least one
+  const char* base;
+  unsigned stride, bytes;       // of a row
+  __device__ __forceinline__ Filler(const elt_t* base_, long long token, unsigned head)
+      : base(reinterpret_cast<const char*>(base_)), stride(2 * (unsigned)token), bytes(2 * head) {}
+  // from row `first` on, `rows` of which there are, at least one
   template <class Skip>
-  __device__ __forceinline__ void operator()(const elt_t* base, size_t first, unsigned stride_bytes, unsigned rows, unsigned lds, const Skip& skip) const
+  __device__ __forceinline__ void operator()(unsigned lane, unsigned wave, unsigned first, unsigned rows, unsigned lds, const Skip& skip) const
   {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(base) + first * stride_bytes;
-    const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
-                        (unsigned)__builtin_amdgcn_readfirstlane((min(rows, ROWS) - 1) * stride_bytes + bytes), 0x00020000u};
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base) + (size_t)first * stride;
+    const u32x4 rsrc = {(unsigned)at, (unsigned)(at >> 32), (min(rows, ROWS) - 1) * stride + bytes, 0x00020000u};
+    asm volatile("" : "+v"(lane));      // what follows from it is a few operations, and not to be kept in registers from tile to tile
+    const unsigned row0 = 8*wave + ((lane)/(8)), chunk = ((lane % 8) ^ ((2*wave + ((lane)/(32))) % 4 + 4*(((lane)/(16)) % 2)));
+    const unsigned offset = 16 * chunk < bytes ? row0 * stride + 16 * chunk : kOutside;
 #pragma unroll
     for (unsigned it = 0; it < COPIES; ++it) {
-      const unsigned row = row0 + it * (ROWS / COPIES);
-      unsigned off = offset + it * step;
-      if (row >= rows || skip(row)) off = kOutside;
+      unsigned off = offset + it * ((ROWS / COPIES) * stride);
+      if (skip(row0 + it * (ROWS / COPIES))) off = kOutside;
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds + it * (WAVES * 1024)) : "memory", "m0");
     }
   }
 };
+
 // 64 words, a statistic or a number of each row, into LDS by one wavefront; rows past the last one read as zeros
 __device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsigned lane, unsigned lds)
 {
@@ -130,6 +128,11 @@ __device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsi
                       (unsigned)__builtin_amdgcn_readfirstlane(4 * min(rows, ROWS)), 0x00020000u};
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(4 * lane), "s"(rsrc), "s"(lds) : "memory", "m0");
 }
+// The scheduler's next instructions of a kind: it would read an operand from LDS only when the one before is used, and wait for each.
+#define LEGO_MFMAS(N) __builtin_amdgcn_sched_group_barrier(0x008, N, 0)
+#define LEGO_READS(N) __builtin_amdgcn_sched_group_barrier(0x100, N, 0)
+#define LEGO_ARITHMETIC(N) __builtin_amdgcn_sched_group_barrier(0x402, N, 0)
+
 __device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Score function, in units of log2 e: what the exponential takes.  CAP: cap * tanh(scale q.k / cap) as cap (1 - 2 / (e^(2x) + 1)); its derivative by
@@ -139,18 +142,23 @@ __device__ __forceinline__ float score(float qk, const Scores& f)
 {
   if (!CAP) return f.scale_log2 * qk;
   const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
-  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+  return __builtin_fmaf(-2.0f * f.cap_log2, r, f.cap_log2);
 }
 
-// The same and the derivative of the score by scale * q.k.
+// For the backward pass with a cap: the score with `less`, which holds the cap too, added, and a quarter of its derivative by scale q.k.
 template <bool CAP>
-__device__ __forceinline__ float score(float qk, const Scores& f, float& slope)
+__device__ __forceinline__ float score(float qk, const Scores& f, float less, float& bend)
 {
-  slope = 1.0f;
-  if (!CAP) return f.scale_log2 * qk;
   const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
-  slope = 4.0f * r * (1.0f - r);
-  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+  bend = __builtin_fmaf(-r, r, r);
+  return __builtin_fmaf(-2.0f * f.cap_log2, r, less);
+}
+
+// The head of a workgroup's turn among `all`: turns go round the XCDs, heads stay on one where that comes out even.
+__device__ __forceinline__ unsigned place(unsigned turn, unsigned all)
+{
+  const unsigned per_xcd = all / 8;
+  return all % 8 ? turn : per_xcd*(turn % 8) + ((turn)/(8));
 }
 
 // What of the keys the queries of a block see.  Query i stands at position i + shift; it sees keys below limit(i), of its own document.
@@ -168,18 +176,23 @@ __device__ __forceinline__ bool same(int2 a, int2 b) { return a.x == a.y && b.x 
 constexpr unsigned kNeeded = 1, kCompare = 2, kPadded = 4;
 __device__ __forceinline__ unsigned look_at(int2 t, int2 own) { return apart(t, own) ? 0u : same(t, own) ? kNeeded : kNeeded | kCompare | (t.x < 0 ? kPadded : 0u); }
 
-// The tiles that a workgroup goes through, in order: 64 at a time are looked at, a lane each.
+// The tiles that a workgroup goes through, in order.  With documents 64 of them are looked at at a time, a lane each.
 struct Step {
   unsigned tile;                // ~0u: none is left
   bool compare, padded;         // documents have to be compared; some rows of the tile are padding
   __device__ __forceinline__ bool there() const { return tile != ~0u; }
 };
-template <class Look>
+template <bool DOCS, class Look>
 struct Walk {
   const Look& look;             // (tile) -> kNeeded, kCompare, kPadded
-  unsigned lane, base, end;
+  unsigned lane, base, end;     // base: the next tile, or the first of the 64
   unsigned long long need = 0, compare = 0, padded = 0;
-  __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin_, unsigned end_) : look(look_), lane(lane_), base(begin_), end(end_) { fetch(); }
+  __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin, unsigned end_) : look(look_), lane(lane_), end(end_) { restart(begin); }
+  __device__ __forceinline__ void restart(unsigned begin)
+  {
+    base = begin;
+    if (DOCS) fetch();
+  }
   __device__ __forceinline__ void fetch()
   {
     const unsigned tile = base + lane;
@@ -190,6 +203,7 @@ struct Walk {
   }
   __device__ __forceinline__ Step next()
   {
+    if (!DOCS) return {base < end ? base++ : ~0u, false, false};
     while (need == 0) {
       if (base + 64 >= end) return {~0u, false, false};
       base += 64;
@@ -244,26 +258,29 @@ namespace {
 
 // A maximum rises by less than this (in units of log2) without the sums being scaled down: P stays below 2^8, which changes no relative rounding.
 constexpr float kLazy = 8.0f;
+constexpr unsigned RING = 4;      // operands read ahead
 
-template <bool CAP, bool BIAS>
-__global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kernel(AttentionArgs a, unsigned per_xcd)
+template <bool CAP, bool BIAS, bool DOCS>
+__global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kernel(AttentionArgs a)
 {
   __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 512];      // K and V, twice; the keys' documents, twice
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
   const unsigned blocks = (a.queries + 32 * WAVES - 1) / (32 * WAVES);
-  const unsigned wg = blockIdx.x;
-  const unsigned pid = per_xcd*(wg % 8) + ((wg)/(8));
-  if (pid >= blocks * a.heads * a.batch) return;
-  const unsigned block = blocks - 1 - pid % blocks, h = pid / blocks % a.heads, b = pid / blocks / a.heads;
+  const unsigned all_heads = a.heads * a.batch, block = blocks - 1 - blockIdx.x / all_heads;      // later queries may see more keys
+  const unsigned head = place(blockIdx.x % all_heads, all_heads);
+  const unsigned h = head % a.heads, b = head / a.heads;
   const unsigned hk = h / (a.heads / a.key_heads);
   const int q0 = (int)(32 * WAVES * block), q_last = min(q0 + 32 * (int)WAVES, a.queries) - 1;
   const int w0 = q0 + 32 * (int)wave;                      // the wavefront's first query
   const int i = w0 + (int)l32;                              // the lane's query
   const Seen seen{a.keys, a.keys - a.queries, a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : -1};
   const int limit = seen.limit(i), limit_w0 = seen.limit(w0), limit_w1 = seen.limit(min(w0 + 31, q_last));
-  const int* const documents = a.documents ? a.documents + (size_t)b * a.keys : nullptr;
-  const int2* const tiles = documents ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
+  const int* const documents = DOCS ? a.documents + (size_t)b * a.keys : nullptr;
+  const int2* const tiles = DOCS ? a.tiles + (size_t)b * ((a.keys + 63) / 64) : nullptr;
 
+  // Without cap and slopes the running maximum is of the products themselves, and the scale comes in with the exponential; a negative one turns the queries round.
+  constexpr bool RAW = !CAP && !BIAS;
+  const float unit = RAW ? fabsf(a.scores.scale_log2) : 1.0f, lazy = kLazy / unit;
   // a lane's query as the second operand; queries past the last one are computed as the last one is
   elt8 qv[KS];
   {
@@ -272,11 +289,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
     for (unsigned ks = 0; ks < KS; ++ks) {
       const unsigned d = 16 * ks + 8 * lhi;
       qv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(row + d) : elt8{};
+      if (RAW && a.scores.scale_log2 < 0.0f) qv[ks] = -qv[ks];
     }
   }
-  const int own_document = documents ? documents[min(i, a.queries - 1) + seen.shift] : 0;
+  const int own_document = DOCS ? documents[min(i, a.queries - 1) + seen.shift] : 0;
   int2 own_tiles = {0, 0};
-  if (documents) {
+  if (DOCS) {
     own_tiles = tiles[(q0 + seen.shift) / 64];
     for (int t = (q0 + seen.shift) / 64 + 1; t <= (q_last + seen.shift) / 64; ++t) own_tiles = {min(own_tiles.x, tiles[t].x), max(own_tiles.y, tiles[t].y)};
   }
@@ -284,32 +302,26 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
 
   const elt_t* const kb = static_cast<const elt_t*>(a.k) + (size_t)b * a.sk.batch + (size_t)hk * a.sk.head;
   const elt_t* const vb = static_cast<const elt_t*>(a.v) + (size_t)b * a.sv.batch + (size_t)hk * a.sv.head;
-  const unsigned k_stride = 2 * (unsigned)a.sk.token, v_stride = 2 * (unsigned)a.sv.token;
-  const Filler fill_k(lane, wave, k_stride, a.head), fill_v(lane, wave, v_stride, a.head);
+  const Filler fill_k(kb, a.sk.token, a.head), fill_v(vb, a.sv.token, a.head);
   const Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
   const auto fill = [&](const Step& step, unsigned buffer) {
     const unsigned first = 64 * step.tile, rows = a.keys - first;
     const unsigned at = lds_at + buffer * (2 * TILE);
-    if (step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + 4 * TILE + buffer * 256);
-    if (step.padded) {      // padding among the keys is read as zeros, whatever it holds
-      const auto skip = [&](unsigned row) { return documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
-      fill_k(kb, first, k_stride, rows, at, skip);
-      fill_v(vb, first, v_stride, rows, at + TILE, skip);
-    } else {
-      const auto skip = [](unsigned) { return false; };
-      fill_k(kb, first, k_stride, rows, at, skip);
-      fill_v(vb, first, v_stride, rows, at + TILE, skip);
-    }
+    if (DOCS && step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + 4 * TILE + buffer * 256);
+    // padding among the keys is read as zeros, whatever it holds
+    const auto skip = [&](unsigned row) { return DOCS && step.padded && documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
+    fill_k(lane, wave, first, rows, at, skip);
+    fill_v(lane, wave, first, rows, at + TILE, skip);
   };
-  const auto look = [&](unsigned tile) { return documents ? look_at(tiles[tile], own_tiles) : kNeeded; };
+  const auto look = [&](unsigned tile) { return look_at(tiles[tile], own_tiles); };
 
   float16v acc[DB];
 #pragma unroll
   for (unsigned db = 0; db < DB; ++db) acc[db] = zeros();
   float most = -INFINITY, sum = 0.0f;      // of the lane's own keys; the halves agree on `most`
-  Walk<decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
+  Walk<DOCS, decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
   Step now = walk.next();
   unsigned buffer = 0;
   if (now.there()) fill(now, 0);
@@ -328,24 +340,39 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
       for (unsigned ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (unsigned kb2 = 0; kb2 < 2; ++kb2) s[kb2] = mfma(read.rows(kt, kb2, ks), qv[ks], s[kb2]);
+      LEGO_READS(6);
+#pragma unroll
+      for (unsigned n = 0; n < KS - 3; ++n) {
+        LEGO_MFMAS(2);
+        LEGO_READS(2);
+      }
+      LEGO_MFMAS(6);
+      __builtin_amdgcn_sched_barrier(0);
+      elt8 ahead[RING];      // operands of the second products, on their way meanwhile
+#pragma unroll
+      for (unsigned j = 0; j < RING; ++j) ahead[j] = read.transposed(vt, j / DB, j % DB);
+      __builtin_amdgcn_sched_barrier(0);
       // scores of keys first + 32 kb2 + 8 (r / 4) + 4 lhi + r % 4
-      const float distance0 = (float)(i + seen.shift - first - 4 * (int)lhi);
+      if (!RAW) {
+        const float distance0 = (float)(i + seen.shift - first - 4 * (int)lhi);
 #pragma unroll
-      for (unsigned kb2 = 0; kb2 < 2; ++kb2)
+        for (unsigned kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float x = score<CAP>(s[kb2][r], a.scores);
-          if (BIAS) x -= slope * fabsf(distance0 - (float)(32 * kb2 + 8 * (r / 4) + r % 4));
-          s[kb2][r] = x;
-        }
+          for (int r = 0; r < 16; ++r) {
+            float x = score<CAP>(s[kb2][r], a.scores);
+            if (BIAS) x -= slope * fabsf(distance0 - (float)(int)(32 * kb2 + 8 * (r / 4) + r % 4));
+            s[kb2][r] = x;
+          }
+      }
       if (first + 64 > limit_w0) {
-        const int end = limit - first - 4 * (int)lhi;
+        int end = limit - first - 4 * (int)lhi;
+        asm volatile("" : "+v"(end));      // a branch, and no comparisons ahead of it: most tiles have nothing to hide
 #pragma unroll
         for (unsigned kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[kb2][r] = (int)(32 * kb2 + 8 * (r / 4) + r % 4) < end ? s[kb2][r] : -INFINITY;
       }
-      if (now.compare) {
+      if (DOCS && now.compare) {
 #pragma unroll
         for (unsigned kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
@@ -361,9 +388,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb2][r]);
       top = across_max(top);
-      if (__builtin_amdgcn_ballot_w64(top > most + kLazy) != 0) {
+      if (__builtin_amdgcn_ballot_w64(top > most + lazy) != 0) {
         // (-inf - -inf where a query has seen nothing yet: its sums are zeros, whatever they are multiplied by but not by NaN)
-        const float risen = fmaxf(most, top), factor = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most - risen);
+        const float risen = fmaxf(most, top), factor = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(unit * (most - risen));
         most = risen;
         sum *= factor;
 #pragma unroll
@@ -371,22 +398,29 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[db][r] *= factor;
       }
-      const float base = most == -INFINITY ? 0.0f : most;
+      const float base = most == -INFINITY ? 0.0f : unit * most;
+      float sums[4] = {sum, 0.0f, 0.0f, 0.0f};
+      const auto exponential = [&](unsigned kb2, int r) {
+        s[kb2][r] = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(unit, s[kb2][r], -base) : s[kb2][r] - base);
+        sums[r % 4] += s[kb2][r];
+      };
 #pragma unroll
-      for (unsigned kb2 = 0; kb2 < 2; ++kb2)
+      for (int r = 0; r < 16; ++r) exponential(0, r);
+      Operands p = as_operands(s[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      // every product has its slot, with the operand of the one RING further on and a part of what the second half of the keys needs
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[kb2][r] = __builtin_amdgcn_exp2f(s[kb2][r] - base);
-          sum += s[kb2][r];
+      for (unsigned j = 0; j < 4 * DB; ++j) {
+        if (j == 2 * DB) p = as_operands(s[1]);
+        acc[j % DB] = mfma(ahead[j % RING], p.step[j / DB % 2], acc[j % DB]);
+        if (j + RING < 4 * DB) ahead[j % RING] = read.transposed(vt, (j + RING) / DB, (j + RING) % DB);
+        if (j < 2 * DB) {
+#pragma unroll
+          for (int r = (int)(16 * j / (2 * DB)); r < (int)(16 * (j + 1) / (2 * DB)); ++r) exponential(1, r);
         }
-#pragma unroll
-      for (unsigned kb2 = 0; kb2 < 2; ++kb2) {
-        const Operands p = as_operands(s[kb2]);
-#pragma unroll
-        for (unsigned st = 0; st < 2; ++st)
-#pragma unroll
-          for (unsigned db = 0; db < DB; ++db) acc[db] = mfma(read.transposed(vt, 2 * kb2 + st, db), p.step[st], acc[db]);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
     now = next;
     buffer ^= 1;
@@ -406,7 +440,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
       for (int r = 0; r < 16; ++r) acc[db][r] -= static_cast<float>(static_cast<elt_t>(acc[db][r]));
     store_columns<DB>(acc, i < a.queries ? static_cast<elt_t*>(a.o_rest) + row_at : nullptr, lane, a.head, 1.0f);
   }
-  if (i < a.queries && lhi == 0) a.lse[((size_t)b * a.heads + h) * a.queries + i] = sum == 0.0f ? -INFINITY : kLn2 * (most + __builtin_amdgcn_logf(sum));
+  if (i < a.queries && lhi == 0) a.lse[((size_t)b * a.heads + h) * a.queries + i] = sum == 0.0f ? -INFINITY : kLn2 * (unit * most + __builtin_amdgcn_logf(sum));
 }
 
 }  // namespace
@@ -414,11 +448,17 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
 hipError_t lego_attention_fwd_f16_d64_launch(const AttentionArgs& a, hipStream_t stream)
 {
   const unsigned blocks = (unsigned)((a.queries + 32 * WAVES - 1) / (32 * WAVES)) * (unsigned)a.heads * (unsigned)a.batch;
-  const unsigned per_xcd = (blocks + 8 - 1) / 8;
   const auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(per_xcd * 8), dim3(64 * WAVES), 0, stream, a, per_xcd);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
     return hipGetLastError();
   };
-  if (a.capped) return a.slopes ? launch(lego_attention_fwd_f16_d64_kernel<true, true>) : launch(lego_attention_fwd_f16_d64_kernel<true, false>);
-  return a.slopes ? launch(lego_attention_fwd_f16_d64_kernel<false, true>) : launch(lego_attention_fwd_f16_d64_kernel<false, false>);
+  if ((a.capped != 0) == true && (a.slopes != nullptr) == true)
+    return a.documents ? launch(lego_attention_fwd_f16_d64_kernel<true, true, true>) : launch(lego_attention_fwd_f16_d64_kernel<true, true, false>);
+  if ((a.capped != 0) == true && (a.slopes != nullptr) == false)
+    return a.documents ? launch(lego_attention_fwd_f16_d64_kernel<true, false, true>) : launch(lego_attention_fwd_f16_d64_kernel<true, false, false>);
+  if ((a.capped != 0) == false && (a.slopes != nullptr) == true)
+    return a.documents ? launch(lego_attention_fwd_f16_d64_kernel<false, true, true>) : launch(lego_attention_fwd_f16_d64_kernel<false, true, false>);
+  if ((a.capped != 0) == false && (a.slopes != nullptr) == false)
+    return a.documents ? launch(lego_attention_fwd_f16_d64_kernel<false, false, true>) : launch(lego_attention_fwd_f16_d64_kernel<false, false, false>);
+  return hipErrorInvalidValue;
 }

@@ -1,6 +1,6 @@
 // generated by lego_amd (python -m lego_amd.build) -- do not edit; edit the generator
 //
-// The passes over rows beside the attention kernels: the lowest and highest document of every 64 positions; sum of out * dout of every query, with
+// The passes over rows beside the attention kernels: the lowest and highest document of every 64 positions; sum of out * dout of every query, what its scores are lessened by, with
 // the power of two that brings the largest dout of 64 queries to 1..2; and the sum of the parts of dk and dv.  Each reads its input once.
 // Index expressions printed from LEGO layouts:
 //   statistics   OrderBy(Row(batch, heads, queries)).TileBy([batch, heads, queries])[b, h, i]
@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(256) lego_attention_tiles_kernel(const int* __
 
 // 64 queries of a head a workgroup, 16 lanes a query.
 template <class E>
-__global__ void __launch_bounds__(256) lego_attention_delta_kernel(AttentionArgs a, unsigned tiles)
+__global__ void __launch_bounds__(256) lego_attention_delta_kernel(AttentionArgs a, unsigned tiles, float shift)
 {
   typedef E elt8 __attribute__((ext_vector_type(8)));
   __shared__ float largest_s[4];
@@ -60,7 +60,11 @@ __global__ void __launch_bounds__(256) lego_attention_delta_kernel(AttentionArgs
     }
 #pragma unroll
     for (int d = 8; d; d /= 2) sum += __shfl_xor(sum, d);
-    if (lane == 0 && inside) a.delta[stat] = sum;
+    if (lane == 0 && inside) {
+      a.delta[stat] = -sum;
+      const float less = shift - 1.4426950408889634f * a.lse[stat];
+      a.less[stat] = a.capped ? less + a.scores.cap_log2 : less * a.scores.unscale;
+    }
   }
 #pragma unroll
   for (int d = 32; d; d /= 2) largest = fmaxf(largest, __shfl_xor(largest, d));
@@ -113,8 +117,8 @@ hipError_t lego_attention_delta_launch(const AttentionArgs& a, int element, hipS
 {
   const unsigned tiles = ((unsigned)a.queries + 63) / 64;
   const dim3 grid(tiles * (unsigned)a.heads * (unsigned)a.batch);
-  if (element == 0) hipLaunchKernelGGL(lego_attention_delta_kernel<_Float16>, grid, dim3(256), 0, stream, a, tiles);
-  else hipLaunchKernelGGL(lego_attention_delta_kernel<__bf16>, grid, dim3(256), 0, stream, a, tiles);
+  if (element == 0) hipLaunchKernelGGL(lego_attention_delta_kernel<_Float16>, grid, dim3(256), 0, stream, a, tiles, 8.0f);
+  else hipLaunchKernelGGL(lego_attention_delta_kernel<__bf16>, grid, dim3(256), 0, stream, a, tiles, 0.0f);
   return hipGetLastError();
 }
 

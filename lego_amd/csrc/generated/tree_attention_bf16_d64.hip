@@ -94,35 +94,33 @@ struct Reader {
 };
 
 // Fills a tile from rows of memory: lane l of copy `it` of wave w fetches the 16-byte chunk that belongs into slot 64 (WAVES it + w) + l.  Chunks past
-// the head's size, rows past the last one and rows that `skip` names lie outside the descriptor, for which zeros are written.  Inline assembly, as the compiler orders
+// the head's size, rows past the last one and rows that `skip` names lie outside the descriptor, for which zeros are written (rows that share their memory with others, tokens
+// no elements apart, are read as those).  Inline assembly, as the compiler orders
 // every LDS read after all outstanding memory->LDS loads it knows of; a scalar write of M0 needs one wait state before the instruction that reads it.
 constexpr unsigned kOutside = 0x80000000u;
 struct Filler {
-  unsigned offset, step, row0, bytes;     // of this lane's first chunk; between copies; its row; a row's extent
-  __device__ __forceinline__ Filler(unsigned lane, unsigned wave, unsigned stride_bytes, unsigned head)
-  {
-    row0 = 8*wave + ((lane)/(8));
-    const unsigned chunk = ((lane % 8) ^ ((2*wave + ((lane)/(32))) % 4 + 4*(((lane)/(16)) % 2)));
-    step = (ROWS / COPIES) * stride_bytes;
-    bytes = 2 * head;
-    offset = 8 * chunk < head ? row0 * stride_bytes + 16 * chunk : kOutside;
-  }
-  // `rows` rows of the tile exist, at least one
+  const char* base;
+  unsigned stride, bytes;       // of a row
+  __device__ __forceinline__ Filler(const elt_t* base_, long long token, unsigned head)
+      : base(reinterpret_cast<const char*>(base_)), stride(2 * (unsigned)token), bytes(2 * head) {}
+  // from row `first` on, `rows` of which there are, at least one
   template <class Skip>
-  __device__ __forceinline__ void operator()(const elt_t* base, size_t first, unsigned stride_bytes, unsigned rows, unsigned lds, const Skip& skip) const
+  __device__ __forceinline__ void operator()(unsigned lane, unsigned wave, unsigned first, unsigned rows, unsigned lds, const Skip& skip) const
   {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(base) + first * stride_bytes;
-    const u32x4 rsrc = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(at >> 32)),
-                        (unsigned)__builtin_amdgcn_readfirstlane((min(rows, ROWS) - 1) * stride_bytes + bytes), 0x00020000u};
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base) + (size_t)first * stride;
+    const u32x4 rsrc = {(unsigned)at, (unsigned)(at >> 32), (min(rows, ROWS) - 1) * stride + bytes, 0x00020000u};
+    asm volatile("" : "+v"(lane));      // what follows from it is a few operations, and not to be kept in registers from tile to tile
+    const unsigned row0 = 8*wave + ((lane)/(8)), chunk = ((lane % 8) ^ ((2*wave + ((lane)/(32))) % 4 + 4*(((lane)/(16)) % 2)));
+    const unsigned offset = 16 * chunk < bytes ? row0 * stride + 16 * chunk : kOutside;
 #pragma unroll
     for (unsigned it = 0; it < COPIES; ++it) {
-      const unsigned row = row0 + it * (ROWS / COPIES);
-      unsigned off = offset + it * step;
-      if (row >= rows || skip(row)) off = kOutside;
+      unsigned off = offset + it * ((ROWS / COPIES) * stride);
+      if (skip(row0 + it * (ROWS / COPIES))) off = kOutside;
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(lds + it * (WAVES * 1024)) : "memory", "m0");
     }
   }
 };
+
 // 64 words, a statistic or a number of each row, into LDS by one wavefront; rows past the last one read as zeros
 __device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsigned lane, unsigned lds)
 {
@@ -131,6 +129,11 @@ __device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsi
                       (unsigned)__builtin_amdgcn_readfirstlane(4 * min(rows, ROWS)), 0x00020000u};
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(4 * lane), "s"(rsrc), "s"(lds) : "memory", "m0");
 }
+// The scheduler's next instructions of a kind: it would read an operand from LDS only when the one before is used, and wait for each.
+#define LEGO_MFMAS(N) __builtin_amdgcn_sched_group_barrier(0x008, N, 0)
+#define LEGO_READS(N) __builtin_amdgcn_sched_group_barrier(0x100, N, 0)
+#define LEGO_ARITHMETIC(N) __builtin_amdgcn_sched_group_barrier(0x402, N, 0)
+
 __device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Score function, in units of log2 e: what the exponential takes.  CAP: cap * tanh(scale q.k / cap) as cap (1 - 2 / (e^(2x) + 1)); its derivative by
@@ -140,18 +143,23 @@ __device__ __forceinline__ float score(float qk, const Scores& f)
 {
   if (!CAP) return f.scale_log2 * qk;
   const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
-  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+  return __builtin_fmaf(-2.0f * f.cap_log2, r, f.cap_log2);
 }
 
-// The same and the derivative of the score by scale * q.k.
+// For the backward pass with a cap: the score with `less`, which holds the cap too, added, and a quarter of its derivative by scale q.k.
 template <bool CAP>
-__device__ __forceinline__ float score(float qk, const Scores& f, float& slope)
+__device__ __forceinline__ float score(float qk, const Scores& f, float less, float& bend)
 {
-  slope = 1.0f;
-  if (!CAP) return f.scale_log2 * qk;
   const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(f.cap_in * qk) + 1.0f);
-  slope = 4.0f * r * (1.0f - r);
-  return f.cap_log2 - 2.0f * f.cap_log2 * r;
+  bend = __builtin_fmaf(-r, r, r);
+  return __builtin_fmaf(-2.0f * f.cap_log2, r, less);
+}
+
+// The head of a workgroup's turn among `all`: turns go round the XCDs, heads stay on one where that comes out even.
+__device__ __forceinline__ unsigned place(unsigned turn, unsigned all)
+{
+  const unsigned per_xcd = all / 8;
+  return all % 8 ? turn : per_xcd*(turn % 8) + ((turn)/(8));
 }
 
 // What of the keys the queries of a block see.  Query i stands at position i + shift; it sees keys below limit(i), of its own document.
@@ -169,18 +177,23 @@ __device__ __forceinline__ bool same(int2 a, int2 b) { return a.x == a.y && b.x 
 constexpr unsigned kNeeded = 1, kCompare = 2, kPadded = 4;
 __device__ __forceinline__ unsigned look_at(int2 t, int2 own) { return apart(t, own) ? 0u : same(t, own) ? kNeeded : kNeeded | kCompare | (t.x < 0 ? kPadded : 0u); }
 
-// The tiles that a workgroup goes through, in order: 64 at a time are looked at, a lane each.
+// The tiles that a workgroup goes through, in order.  With documents 64 of them are looked at at a time, a lane each.
 struct Step {
   unsigned tile;                // ~0u: none is left
   bool compare, padded;         // documents have to be compared; some rows of the tile are padding
   __device__ __forceinline__ bool there() const { return tile != ~0u; }
 };
-template <class Look>
+template <bool DOCS, class Look>
 struct Walk {
   const Look& look;             // (tile) -> kNeeded, kCompare, kPadded
-  unsigned lane, base, end;
+  unsigned lane, base, end;     // base: the next tile, or the first of the 64
   unsigned long long need = 0, compare = 0, padded = 0;
-  __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin_, unsigned end_) : look(look_), lane(lane_), base(begin_), end(end_) { fetch(); }
+  __device__ __forceinline__ Walk(const Look& look_, unsigned lane_, unsigned begin, unsigned end_) : look(look_), lane(lane_), end(end_) { restart(begin); }
+  __device__ __forceinline__ void restart(unsigned begin)
+  {
+    base = begin;
+    if (DOCS) fetch();
+  }
   __device__ __forceinline__ void fetch()
   {
     const unsigned tile = base + lane;
@@ -191,6 +204,7 @@ struct Walk {
   }
   __device__ __forceinline__ Step next()
   {
+    if (!DOCS) return {base < end ? base++ : ~0u, false, false};
     while (need == 0) {
       if (base + 64 >= end) return {~0u, false, false};
       base += 64;

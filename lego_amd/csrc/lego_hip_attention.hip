@@ -47,7 +47,8 @@ inline bool take_mask(AttentionArgs& a, float scale, float softcap, const float*
   if (!(fabsf(scale) < INFINITY) || !(softcap >= 0.0f && softcap < INFINITY) || (causal != 0 && causal != 1)) return false;
   if (!aligned4(slopes) || !aligned4(documents) || !aligned4(prefix) || (prefix && !causal) || (documents && a.keys < a.queries)) return false;
   const float log2e = 1.4426950408889634f;
-  a.scores = {scale, scale * log2e, softcap > 0.0f ? 2.0f * scale * log2e / softcap : 0.0f, softcap * log2e};
+  const float steep = fabsf(scale * log2e) < 1e-30f ? copysignf(1e-30f, scale) : scale * log2e;      // a scale of nothing: differences of nothing
+  a.scores = {scale, steep, 1.0f / steep, softcap > 0.0f ? 2.0f * scale * log2e / softcap : 0.0f, softcap * log2e};
   a.capped = softcap > 0.0f;
   a.slopes = slopes, a.documents = documents, a.prefix = prefix, a.causal = causal;
   return true;
@@ -65,17 +66,15 @@ inline int heads_per_part(const AttentionArgs& a)
   return 1;
 }
 
-struct Room { size_t tiles, delta, ups, parts, all; };
+struct Room { size_t delta, less, ups, parts, all; };
 inline Room room_of(const AttentionArgs& a, bool documents, bool backward)
 {
-  Room r = {0, 0, 0, 0, 0};
-  r.delta = documents ? tiles_bytes(a) : 0;
-  r.ups = r.delta;
-  r.parts = r.ups;
-  r.all = r.parts;
+  Room r = {};
+  r.delta = r.all = documents ? tiles_bytes(a) : 0;
   if (!backward) return r;
   const size_t rows = (size_t)a.batch * a.heads;
-  r.ups = r.delta + up16(rows * a.queries * sizeof(float));
+  r.less = r.delta + up16(rows * a.queries * sizeof(float));
+  r.ups = r.less + up16(rows * a.queries * sizeof(float));
   r.parts = r.ups + up16(rows * ((a.queries + 63) / 64) * sizeof(float));
   const int per = heads_per_part(a), parts = a.heads / a.key_heads / per;
   r.all = r.parts + (parts > 1 ? (size_t)parts * 2 * a.batch * a.key_heads * a.keys * a.head * sizeof(float) : 0);
@@ -171,7 +170,8 @@ int lego_hip_tree_attention(const void* q, const void* k, const void* v, const v
   if (a.tree_batch < 0) return kInvalid;
   if (plan.all && (!aligned16(workspace) || workspace_bytes < plan.all)) return kInvalid;
   const float log2e = 1.4426950408889634f;
-  a.scores = {scale, scale * log2e, softcap > 0.0f ? 2.0f * scale * log2e / softcap : 0.0f, softcap * log2e};
+  const float steep = fabsf(scale * log2e) < 1e-30f ? copysignf(1e-30f, scale) : scale * log2e;      // a scale of nothing: differences of nothing
+  a.scores = {scale, steep, 1.0f / steep, softcap > 0.0f ? 2.0f * scale * log2e / softcap : 0.0f, softcap * log2e};
   a.capped = softcap > 0.0f;
   a.q = q, a.k = k, a.v = v, a.k_cache = k_cache, a.v_cache = v_cache, a.o = out, a.pages = pages, a.lengths = lengths, a.tree = tree, a.slopes = slopes, a.positions = positions;
   a.sums = static_cast<float*>(workspace);
@@ -223,7 +223,7 @@ int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const
   if (!aligned16(workspace) || workspace_bytes < room.all) return kInvalid;
   char* const at = static_cast<char*>(workspace);
   a.q = q, a.k = k, a.v = v, a.out = out, a.rest = rest, a.dout = dout, a.lse = const_cast<float*>(lse), a.dq = dq, a.dk = dk, a.dv = dv;
-  a.tiles = reinterpret_cast<int2*>(at), a.delta = reinterpret_cast<float*>(at + room.delta), a.ups = reinterpret_cast<float*>(at + room.ups);
+  a.tiles = reinterpret_cast<int2*>(at), a.delta = reinterpret_cast<float*>(at + room.delta), a.less = reinterpret_cast<float*>(at + room.less), a.ups = reinterpret_cast<float*>(at + room.ups);
   a.parts = room.all > room.parts ? reinterpret_cast<float*>(at + room.parts) : nullptr;
   a.heads_per_part = heads_per_part(a);
   hipError_t e = documents ? lego_attention_tiles_launch(documents, a.tiles, a.batch, a.keys, as_stream(stream)) : hipSuccess;

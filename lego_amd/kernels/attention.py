@@ -22,6 +22,7 @@ MAX_HEAD = HEADS[-1]
 ROWS = 64
 WAVES = 4
 LAZY = 8
+PSHIFT = {"f16": 8, "bf16": 0}      # P is held as 2^PSHIFT P in the backward pass
 TREE_LEAST = 2      # tiles of a run at least
 
 
@@ -84,13 +85,15 @@ def _tile_params(head, waves):
 def emit():
     """The translation units: one per kernel, element type and computed head size."""
     units = []
-    per, wg = size("per_xcd"), idx("wg")
-    pid = code(tidy(xcd_remap(per, wg), {wg: (0, XCDS * per)}))
-    launch = f"OrderBy(Col(per_xcd, {XCDS})).TileBy([per_xcd, {XCDS}])[Row(per_xcd, {XCDS}).inv(wg)]; pid = ((batch, head), block of queries, last first)"
+    # workgroups one after the other have the same block of rows of different heads, the block with the most work first; heads whose number a multiple of XCDS allows it
+    # stay on one XCD, neighbours together
+    per, turn = size("per_xcd"), idx("turn")
+    place = code(tidy(xcd_remap(per, turn), {turn: (0, XCDS * per)}))
+    launch = f"Row(blocks, heads).inv(wg) = block, turn; head = OrderBy(Col(per_xcd, {XCDS})).TileBy([per_xcd, {XCDS}])[Row(per_xcd, {XCDS}).inv(turn)]"
     for dt, elt in ELEMENTS.items():
         for head in HEADS:
-            params = dict(_tile_params(head, WAVES), banner=BANNER, elt=elt, dt=dt, tag=f"{dt}_d{head}", pid=pid, launch_layout=launch,
-                          PSHIFT=8 if dt == "f16" else 0)
+            params = dict(_tile_params(head, WAVES), banner=BANNER, elt=elt, dt=dt, tag=f"{dt}_d{head}", place=place, launch_layout=launch,
+                          PSHIFT=PSHIFT[dt], RING=3 if head == 128 else 4)
             params["LEAST"] = TREE_LEAST
             units.append(Emitted(f"tree_attention_{dt}_d{head}.hip", template("tree_attention.hip.j2").render(**params), [f"lego_tree_{dt}_d{head}_launch"]))
             for way in ("fwd", "bwd"):
@@ -102,7 +105,7 @@ def emit():
     for name, text in (("b", "(size_t)b"), ("H", "a.heads"), ("T", "a.queries")):
         stat = re.sub(rf"\b{name}\b", text, stat)
     units.append(Emitted("attention_rows.hip", template("attention_rows.hip.j2").render(
-        banner=BANNER, stat=stat, stat_layout="OrderBy(Row(batch, heads, queries)).TileBy([batch, heads, queries])[b, h, i]",
+        banner=BANNER, stat=stat, PSHIFT=PSHIFT["f16"], stat_layout="OrderBy(Row(batch, heads, queries)).TileBy([batch, heads, queries])[b, h, i]",
         parts_layout="OrderBy(Row(parts, 2, batch, key heads, keys, head))"),
         ["lego_attention_tiles_launch", "lego_attention_delta_launch", "lego_attention_join_launch"]))
     return units, dict(HEADS=HEADS, TREE_LEAST=TREE_LEAST, MAX_HEAD=MAX_HEAD, ELEMENTS=tuple(ELEMENTS))
