@@ -60,21 +60,20 @@ struct TreeArgs {
   long long tree_batch;
   Scores scores;
   int batch, drafts, heads, key_heads, head, page, count, width;
-  int capped, whole;            // whole: a workgroup goes through all keys of its rows
+  int capped, whole;            // whole: a workgroup goes through all keys of an item
   unsigned row_blocks;          // of a key head's rows, drafts * (heads / key_heads)
-  unsigned workgroups;
+  unsigned tile;                // keys of a tile
+  unsigned runs, least;         // runs at most; tiles of a run at least
 };
 
-// Where a cached key lies: the page that holds it, or -1 where the sequence is shorter or its table names no page of the cache.
+// The page of a cached key by entry `at` of a piece of `entries` of its sequence's table: -1 where the key is not there, or the table names no page of the cache.
 static inline
 #ifdef __HIPCC__
 __host__ __device__
 #endif
-int page_of(const int* pages, unsigned width, unsigned page, unsigned count, unsigned length, unsigned key)
+int page_of(const int* table, unsigned entries, unsigned count, bool within, unsigned at)
 {
-  if (key >= length) return -1;
-  const unsigned at = key / page;
-  if (at >= width) return -1;
-  const int p = pages[at];
-  return p >= 0 && (unsigned)p < count ? p : -1;
+  if (!within || at >= entries) return -1;
+  const int page = table[at];
+  return page >= 0 && (unsigned)page < count ? page : -1;
 }

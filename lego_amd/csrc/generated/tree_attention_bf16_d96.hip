@@ -3,11 +3,9 @@
 // Attention of drafted tokens over a paged cache, bf16, up to 96 head elements: a draft sees all cached keys of its sequence and the drafts that the tree shows
 // it.  One draft a sequence is ordinary decoding.
 // Bound by memory where drafts are few: every cached key and value is read once for all drafts and all query heads that share its head.  Those are the rows of an item, 32 to a
-// wavefront; up to 32 rows leave the keys of a tile to two wavefronts, up to 64 to two pairs, more share the tile.  Sequences have any length, so the tiles of
-// all items, one after another, are dealt to the workgroups in equal runs, whatever item they belong to; an item in one run is done there, sums of one in several are joined by a second kernel,
-// in their order.  With few tiles an item a workgroup takes an item, in one launch.
-// Scores are transposed as in the forward kernel: a row to a lane of each half.  Tiles of 64 keys go from memory into LDS without passing registers, the next one on its way
-// while one is computed, the pages of the one after that looked up meanwhile.
+// wavefront.  Sequences have any length, so the tiles of all items, one after another, are dealt out in equal runs, whatever item they belong to; an item within one run is done there, the sums of one
+// in several are joined by a second kernel, in their order.  With few tiles an item a workgroup takes an item, in one launch.
+// Scores are transposed as in the forward kernel: a row to a lane of each half.  Tiles go from memory into LDS without passing registers; a piece of the sequence's table of pages is kept there too.
 // Index expressions printed from LEGO layouts:
 //   LDS tile   OrderBy(GenP((64, 16), row*16 + (chunk ^ key(row)))).TileBy([64, 16])
 
@@ -258,15 +256,16 @@ __device__ __forceinline__ void store_columns(const float16v (&acc)[BLOCKS], elt
 namespace {
 
 constexpr float kLazy = 8.0f;
+constexpr unsigned RING = 4;      // operands read ahead
 
 // Tiles of a sequence's items
-struct Sequence { unsigned b, length, cached, tiles; };
+struct Sequence { unsigned length, cached, tiles; };      // (its keys, tiles of them, and with the drafts')
 
 __device__ __forceinline__ Sequence sequence_of(const TreeArgs& a, unsigned b)
 {
-  const unsigned most = (unsigned)a.width * (unsigned)a.page;
-  const unsigned length = (unsigned)min((unsigned)max(a.lengths[b], 0), most), cached = (length + 63) / 64;
-  return {b, length, cached, cached + (a.k ? ((unsigned)a.drafts + 63) / 64 : 0u)};
+  const unsigned most = (unsigned)a.width * (unsigned)a.page, keys = a.tile;
+  const unsigned length = (unsigned)min((unsigned)max(a.lengths[b], 0), most), cached = (length + keys - 1) / keys;
+  return {length, cached, cached + (a.k ? ((unsigned)a.drafts + keys - 1) / keys : 0u)};
 }
 
 __device__ __forceinline__ unsigned scan_of_wave(unsigned x, unsigned lane)      // sum over lanes up to this one
@@ -313,13 +312,289 @@ __device__ __forceinline__ unsigned tiles_before(const TreeArgs& a, unsigned lan
   return __builtin_amdgcn_readfirstlane(sum);
 }
 
-__device__ __forceinline__ unsigned run_of(const TreeArgs& a, unsigned total) { return max(2u, (total + a.workgroups - 1) / a.workgroups); }
+__device__ __forceinline__ unsigned run_of(const TreeArgs& a, unsigned total) { return max(a.least, (total + a.runs - 1) / a.runs); }
 
-template <bool CAP, bool BIAS, unsigned RW>
-__global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tree_bf16_d96_kernel(TreeArgs a)
+// N memory->LDS instructions of this wavefront may be on their way
+template <unsigned N>
+__device__ __forceinline__ void wait_for_copies_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// what this wavefront has asked of LDS is done: a copy may go where it was read
+__device__ __forceinline__ void wait_for_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+constexpr unsigned NW = 4;                     // wavefronts of a workgroup
+constexpr unsigned PIECE = 1024;               // entries of a page table in LDS
+
+// A row of a tile, as the lane knows it that looks it up: 16-byte chunks from the base of what it lies in.
+struct Place { unsigned k, v; bool there; };
+__device__ __forceinline__ Place place_of(const TreeArgs& a, unsigned b, unsigned hk, const Sequence& seq, const int* table, unsigned piece, unsigned entries, bool cached, unsigned key)
 {
-  constexpr unsigned NW = RW == 1 ? 2 : 4, KW = NW / RW, NB = 2 / KW, FILLS = TILE / 1024 / NW;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];      // K and V, twice
+  size_t k = 0, v = 0;
+  bool there;
+  if (cached) {
+    const unsigned at = key / (unsigned)a.page, row = key - at * (unsigned)a.page;
+    const int page = page_of(table, entries, a.count, key < seq.length, at - piece);
+    there = page >= 0;
+    if (there) {
+      k = (size_t)page * a.skc.batch + (size_t)row * a.skc.token + (size_t)hk * a.skc.head;
+      v = (size_t)page * a.svc.batch + (size_t)row * a.svc.token + (size_t)hk * a.svc.head;
+    }
+  } else {
+    there = key < (unsigned)a.drafts;
+    if (there) {
+      k = (size_t)b * a.sk.batch + (size_t)key * a.sk.token + (size_t)hk * a.sk.head;
+      v = (size_t)b * a.sv.batch + (size_t)key * a.sv.token + (size_t)hk * a.sv.head;
+    }
+  }
+  return {(unsigned)(k / 8), (unsigned)(v / 8), there};
+}
+
+// Copy number g of a tile: 1 KiB of the rows' chunks.  Every instruction has all its lanes, so that each counts for one: a row that is not there reads the base's first one, and a chunk past
+// the head its row's first one, which meets zeros of Q and gives columns that nobody stores.
+__device__ __forceinline__ void copy_rows(const void* base, unsigned own, unsigned g, unsigned lane, unsigned head, unsigned lds)
+{
+  const unsigned row = 4*g + ((lane)/(16)), chunk = ((lane % 16) ^ (g % 4 + 4*((lane)/(16))));
+  const char* const from = static_cast<const char*>(base) + (size_t)__shfl(own, row) * 16 + (8 * chunk < head ? 16 * chunk : 0u);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds + g * 1024) : "memory", "m0");
+}
+
+// Up to 32 rows: a workgroup's tiles of an item are shared out among its wavefronts, and each goes through its own by itself, with no other one to wait for, in tiles of 32 keys; eight of them and more
+// on a CU keep the memory busy.  The keys of the next tile come while the products with the present values are formed, its values while those with the keys are.  The sums meet in LDS at the end.
+template <bool CAP, bool BIAS>
+__global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_bf16_d96_kernel(TreeArgs a)
+{
+  constexpr unsigned HALF = TILE / 2, FILLS = HALF / 1024;      // bytes of 32 rows; copies
+  __shared__ __attribute__((aligned(1024))) char lds[NW][2 * HALF];
+  __shared__ int pages_s[NW][PIECE / NW];
+  __shared__ float2 stats_s[NW][64];
+  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
+  const unsigned group = a.heads / a.key_heads, rows = group * a.drafts, items = a.key_heads;
+  const Reader read(lane);
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  char *const kt = lds[wave], *const vt = kt + HALF;
+  const unsigned lds_at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_ptr)lds + wave * (2 * HALF));
+  int* const table = pages_s[wave];
+  constexpr bool RAW = !CAP && !BIAS;
+  const float unit = RAW ? fabsf(a.scores.scale_log2) : 1.0f, lazy = kLazy / unit;
+
+  unsigned b, item, tile, left;      // the present sequence, item of it, tile of that; tiles of the run that are left
+  Sequence seq;
+  if (a.whole) {
+    b = blockIdx.x / items;
+    item = blockIdx.x % items;
+    seq = sequence_of(a, b);
+    tile = 0;
+    left = seq.tiles;
+  } else {
+    const unsigned total = total_tiles(a, lane, items), run = run_of(a, total), first = blockIdx.x * run;
+    if (first >= total) return;
+    left = min(run, total - first);
+    unsigned before;
+    b = find_sequence(a, lane, items, first, before);
+    seq = sequence_of(a, b);
+    item = (first - before) / seq.tiles;
+    tile = (first - before) % seq.tiles;
+  }
+
+  while (true) {
+    const unsigned hk = item, count = min(left, seq.tiles - tile), share = (count + NW - 1) / NW;      // tiles of this item, and of a wavefront
+    const unsigned own_first = tile + min(wave * share, count), last = tile + min((wave + 1) * share, count);
+    const bool mine = l32 < rows;
+    const unsigned t = min(l32, rows - 1) / group, h = hk * group + min(l32, rows - 1) % group;
+    elt8 qv[KS];
+    {
+      const elt_t* const row = static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch + (size_t)t * a.sq.token + (size_t)h * a.sq.head;
+#pragma unroll
+      for (unsigned ks = 0; ks < KS; ++ks) {
+        const unsigned d = 16 * ks + 8 * lhi;
+        qv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(row + d) : elt8{};
+        if (RAW && a.scores.scale_log2 < 0.0f) qv[ks] = -qv[ks];
+      }
+    }
+    const int* const pages = a.pages + (size_t)b * a.width;
+    const float slope = BIAS ? kLog2e * a.slopes[h] : 0.0f;
+    const int position = BIAS ? (a.positions ? a.positions[(size_t)b * a.drafts + t] : (int)(seq.length + t)) : 0;
+    const unsigned char* const shown = a.tree ? a.tree + (size_t)b * a.tree_batch + (size_t)t * a.drafts : nullptr;
+
+    unsigned piece = 0, piece_end = 0;      // entries of the table in LDS
+    const auto look_up = [&](unsigned n) __attribute__((always_inline)) {
+      const bool cached = n < seq.cached;
+      if (cached) {
+        const unsigned after = min(32 * n + 31, seq.length - 1) / (unsigned)a.page + 1;
+        if (after > piece_end) {
+          piece = 32 * n / (unsigned)a.page;
+          piece_end = min(piece + PIECE / NW, (unsigned)a.width);
+          wait_for_reads();
+          for (unsigned i = lane; i < piece_end - piece; i += 64) table[i] = pages[piece + i];
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+      return place_of(a, b, hk, seq, table, piece, piece_end - piece, cached, 32 * (cached ? n : n - seq.cached) + l32);
+    };
+    const auto fill = [&](unsigned n, unsigned own, bool values) __attribute__((always_inline)) {
+      const void* const base = n < seq.cached ? (values ? a.v_cache : a.k_cache) : (values ? a.v : a.k);
+#pragma unroll
+      for (unsigned g = 0; g < FILLS; ++g) copy_rows(base, own, g, lane, a.head, lds_at + (values ? HALF : 0));
+    };
+
+    float16v acc[DB];
+#pragma unroll
+    for (unsigned db = 0; db < DB; ++db) acc[db] = zeros();
+    float most = -INFINITY, sum = 0.0f;
+    wait_for_copies();      // nothing of what came before is counted
+    Place next = {0, 0, false};
+    if (own_first < last) {
+      next = look_up(own_first);
+      fill(own_first, next.k, false);
+      fill(own_first, next.v, true);
+    }
+    for (unsigned n = own_first; n < last; ++n) {
+      const unsigned here = (unsigned)__builtin_amdgcn_ballot_w64(next.there);
+      const bool more = n + 1 < last, cached = n < seq.cached;
+      if (more) next = look_up(n + 1);
+      wait_for_copies_but<FILLS>();
+      float16v s = zeros();
+#pragma unroll
+      for (unsigned ks = 0; ks < KS; ++ks) s = mfma(read.rows(kt, 0, ks), qv[ks], s);
+      LEGO_READS(4);
+#pragma unroll
+      for (unsigned i = 0; i < KS - 4; ++i) {
+        LEGO_MFMAS(1);
+        LEGO_READS(1);
+      }
+      LEGO_MFMAS(4);
+      __builtin_amdgcn_sched_barrier(0);
+      wait_for_reads();
+      if (more) fill(n + 1, next.k, false);
+      const int first = (int)(32 * (cached ? n : n - seq.cached));
+      if (!RAW) {
+        const float distance0 = (float)(position - first - 4 * (int)lhi);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float x = score<CAP>(s[e], a.scores);
+          if (BIAS && cached) x -= slope * fabsf(distance0 - (float)(8 * (e / 4) + e % 4));
+          s[e] = x;
+        }
+      }
+      // what of the cache's tile is not there, and what the tree hides
+      if (!cached) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j = first + 8 * (e / 4) + 4 * (int)lhi + e % 4;
+          const bool inside = j < a.drafts;
+          const bool seen = inside && (shown ? shown[inside ? j : 0] != 0 : j <= (int)t);
+          float x = s[e];
+          if (BIAS) x -= slope * fabsf((float)(position - (a.positions ? a.positions[(size_t)b * a.drafts + (inside ? j : 0)] : (int)seq.length + j)));
+          s[e] = seen ? x : -INFINITY;
+        }
+      } else if (here != ~0u) {
+        const unsigned own = here >> (4 * lhi);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = own >> (8 * (e / 4) + e % 4) & 1 ? s[e] : -INFINITY;
+      }
+      float top = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+      top = across_max(top);
+      if (__builtin_amdgcn_ballot_w64(top > most + lazy) != 0) {
+        const float risen = fmaxf(most, top), factor = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(unit * (most - risen));
+        most = risen;
+        sum *= factor;
+#pragma unroll
+        for (unsigned db = 0; db < DB; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[db][e] *= factor;
+      }
+      const float base = most == -INFINITY ? 0.0f : unit * most;
+      float sums[4] = {sum, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(unit, s[e], -base) : s[e] - base);
+        sums[e % 4] += s[e];
+      }
+      sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      const Operands p = as_operands(s);
+      if (more) wait_for_copies_but<FILLS>();
+      else wait_for_copies();
+      if (here != ~0u) {      // values that are not there are zeros: whatever was read in their place, times a P of zero
+#pragma unroll
+        for (unsigned at = lane; at < HALF / 16; at += 64)
+          if (!(here >> (at / (PITCH / 8)) & 1)) reinterpret_cast<u32x4*>(vt)[at] = u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (unsigned j = 0; j < 2 * DB; ++j) acc[j % DB] = mfma(read.transposed(vt, j / DB, j % DB), p.step[j / DB], acc[j % DB]);
+      LEGO_READS(6);
+#pragma unroll
+      for (unsigned j = 0; j < 2 * DB - 3; ++j) {
+        LEGO_MFMAS(1);
+        LEGO_READS(2);
+      }
+      LEGO_MFMAS(3);
+      __builtin_amdgcn_sched_barrier(0);
+      wait_for_reads();
+      if (more) fill(n + 1, next.v, true);
+    }
+    sum = across_sum(sum);
+    most *= unit;      // in units of log2 from here on
+    // every wavefront's sums into its own place, then each joins blocks of 32 elements of the head
+    float4v* const own = reinterpret_cast<float4v*>(lds[wave]);
+    static_assert(64 * 16 * DB * 4 <= 2 * HALF, "a wavefront's sums in its tiles' place");
+#pragma unroll
+    for (unsigned db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) own[(4 * db + g) * 64 + lane] = float4v{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+    stats_s[wave][lane] = float2{most, sum};
+    __syncthreads();
+    if (wave < DB) {
+      float all = 0.0f, factor[NW];
+      most = -INFINITY;
+#pragma unroll
+      for (unsigned w = 0; w < NW; ++w) most = fmaxf(most, stats_s[w][lane].x);
+#pragma unroll
+      for (unsigned w = 0; w < NW; ++w) {
+        const float2 o = stats_s[w][lane];
+        factor[w] = o.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(o.x - most);
+        all += factor[w] * o.y;
+      }
+      float16v joined[1] = {zeros()};
+#pragma unroll
+      for (unsigned w = 0; w < NW; ++w)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4v x = reinterpret_cast<const float4v*>(lds[w])[(4 * wave + g) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) joined[0][4 * g + e] += factor[w] * x[e];
+        }
+      if (count == seq.tiles) {
+        elt_t* const row = static_cast<elt_t*>(a.o) + (size_t)b * a.so.batch + (size_t)t * a.so.token + (size_t)h * a.so.head + 32 * wave;
+        store_columns<1>(joined, mine && 32 * wave < (unsigned)a.head ? row : nullptr, lane, a.head - min(32 * wave, (unsigned)a.head), all == 0.0f ? 0.0f : 1.0f / all);
+      } else if (mine) {      // slot: the workgroup's number and the item's, which no two parts share
+        const size_t at = ((size_t)blockIdx.x + (size_t)b * items + item) * 32 + l32;
+        if (lhi == 0 && wave == 0) a.stats[at] = float2{most, all};
+        float* const to = a.sums + at * DC + 32 * wave;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4v*>(to + 8 * g + 4 * lhi) = float4v{joined[0][4 * g], joined[0][4 * g + 1], joined[0][4 * g + 2], joined[0][4 * g + 3]};
+      }
+    }
+    left -= count;
+    if (left == 0) return;
+    __syncthreads();      // the tiles' places are free again
+    tile = 0;
+    if (++item == items) {
+      item = 0;
+      do seq = sequence_of(a, ++b);
+      while (seq.tiles == 0);
+    }
+  }
+}
+
+// More rows: wavefronts of 32 rows share tiles of 64 keys, two pairs of them or four.
+template <bool CAP, bool BIAS, unsigned RW>
+__global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d96_kernel(TreeArgs a)
+{
+  constexpr unsigned STAGES = 2, KW = RW == 4 ? 1 : 2, NB = 2 / KW, FILLS = TILE / 1024 / NW;
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * TILE];      // K and V, STAGES times
+  __shared__ int pages_s[PIECE];
+  __shared__ unsigned long long here_s[STAGES];      // the rows of a tile that are there
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
   const unsigned rw = wave % RW, kw = wave / RW;
   const unsigned group = a.heads / a.key_heads, rows = group * a.drafts, items = a.key_heads * a.row_blocks;
@@ -345,9 +620,10 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
     item = (first - before) / seq.tiles;
     tile = (first - before) % seq.tiles;
   }
+
   do {
     const unsigned hk = item / a.row_blocks, rb = item % a.row_blocks;
-    const unsigned count = min(left, seq.tiles - tile);      // tiles of this item
+    const unsigned count = min(left, seq.tiles - tile), last = tile + count;      // tiles of this item
     const unsigned r = 32 * (rb * RW + rw) + l32;             // the lane's row
     const bool mine = r < rows;
     const unsigned t = min(r, rows - 1) / group, h = hk * group + min(r, rows - 1) % group;
@@ -358,6 +634,7 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
       for (unsigned ks = 0; ks < KS; ++ks) {
         const unsigned d = 16 * ks + 8 * lhi;
         qv[ks] = d < (unsigned)a.head ? *reinterpret_cast<const elt8*>(row + d) : elt8{};
+        if (!CAP && !BIAS && a.scores.scale_log2 < 0.0f) qv[ks] = -qv[ks];
       }
     }
     const int* const pages = a.pages + (size_t)b * a.width;
@@ -365,66 +642,53 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
     const int position = BIAS ? (a.positions ? a.positions[(size_t)b * a.drafts + t] : (int)(seq.length + t)) : 0;
     const unsigned char* const shown = a.tree ? a.tree + (size_t)b * a.tree_batch + (size_t)t * a.drafts : nullptr;
 
-    // Where the rows of a tile lie, a row to a lane: 16-byte chunks from the base, ~0 for none.  One division a tile; the lanes that copy a row ask the lane that knows it.
-    struct Rows { unsigned k, v; };
-    const auto look_up = [&](unsigned n) {
-      Rows p = {~0u, ~0u};
-      if (n < seq.cached) {
-        const unsigned key = 64 * n + lane;
-        const int at = page_of(pages, a.width, a.page, a.count, seq.length, key);
-        const unsigned slot = key % (unsigned)a.page;
-        if (at >= 0)
-          p = {(unsigned)(((size_t)at * a.skc.batch + (size_t)slot * a.skc.token + (size_t)hk * a.skc.head) / 8), (unsigned)(((size_t)at * a.svc.batch + (size_t)slot * a.svc.token + (size_t)hk * a.svc.head) / 8)};
-      } else {
-        const unsigned j = 64 * (n - seq.cached) + lane;
-        if (j < (unsigned)a.drafts)
-          p = {(unsigned)(((size_t)b * a.sk.batch + (size_t)j * a.sk.token + (size_t)hk * a.sk.head) / 8), (unsigned)(((size_t)b * a.sv.batch + (size_t)j * a.sv.token + (size_t)hk * a.sv.head) / 8)};
+    unsigned piece = 0, piece_end = 0;      // entries of the table that pages_s holds
+    const auto fill = [&](unsigned n, unsigned stage) __attribute__((always_inline)) {
+      const bool cached = n < seq.cached;
+      if (cached) {
+        const unsigned after = min(64 * n + 63, seq.length - 1) / (unsigned)a.page + 1;
+        if (after > piece_end) {      // the table's next piece (uniform: all wavefronts come here together)
+          __syncthreads();
+          piece = 64 * n / (unsigned)a.page;
+          piece_end = min(piece + PIECE, (unsigned)a.width);
+          for (unsigned i = threadIdx.x; i < piece_end - piece; i += 64 * NW) pages_s[i] = pages[piece + i];
+          __syncthreads();
+        }
       }
-      return p;
-    };
-    const auto fill = [&](unsigned n, const Rows& p, unsigned buffer) {
-      const char* const kb = static_cast<const char*>(n < seq.cached ? a.k_cache : a.k);
-      const char* const vb = static_cast<const char*>(n < seq.cached ? a.v_cache : a.v);
+      const Place place = place_of(a, b, hk, seq, pages_s, piece, piece_end - piece, cached, 64 * (cached ? n : n - seq.cached) + lane);
+      const unsigned long long here = __builtin_amdgcn_ballot_w64(place.there);
+      if (threadIdx.x == 0) here_s[stage] = here;
 #pragma unroll
       for (unsigned it = 0; it < FILLS; ++it) {
-        const unsigned g = it * NW + wave, row = 4*g + ((lane)/(16)), chunk = ((lane % 16) ^ (g % 4 + 4*((lane)/(16))));
-        const unsigned k_at = __shfl(p.k, row), v_at = __shfl(p.v, row);
-        const unsigned to = buffer * (2 * TILE) + g * 1024;
-        if (k_at != ~0u && 8 * chunk < (unsigned)a.head) {
-          asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(kb + ((size_t)k_at + chunk) * 16), "s"(lds_at + to) : "memory", "m0");
-          asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(vb + ((size_t)v_at + chunk) * 16), "s"(lds_at + to + TILE) : "memory", "m0");
-        } else if (8 * chunk < DC) {      // whatever another sequence left there
-          *reinterpret_cast<u32x4*>(lds + to + lane * 16) = u32x4{0u, 0u, 0u, 0u};
-          *reinterpret_cast<u32x4*>(lds + to + TILE + lane * 16) = u32x4{0u, 0u, 0u, 0u};
-        }
+        copy_rows(cached ? a.k_cache : a.k, place.k, it * NW + wave, lane, a.head, lds_at + stage * (2 * TILE));
+        copy_rows(cached ? a.v_cache : a.v, place.v, it * NW + wave, lane, a.head, lds_at + stage * (2 * TILE) + TILE);
       }
     };
 
+    // as in the forward kernel: the running maximum is of the products themselves where nothing but the scale comes in between
+    constexpr bool RAW = !CAP && !BIAS;
+    const float unit = RAW ? fabsf(a.scores.scale_log2) : 1.0f, lazy = kLazy / unit;
     float16v acc[DB];
 #pragma unroll
     for (unsigned db = 0; db < DB; ++db) acc[db] = zeros();
     float most = -INFINITY, sum = 0.0f;
-    unsigned buffer = 0;
-    Rows next_rows = look_up(tile);
-    unsigned long long here = 0, here_next = __builtin_amdgcn_ballot_w64(next_rows.k != ~0u);
-    if (count) {
-      const Rows rows_now = next_rows;
-      if (count > 1) next_rows = look_up(tile + 1);
-      fill(tile, rows_now, 0);
-    }
-    for (unsigned n = tile; n < tile + count; ++n) {
-      here = here_next;
+    unsigned stage = 0;
+    if (tile < last) fill(tile, 0);
+    for (unsigned n = tile; n < last; ++n) {
       wait_for_copies();
       __syncthreads();
-      if (n + 1 < tile + count) {
-        const Rows rows_now = next_rows;
-        here_next = __builtin_amdgcn_ballot_w64(rows_now.k != ~0u);
-        if (n + 2 < tile + count) next_rows = look_up(n + 2);
-        fill(n + 1, rows_now, buffer ^ 1);
-      }
-      const char* const kt = lds + buffer * (2 * TILE);
-      const char* const vt = kt + TILE;
+      if (n + 1 < last) fill(n + 1, stage ^ 1);
+      char* const kt = lds + stage * (2 * TILE);
+      char* const vt = kt + TILE;
       const bool cached = n < seq.cached;
+      const unsigned long long here = (unsigned long long)__builtin_amdgcn_readfirstlane((unsigned)(here_s[stage] >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((unsigned)here_s[stage]);
+      stage ^= 1;
+      if (here != ~0ull) {      // values that are not there are zeros: whatever was read in their place, times a P of zero
+#pragma unroll
+        for (unsigned at = threadIdx.x; at < TILE / 16; at += 64 * NW)
+          if (!(here >> (at / (PITCH / 8)) & 1)) reinterpret_cast<u32x4*>(vt)[at] = u32x4{0u, 0u, 0u, 0u};
+        __syncthreads();
+      }
       const int first = (int)(64 * (cached ? n : n - seq.cached)) + (int)(32 * NB * kw);      // of this wavefront's keys
       float16v s[NB];
 #pragma unroll
@@ -433,25 +697,33 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
       for (unsigned ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (unsigned i = 0; i < NB; ++i) s[i] = mfma(read.rows(kt, NB * kw + i, ks), qv[ks], s[i]);
-      const float distance0 = (float)(position - first - 4 * (int)lhi);
+      constexpr unsigned ROW_READS = KS * NB, FIRST_READS = ROW_READS < 6 ? ROW_READS : 6;
+      LEGO_READS(FIRST_READS);
 #pragma unroll
-      for (unsigned i = 0; i < NB; ++i)
+      for (unsigned i = 0; i < (ROW_READS - FIRST_READS) / 2; ++i) {
+        LEGO_MFMAS(2);
+        LEGO_READS(2);
+      }
+      LEGO_MFMAS(FIRST_READS);
+      __builtin_amdgcn_sched_barrier(0);
+      const auto operand = [&](unsigned j) { return read.transposed(vt, 2 * NB * kw + j / DB, j % DB); };
+      elt8 ahead[RING];      // operands of the second products, on their way meanwhile
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x = score<CAP>(s[i][e], a.scores);
-          if (BIAS && cached) x -= slope * fabsf(distance0 - (float)(int)(32 * i + 8 * (e / 4) + e % 4));
-          s[i][e] = x;
-        }
-      // what of the cache's tile is not there
-      if (cached) {
-        if (here != ~0ull) {
-          const unsigned long long own = here >> (32 * NB * kw + 4 * lhi);
+      for (unsigned j = 0; j < RING; ++j) ahead[j] = operand(j);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!RAW) {
+        const float distance0 = (float)(position - first - 4 * (int)lhi);
 #pragma unroll
-          for (unsigned i = 0; i < NB; ++i)
+        for (unsigned i = 0; i < NB; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[i][e] = own >> (32 * i + 8 * (e / 4) + e % 4) & 1 ? s[i][e] : -INFINITY;
-        }
-      } else {
+          for (int e = 0; e < 16; ++e) {
+            float x = score<CAP>(s[i][e], a.scores);
+            if (BIAS && cached) x -= slope * fabsf(distance0 - (float)(int)(32 * i + 8 * (e / 4) + e % 4));
+            s[i][e] = x;
+          }
+      }
+      // what of the cache's tile is not there, and what the tree hides
+      if (!cached) {
 #pragma unroll
         for (unsigned i = 0; i < NB; ++i)
 #pragma unroll
@@ -463,6 +735,12 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
             if (BIAS) x -= slope * fabsf((float)(position - (a.positions ? a.positions[(size_t)b * a.drafts + (inside ? j : 0)] : (int)seq.length + j)));
             s[i][e] = seen ? x : -INFINITY;
           }
+      } else if (here != ~0ull) {
+        const unsigned long long own = here >> (32 * NB * kw + 4 * lhi);
+#pragma unroll
+        for (unsigned i = 0; i < NB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[i][e] = own >> (32 * i + 8 * (e / 4) + e % 4) & 1 ? s[i][e] : -INFINITY;
       }
       float top = s[0][0];
 #pragma unroll
@@ -470,8 +748,8 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, s[i][e]);
       top = across_max(top);
-      if (__builtin_amdgcn_ballot_w64(top > most + kLazy) != 0) {
-        const float risen = fmaxf(most, top), factor = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most - risen);
+      if (__builtin_amdgcn_ballot_w64(top > most + lazy) != 0) {
+        const float risen = fmaxf(most, top), factor = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(unit * (most - risen));
         most = risen;
         sum *= factor;
 #pragma unroll
@@ -479,25 +757,32 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[db][e] *= factor;
       }
-      const float base = most == -INFINITY ? 0.0f : most;
+      const float base = most == -INFINITY ? 0.0f : unit * most;
+      float sums[4] = {sum, 0.0f, 0.0f, 0.0f};
+      const auto exponential = [&](unsigned i, int e) {
+        s[i][e] = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(unit, s[i][e], -base) : s[i][e] - base);
+        sums[e % 4] += s[i][e];
+      };
 #pragma unroll
-      for (unsigned i = 0; i < NB; ++i)
+      for (int e = 0; e < 16; ++e) exponential(0, e);
+      Operands p = as_operands(s[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      // every product has its slot, with the operand of the one RING further on and a part of what the second half of the keys needs
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[i][e] = __builtin_amdgcn_exp2f(s[i][e] - base);
-          sum += s[i][e];
+      for (unsigned j = 0; j < 2 * NB * DB; ++j) {
+        if (j == 2 * DB) p = as_operands(s[NB - 1]);
+        acc[j % DB] = mfma(ahead[j % RING], p.step[j / DB % 2], acc[j % DB]);
+        if (j + RING < 2 * NB * DB) ahead[j % RING] = operand(j + RING);
+        if (NB == 2 && j < 2 * DB) {
+#pragma unroll
+          for (int e = (int)(16 * j / (2 * DB)); e < (int)(16 * (j + 1) / (2 * DB)); ++e) exponential(NB - 1, e);
         }
-#pragma unroll
-      for (unsigned i = 0; i < NB; ++i) {
-        const Operands p = as_operands(s[i]);
-#pragma unroll
-        for (unsigned st = 0; st < 2; ++st)
-#pragma unroll
-          for (unsigned db = 0; db < DB; ++db) acc[db] = mfma(read.transposed(vt, 2 * (NB * kw + i) + st, db), p.step[st], acc[db]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      buffer ^= 1;
+      sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
     sum = across_sum(sum);
+    most *= unit;      // in units of log2 from here on
     if constexpr (KW == 2) {      // the second wavefront's sums through LDS, past its tiles
       __syncthreads();
       float4v* const acc_s = reinterpret_cast<float4v*>(lds) + rw * (64 * 4 * DB);
@@ -545,7 +830,7 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
     }
     left -= count;
     if (left == 0) break;
-    __syncthreads();      // the tiles' place is free again
+    __syncthreads();      // the tiles' place and the table's are free again
     tile = 0;
     if (++item == items) {
       item = 0;
@@ -555,72 +840,71 @@ __global__ void __launch_bounds__(RW == 1 ? 128 : 256, RW == 1 ? 1 : 2) lego_tre
   } while (true);
 }
 
-// The rows of items in several runs, and of those that have no tile: a workgroup a row, DC / 4 lanes a part of its sums, the parts in turn.
-__global__ void __launch_bounds__(256) lego_tree_join_bf16_d96_kernel(TreeArgs a, unsigned block_rows)
+// The rows of items in several runs, and of those that have no tile, `share` rows of an item a workgroup: a few parts are gone through by the lanes of each row, many by teams of lanes, a row
+// after the other.  Either order is the same whenever the lengths are.
+__global__ void __launch_bounds__(256) lego_tree_join_bf16_d96_kernel(TreeArgs a, unsigned block_rows, unsigned share, unsigned chunks)
 {
   constexpr unsigned LANES = DC / 4 > 16 ? 32 : 16, TEAMS = 256 / LANES;
   __shared__ float4v sums_s[TEAMS][LANES];
-  __shared__ float2 stats_s[4];
+  __shared__ float sum_s[TEAMS], most_s[4];
   const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = threadIdx.x % LANES, team = threadIdx.x / LANES;
   const unsigned group = a.heads / a.key_heads, rows = group * a.drafts, items = a.key_heads * a.row_blocks;
-  const unsigned b = blockIdx.x / (a.key_heads * rows), hk = blockIdx.x / rows % a.key_heads, r = blockIdx.x % rows;
-  const unsigned total = total_tiles(a, lane, items), run = run_of(a, total);
-  const unsigned item = hk * a.row_blocks + r / block_rows;
-  const unsigned tiles = sequence_of(a, b).tiles, first = tiles_before(a, lane, items, b) + item * tiles;
-  const unsigned t = r / group, h = hk * group + r % group;
-  elt_t* const row = static_cast<elt_t*>(a.o) + (size_t)b * a.so.batch + (size_t)t * a.so.token + (size_t)h * a.so.head;
-  if (tiles == 0) {
-    if (threadIdx.x < (unsigned)a.head / 8) *reinterpret_cast<u32x4*>(row + 8 * threadIdx.x) = u32x4{0u, 0u, 0u, 0u};
-    return;
-  }
-  const unsigned w0 = first / run, parts = (first + tiles - 1) / run - w0 + 1;
+  const unsigned chunk = blockIdx.x % chunks, item = blockIdx.x / chunks % items, b = blockIdx.x / chunks / items;
+  const unsigned hk = item / a.row_blocks, r0 = item % a.row_blocks * block_rows;      // the item's first row
+  const unsigned begin = chunk * share, end = min(min(begin + share, block_rows), rows - r0);      // of its rows
+  if (begin >= end) return;
+  const unsigned tiles = sequence_of(a, b).tiles, total = total_tiles(a, lane, items), run = run_of(a, total), first = tiles_before(a, lane, items, b) + item * tiles;
+  const auto row_at = [&](unsigned i) {
+    const unsigned t = (r0 + i) / group, h = hk * group + (r0 + i) % group;
+    return static_cast<elt_t*>(a.o) + (size_t)b * a.so.batch + (size_t)t * a.so.token + (size_t)h * a.so.head + 4 * c;
+  };
+  const unsigned w0 = tiles ? first / run : 0, parts = tiles ? (first + tiles - 1) / run - w0 + 1 : 0;
   if (parts == 1) return;
-  const size_t place0 = ((size_t)w0 + (size_t)b * items + item) * block_rows + r % block_rows;      // parts are block_rows apart
-  float most = -INFINITY;
-  for (unsigned p = threadIdx.x; p < parts; p += 256) most = fmaxf(most, a.stats[place0 + (size_t)p * block_rows].x);
-#pragma unroll
-  for (int d = 32; d; d /= 2) most = fmaxf(most, __shfl_xor(most, d));
-  if (lane == 0) stats_s[wave].x = most;
-  __syncthreads();
-  most = fmaxf(fmaxf(stats_s[0].x, stats_s[1].x), fmaxf(stats_s[2].x, stats_s[3].x));
-  float sum = 0.0f;      // the same in every lane of a team
-  float4v x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (unsigned p = team; p < parts; p += TEAMS) {
-    const size_t place = place0 + (size_t)p * block_rows;
+  const size_t place0 = ((size_t)w0 + (size_t)b * items + item) * block_rows;      // parts are block_rows apart
+  const auto store = [&](unsigned i, float sum, const float4v& x) {
+    const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (4 * c < (unsigned)a.head) *reinterpret_cast<u32x2*>(row_at(i)) = u32x2{pack(factor * x[0], factor * x[1]), pack(factor * x[2], factor * x[3])};
+  };
+  const auto add = [&](size_t place, float most, float& sum, float4v& x) {
     const float2 stat = a.stats[place];
     const float f = stat.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat.x - most);
     sum += f * stat.y;
     if (4 * c < DC) x += f * *reinterpret_cast<const float4v*>(a.sums + place * DC + 4 * c);
-  }
-  sums_s[team][c] = x;
-  __shared__ float sum_s[TEAMS];
-  if (c == 0) sum_s[team] = sum;
-  __syncthreads();
-  if (team) return;
-#pragma unroll
-  for (unsigned i = 1; i < TEAMS; ++i) {
-    x += sums_s[i][c];
-    sum += sum_s[i];
-  }
-  const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (4 * c < (unsigned)a.head) *reinterpret_cast<u32x2*>(row + 4 * c) = u32x2{pack(factor * x[0], factor * x[1]), pack(factor * x[2], factor * x[3])};
-}
-
-template <unsigned RW>
-hipError_t launch_rows(const TreeArgs& a, hipStream_t stream)
-{
-  const auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(a.whole ? (unsigned)(a.batch * a.key_heads) * a.row_blocks : a.workgroups), dim3(RW == 1 ? 128 : 256), 0, stream, a);
-    return hipGetLastError();
   };
-  hipError_t e;
-  if (a.capped) e = a.slopes ? launch(lego_tree_bf16_d96_kernel<true, true, RW>) : launch(lego_tree_bf16_d96_kernel<true, false, RW>);
-  else e = a.slopes ? launch(lego_tree_bf16_d96_kernel<false, true, RW>) : launch(lego_tree_bf16_d96_kernel<false, false, RW>);
-  if (e != hipSuccess || a.whole) return e;
-  const unsigned all = (unsigned)(a.batch * a.heads * a.drafts);
-  hipLaunchKernelGGL(lego_tree_join_bf16_d96_kernel, dim3(all), dim3(256), 0, stream, a, 32 * RW);
-  return hipGetLastError();
+  if (parts <= 8) {
+    for (unsigned i = begin + team; i < end; i += TEAMS) {
+      float most = -INFINITY, sum = 0.0f;
+      float4v x = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (unsigned p = 0; p < parts; ++p) most = fmaxf(most, a.stats[place0 + i + (size_t)p * block_rows].x);
+#pragma unroll 2
+      for (unsigned p = 0; p < parts; ++p) add(place0 + i + (size_t)p * block_rows, most, sum, x);
+      store(i, sum, x);
+    }
+    return;
+  }
+  for (unsigned i = begin; i < end; ++i) {
+    float most = -INFINITY, sum = 0.0f;
+    float4v x = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (unsigned p = threadIdx.x; p < parts; p += 256) most = fmaxf(most, a.stats[place0 + i + (size_t)p * block_rows].x);
+#pragma unroll
+    for (int d = 32; d; d /= 2) most = fmaxf(most, __shfl_xor(most, d));
+    if (lane == 0) most_s[wave] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(most_s[0], most_s[1]), fmaxf(most_s[2], most_s[3]));
+#pragma unroll 4
+    for (unsigned p = team; p < parts; p += TEAMS) add(place0 + i + (size_t)p * block_rows, most, sum, x);
+    sums_s[team][c] = x;
+    if (c == 0) sum_s[team] = sum;
+    __syncthreads();
+    if (team == 0) {
+#pragma unroll
+      for (unsigned o = 1; o < TEAMS; ++o) {
+        x += sums_s[o][c];
+        sum += sum_s[o];
+      }
+      store(i, sum, x);
+    }
+  }
 }
 
 }  // namespace
@@ -628,5 +912,27 @@ hipError_t launch_rows(const TreeArgs& a, hipStream_t stream)
 // row_waves: wavefronts of 32 rows that share a tile, 1, 2 or 4
 hipError_t lego_tree_bf16_d96_launch(const TreeArgs& a, int row_waves, hipStream_t stream)
 {
-  return row_waves == 1 ? launch_rows<1>(a, stream) : row_waves == 2 ? launch_rows<2>(a, stream) : launch_rows<4>(a, stream);
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(a.whole ? (unsigned)(a.batch * a.key_heads) * a.row_blocks : a.runs), dim3(64 * NW), 0, stream, a);
+    return hipGetLastError();
+  };
+  hipError_t e = hipErrorInvalidValue;
+  if ((a.capped != 0) == true && (a.slopes != nullptr) == true)
+    e = row_waves == 1 ? launch(lego_tree_few_bf16_d96_kernel<true, true>)
+        : row_waves == 2 ? launch(lego_tree_many_bf16_d96_kernel<true, true, 2>) : launch(lego_tree_many_bf16_d96_kernel<true, true, 4>);
+  if ((a.capped != 0) == true && (a.slopes != nullptr) == false)
+    e = row_waves == 1 ? launch(lego_tree_few_bf16_d96_kernel<true, false>)
+        : row_waves == 2 ? launch(lego_tree_many_bf16_d96_kernel<true, false, 2>) : launch(lego_tree_many_bf16_d96_kernel<true, false, 4>);
+  if ((a.capped != 0) == false && (a.slopes != nullptr) == true)
+    e = row_waves == 1 ? launch(lego_tree_few_bf16_d96_kernel<false, true>)
+        : row_waves == 2 ? launch(lego_tree_many_bf16_d96_kernel<false, true, 2>) : launch(lego_tree_many_bf16_d96_kernel<false, true, 4>);
+  if ((a.capped != 0) == false && (a.slopes != nullptr) == false)
+    e = row_waves == 1 ? launch(lego_tree_few_bf16_d96_kernel<false, false>)
+        : row_waves == 2 ? launch(lego_tree_many_bf16_d96_kernel<false, false, 2>) : launch(lego_tree_many_bf16_d96_kernel<false, false, 4>);
+  if (e != hipSuccess || a.whole) return e;
+  // One row a workgroup while they are few, and have many parts each; 8 of many rows share the search for their parts.
+  const unsigned block = 32u * (unsigned)row_waves, rows = (unsigned)(a.drafts * (a.heads / a.key_heads)), held = rows < block ? rows : block;
+  const unsigned share = (unsigned)(a.batch * a.heads * a.drafts) <= 4096 ? 1 : 8, chunks = (held + share - 1) / share;
+  hipLaunchKernelGGL(lego_tree_join_bf16_d96_kernel, dim3((unsigned)(a.batch * a.key_heads) * a.row_blocks * chunks), dim3(256), 0, stream, a, block, share, chunks);
+  return hipGetLastError();
 }

@@ -42,13 +42,18 @@ inline bool take_sizes(AttentionArgs& a, const long long* sizes)
   return tiles * a.heads * a.batch < (1u << 30) && (unsigned __int128)a.batch * a.key_heads * a.keys * a.head < ((unsigned __int128)1 << 38);
 }
 
+inline Scores scores_of(float scale, float softcap)
+{
+  const float log2e = 1.4426950408889634f;
+  const float steep = fabsf(scale * log2e) < 1e-30f ? copysignf(1e-30f, scale) : scale * log2e;      // a scale of nothing: differences of nothing
+  return {scale, steep, 1.0f / steep, softcap > 0.0f ? 2.0f * scale * log2e / softcap : 0.0f, softcap * log2e};
+}
+
 inline bool take_mask(AttentionArgs& a, float scale, float softcap, const float* slopes, const int* documents, const int* prefix, int causal)
 {
   if (!(fabsf(scale) < INFINITY) || !(softcap >= 0.0f && softcap < INFINITY) || (causal != 0 && causal != 1)) return false;
   if (!aligned4(slopes) || !aligned4(documents) || !aligned4(prefix) || (prefix && !causal) || (documents && a.keys < a.queries)) return false;
-  const float log2e = 1.4426950408889634f;
-  const float steep = fabsf(scale * log2e) < 1e-30f ? copysignf(1e-30f, scale) : scale * log2e;      // a scale of nothing: differences of nothing
-  a.scores = {scale, steep, 1.0f / steep, softcap > 0.0f ? 2.0f * scale * log2e / softcap : 0.0f, softcap * log2e};
+  a.scores = scores_of(scale, softcap);
   a.capped = softcap > 0.0f;
   a.slopes = slopes, a.documents = documents, a.prefix = prefix, a.causal = causal;
   return true;
@@ -115,17 +120,19 @@ inline bool plan_of(TreeArgs& a, const long long* sizes, TreePlan& plan)
   plan.row_waves = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
   const unsigned block = 32 * plan.row_waves;
   a.row_blocks = (rows + block - 1) / block;
+  a.tile = plan.row_waves == 1 ? 32 : 64;
   const unsigned long long items = (unsigned long long)a.batch * a.key_heads * a.row_blocks;
-  const unsigned long long most = ((unsigned long long)a.page * a.width + 63) / 64 + ((unsigned)a.drafts + 63) / 64;
+  const unsigned long long most = ((unsigned long long)a.page * a.width + a.tile - 1) / a.tile + ((unsigned)a.drafts + a.tile - 1) / a.tile;
   if (items * most >= (1ull << 31)) return false;
-  // An item of few tiles is one workgroup's; else the tiles are dealt in equal runs to as many workgroups as the chip holds at a time, but no run is shorter than LEGO_TREE_LEAST.
-  a.whole = most <= 2 * LEGO_TREE_LEAST;
-  const unsigned long long held = a.head <= 64 ? 1024 : 512, runs = (items * most + LEGO_TREE_LEAST - 1) / LEGO_TREE_LEAST;
-  a.workgroups = (unsigned)(runs < held ? runs : held);
+  // An item of few tiles is one workgroup's; else the tiles are dealt in equal runs to as many workgroups as the chip holds at a time, but no run is shorter than a tile or two a wavefront.
+  a.least = plan.row_waves == 1 ? 2 * LEGO_TREE_LEAST : LEGO_TREE_LEAST;
+  a.whole = most <= (plan.row_waves == 1 ? 16 : 4);
+  const unsigned long long held = plan.row_waves == 1 && a.head <= 64 ? 768 : 512, runs = (items * most + a.least - 1) / a.least;
+  a.runs = (unsigned)(runs < held ? runs : held);
   plan.stats = plan.all = 0;
   if (a.whole) return true;
   const unsigned pitch = a.head <= 64 ? 64 : a.head <= 96 ? 96 : 128;
-  const size_t slots = (size_t)a.workgroups + items;
+  const size_t slots = (size_t)a.runs + items;
   plan.stats = slots * block * pitch * sizeof(float);
   plan.all = plan.stats + slots * block * sizeof(float2);
   return true;

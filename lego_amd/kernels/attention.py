@@ -23,6 +23,8 @@ ROWS = 64
 WAVES = 4
 LAZY = 8
 PSHIFT = {"f16": 8, "bf16": 0}      # P is held as 2^PSHIFT P in the backward pass
+JOIN_ROWS, JOIN_MANY, JOIN_FEW = 8, 4096, 8      # rows of a workgroup that joins parts, from how many rows on; parts that the lanes of a row go through
+TREE_PIECE = 1024      # entries of a page table in LDS
 TREE_LEAST = 2      # tiles of a run at least
 
 
@@ -94,7 +96,7 @@ def emit():
         for head in HEADS:
             params = dict(_tile_params(head, WAVES), banner=BANNER, elt=elt, dt=dt, tag=f"{dt}_d{head}", place=place, launch_layout=launch,
                           PSHIFT=PSHIFT[dt], RING=3 if head == 128 else 4)
-            params["LEAST"] = TREE_LEAST
+            params |= dict(LEAST=TREE_LEAST, JOIN_ROWS=JOIN_ROWS, JOIN_MANY=JOIN_MANY, JOIN_FEW=JOIN_FEW, PIECE=TREE_PIECE)
             units.append(Emitted(f"tree_attention_{dt}_d{head}.hip", template("tree_attention.hip.j2").render(**params), [f"lego_tree_{dt}_d{head}_launch"]))
             for way in ("fwd", "bwd"):
                 name = f"attention_{way}_{dt}_d{head}"
@@ -108,4 +110,4 @@ def emit():
         banner=BANNER, stat=stat, PSHIFT=PSHIFT["f16"], stat_layout="OrderBy(Row(batch, heads, queries)).TileBy([batch, heads, queries])[b, h, i]",
         parts_layout="OrderBy(Row(parts, 2, batch, key heads, keys, head))"),
         ["lego_attention_tiles_launch", "lego_attention_delta_launch", "lego_attention_join_launch"]))
-    return units, dict(HEADS=HEADS, TREE_LEAST=TREE_LEAST, MAX_HEAD=MAX_HEAD, ELEMENTS=tuple(ELEMENTS))
+    return units, dict(HEADS=HEADS, TREE_LEAST=TREE_LEAST, JOIN_ROWS=JOIN_ROWS, JOIN_MANY=JOIN_MANY, JOIN_FEW=JOIN_FEW, MAX_HEAD=MAX_HEAD, ELEMENTS=tuple(ELEMENTS))

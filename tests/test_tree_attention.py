@@ -275,17 +275,15 @@ typedef struct { int x, y; } int2; typedef struct { float x, y; } float2;
 #define HIP_INCLUDE_HIP_HIP_RUNTIME_H
 #include <stdint.h>
 ''' + (CSRC / "attention_args.h").read_text().replace("#include <hip/hip_runtime.h>", "").replace("#pragma once", "") + '''
-extern "C" int lookup(const int* p, unsigned w, unsigned s, unsigned c, unsigned n, unsigned k) { return page_of(p, w, s, c, n, k); }
+extern "C" int lookup(const int* p, unsigned n, unsigned c, bool w, unsigned at) { return page_of(p, n, c, w, at); }
 ''')
     lib = tmp_path / "p.so"
     subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-o", str(lib), str(tmp_path / "p.cpp")], check=True, capture_output=True)
     look = ctypes.CDLL(str(lib)).lookup
-    table = (ctypes.c_int * 4)(5, -1, 9, 10)
-    for key in range(200):
-        got = look(table, 4, 16, 10, 60, key)
-        want = -1 if key >= 60 or key // 16 in (1, 3) else table[key // 16]
-        assert got == want, key
-    assert look(table, 1, 16, 10, 60, 16) == -1 and look(table, 1, 16, 10, 60, 0xffffffff) == -1 and look(table, 4, 1 << 30, 10, 1 << 31, 5) == 5
+    look.argtypes = [ctypes.POINTER(ctypes.c_int), ctypes.c_uint, ctypes.c_uint, ctypes.c_bool, ctypes.c_uint]
+    table = (ctypes.c_int * 5)(5, -1, 9, 10, 1 << 30)
+    assert [look(table, 5, 10, True, at) for at in range(5)] == [5, -1, 9, -1, -1]
+    assert look(table, 5, 10, False, 0) == -1 and look(table, 2, 10, True, 2) == -1 and look(table, 5, 10, True, 0xffffffff) == -1
 
 
 def test_refusals_of_the_entry_points():
