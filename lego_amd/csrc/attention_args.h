@@ -64,14 +64,27 @@ struct TreeArgs {
   unsigned row_blocks;          // of a key head's rows, drafts * (heads / key_heads)
   unsigned tile;                // keys of a tile
   unsigned runs, least;         // runs at most; tiles of a run at least
+  unsigned page_factor, page_shift;
 };
 
-// The page of a cached key by entry `at` of a piece of `entries` of its sequence's table: -1 where the key is not there, or the table names no page of the cache.
-static inline
 #ifdef __HIPCC__
-__host__ __device__
+#define LEGO_HOST_DEVICE __host__ __device__
+#else
+#define LEGO_HOST_DEVICE
 #endif
-int page_of(const int* table, unsigned entries, unsigned count, bool within, unsigned at)
+
+// Quotients by the page's tokens, of whole numbers below 2^31, as one product and a shift: with 2^l the first power of two that is not below the divisor, the factor ceil(2^(31 + l) / divisor) is off by
+// less than 2^l / divisor ulps of 2^-31, which below 2^31 never reaches the next whole quotient; and it is below 2^32.
+static inline void quotients_by(unsigned divisor, unsigned& factor, unsigned& shift)
+{
+  shift = 31;
+  while ((1ull << (shift - 31)) < divisor) ++shift;
+  factor = (unsigned)(((unsigned __int128)1 << shift) / divisor + ((((unsigned __int128)1 << shift) % divisor) != 0));
+}
+static inline LEGO_HOST_DEVICE unsigned quotient(unsigned x, unsigned factor, unsigned shift) { return (unsigned)(((unsigned long long)x * factor) >> shift); }
+
+// The page of a cached key by entry `at` of a piece of `entries` of its sequence's table: -1 where the key is not there, or the table names no page of the cache.
+static inline LEGO_HOST_DEVICE int page_of(const int* table, unsigned entries, unsigned count, bool within, unsigned at)
 {
   if (!within || at >= entries) return -1;
   const int page = table[at];

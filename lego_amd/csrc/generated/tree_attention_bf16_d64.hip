@@ -327,32 +327,35 @@ constexpr unsigned PIECE = 1024;               // entries of a page table in LDS
 struct Place { unsigned k, v; bool there; };
 __device__ __forceinline__ Place place_of(const TreeArgs& a, unsigned b, unsigned hk, const Sequence& seq, const int* table, unsigned piece, unsigned entries, bool cached, unsigned key)
 {
-  size_t k = 0, v = 0;
+  // 32 bits of every product are enough: they are all that is left of the sum in 16-byte chunks, which lies in what the strides reach
+  unsigned k = 0, v = 0;
   bool there;
+  const auto chunks = [](long long elements) { return (unsigned)(elements >> 3); };
   if (cached) {
-    const unsigned at = key / (unsigned)a.page, row = key - at * (unsigned)a.page;
+    const unsigned at = quotient(key, a.page_factor, a.page_shift), row = key - at * (unsigned)a.page;
     const int page = page_of(table, entries, a.count, key < seq.length, at - piece);
     there = page >= 0;
     if (there) {
-      k = (size_t)page * a.skc.batch + (size_t)row * a.skc.token + (size_t)hk * a.skc.head;
-      v = (size_t)page * a.svc.batch + (size_t)row * a.svc.token + (size_t)hk * a.svc.head;
+      k = (unsigned)page * chunks(a.skc.batch) + row * chunks(a.skc.token) + hk * chunks(a.skc.head);
+      v = (unsigned)page * chunks(a.svc.batch) + row * chunks(a.svc.token) + hk * chunks(a.svc.head);
     }
   } else {
     there = key < (unsigned)a.drafts;
     if (there) {
-      k = (size_t)b * a.sk.batch + (size_t)key * a.sk.token + (size_t)hk * a.sk.head;
-      v = (size_t)b * a.sv.batch + (size_t)key * a.sv.token + (size_t)hk * a.sv.head;
+      k = b * chunks(a.sk.batch) + key * chunks(a.sk.token) + hk * chunks(a.sk.head);
+      v = b * chunks(a.sv.batch) + key * chunks(a.sv.token) + hk * chunks(a.sv.head);
     }
   }
-  return {(unsigned)(k / 8), (unsigned)(v / 8), there};
+  return {k, v, there};
 }
 
 // Copy number g of a tile: 1 KiB of the rows' chunks.  Every instruction has all its lanes, so that each counts for one: a row that is not there reads the base's first one, and a chunk past
-// the head its row's first one, which meets zeros of Q and gives columns that nobody stores.
-__device__ __forceinline__ void copy_rows(const void* base, unsigned own, unsigned g, unsigned lane, unsigned head, unsigned lds)
+// the head its row's first one, which meets zeros of Q and gives columns that nobody stores.  The lane's row of the copy is asked for (row_of_copy) well before its place is used.
+__device__ __forceinline__ unsigned row_of_copy(unsigned own, unsigned g, unsigned lane) { return __shfl(own, 8*g + ((lane)/(8))); }
+__device__ __forceinline__ void copy_row(const void* base, unsigned at, unsigned g, unsigned lane, unsigned head, unsigned lds)
 {
-  const unsigned row = 8*g + ((lane)/(8)), chunk = ((lane % 8) ^ ((2*g + ((lane)/(32))) % 4 + 4*(((lane)/(16)) % 2)));
-  const char* const from = static_cast<const char*>(base) + (size_t)__shfl(own, row) * 16 + (8 * chunk < head ? 16 * chunk : 0u);
+  const unsigned chunk = ((lane % 8) ^ ((2*g + ((lane)/(32))) % 4 + 4*(((lane)/(16)) % 2)));
+  const char* const from = static_cast<const char*>(base) + (size_t)at * 16 + (8 * chunk < head ? 16 * chunk : 0u);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds + g * 1024) : "memory", "m0");
 }
 
@@ -415,24 +418,28 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_bf16_d64_kernel(Tree
     const unsigned char* const shown = a.tree ? a.tree + (size_t)b * a.tree_batch + (size_t)t * a.drafts : nullptr;
 
     unsigned piece = 0, piece_end = 0;      // entries of the table in LDS
+    unsigned next_k[FILLS], next_v[FILLS], next_here = 0;      // of the next tile: the lane's rows, and which there are
     const auto look_up = [&](unsigned n) __attribute__((always_inline)) {
       const bool cached = n < seq.cached;
       if (cached) {
-        const unsigned after = min(32 * n + 31, seq.length - 1) / (unsigned)a.page + 1;
+        const unsigned after = quotient(min(32 * n + 31, seq.length - 1), a.page_factor, a.page_shift) + 1;
         if (after > piece_end) {
-          piece = 32 * n / (unsigned)a.page;
+          piece = quotient(32 * n, a.page_factor, a.page_shift);
           piece_end = min(piece + PIECE / NW, (unsigned)a.width);
           wait_for_reads();
           for (unsigned i = lane; i < piece_end - piece; i += 64) table[i] = pages[piece + i];
           __builtin_amdgcn_wave_barrier();
         }
       }
-      return place_of(a, b, hk, seq, table, piece, piece_end - piece, cached, 32 * (cached ? n : n - seq.cached) + l32);
+      const Place place = place_of(a, b, hk, seq, table, piece, piece_end - piece, cached, 32 * (cached ? n : n - seq.cached) + l32);
+      next_here = (unsigned)__builtin_amdgcn_ballot_w64(place.there);
+#pragma unroll
+      for (unsigned g = 0; g < FILLS; ++g) next_k[g] = row_of_copy(place.k, g, lane), next_v[g] = row_of_copy(place.v, g, lane);
     };
-    const auto fill = [&](unsigned n, unsigned own, bool values) __attribute__((always_inline)) {
+    const auto fill = [&](unsigned n, const unsigned* from, bool values) __attribute__((always_inline)) {
       const void* const base = n < seq.cached ? (values ? a.v_cache : a.k_cache) : (values ? a.v : a.k);
 #pragma unroll
-      for (unsigned g = 0; g < FILLS; ++g) copy_rows(base, own, g, lane, a.head, lds_at + (values ? HALF : 0));
+      for (unsigned g = 0; g < FILLS; ++g) copy_row(base, from[g], g, lane, a.head, lds_at + (values ? HALF : 0));
     };
 
     float16v acc[DB];
@@ -440,16 +447,15 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_bf16_d64_kernel(Tree
     for (unsigned db = 0; db < DB; ++db) acc[db] = zeros();
     float most = -INFINITY, sum = 0.0f;
     wait_for_copies();      // nothing of what came before is counted
-    Place next = {0, 0, false};
     if (own_first < last) {
-      next = look_up(own_first);
-      fill(own_first, next.k, false);
-      fill(own_first, next.v, true);
+      look_up(own_first);
+      fill(own_first, next_k, false);
+      fill(own_first, next_v, true);
     }
     for (unsigned n = own_first; n < last; ++n) {
-      const unsigned here = (unsigned)__builtin_amdgcn_ballot_w64(next.there);
+      const unsigned here = next_here;
       const bool more = n + 1 < last, cached = n < seq.cached;
-      if (more) next = look_up(n + 1);
+      if (more) look_up(n + 1);
       wait_for_copies_but<FILLS>();
       float16v s = zeros();
 #pragma unroll
@@ -463,7 +469,7 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_bf16_d64_kernel(Tree
       LEGO_MFMAS(4);
       __builtin_amdgcn_sched_barrier(0);
       wait_for_reads();
-      if (more) fill(n + 1, next.k, false);
+      if (more) fill(n + 1, next_k, false);
       const int first = (int)(32 * (cached ? n : n - seq.cached));
       if (!RAW) {
         const float distance0 = (float)(position - first - 4 * (int)lhi);
@@ -476,9 +482,11 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_bf16_d64_kernel(Tree
       }
       // what of the cache's tile is not there, and what the tree hides
       if (!cached) {
+        int j0 = first + 4 * (int)lhi;
+        asm volatile("" : "+v"(j0));      // nothing of this is made ahead of the branch
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int j = first + 8 * (e / 4) + 4 * (int)lhi + e % 4;
+          const int j = j0 + 8 * (e / 4) + e % 4;
           const bool inside = j < a.drafts;
           const bool seen = inside && (shown ? shown[inside ? j : 0] != 0 : j <= (int)t);
           float x = s[e];
@@ -530,7 +538,7 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_bf16_d64_kernel(Tree
       LEGO_MFMAS(3);
       __builtin_amdgcn_sched_barrier(0);
       wait_for_reads();
-      if (more) fill(n + 1, next.v, true);
+      if (more) fill(n + 1, next_v, true);
     }
     sum = across_sum(sum);
     most *= unit;      // in units of log2 from here on
@@ -594,25 +602,27 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
   constexpr unsigned STAGES = 2, KW = RW == 4 ? 1 : 2, NB = 2 / KW, FILLS = TILE / 1024 / NW;
   __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * TILE];      // K and V, STAGES times
   __shared__ int pages_s[PIECE];
-  __shared__ unsigned long long here_s[STAGES];      // the rows of a tile that are there
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
   const unsigned rw = wave % RW, kw = wave / RW;
-  const unsigned group = a.heads / a.key_heads, rows = group * a.drafts, items = a.key_heads * a.row_blocks;
+  const unsigned group = a.heads / a.key_heads, rows = group * a.drafts, items = a.key_heads;
   const Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds;
 
   unsigned b, item, tile, left;      // the present sequence, item of it, tile of that; tiles of the run that are left
   Sequence seq;
+  // the workgroups of a run, one for each block of its rows, are 8 apart: they go over its tiles side by side on one XCD, whose L2 the later ones find them in
+  const unsigned at8 = blockIdx.x / 8, worker = at8 / a.row_blocks * 8 + blockIdx.x % 8, rb = at8 % a.row_blocks;
   if (a.whole) {
-    b = blockIdx.x / items;
-    item = blockIdx.x % items;
+    if (worker >= (unsigned)a.batch * items) return;
+    b = worker / items;
+    item = worker % items;
     seq = sequence_of(a, b);
     tile = 0;
     left = seq.tiles;
   } else {
-    const unsigned total = total_tiles(a, lane, items), run = run_of(a, total), first = blockIdx.x * run;
-    if (first >= total) return;
+    const unsigned total = total_tiles(a, lane, items), run = run_of(a, total), first = worker * run;
+    if (worker >= a.runs || first >= total) return;
     left = min(run, total - first);
     unsigned before;
     b = find_sequence(a, lane, items, first, before);
@@ -622,7 +632,7 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
   }
 
   do {
-    const unsigned hk = item / a.row_blocks, rb = item % a.row_blocks;
+    const unsigned hk = item;
     const unsigned count = min(left, seq.tiles - tile), last = tile + count;      // tiles of this item
     const unsigned r = 32 * (rb * RW + rw) + l32;             // the lane's row
     const bool mine = r < rows;
@@ -643,26 +653,30 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
     const unsigned char* const shown = a.tree ? a.tree + (size_t)b * a.tree_batch + (size_t)t * a.drafts : nullptr;
 
     unsigned piece = 0, piece_end = 0;      // entries of the table that pages_s holds
-    const auto fill = [&](unsigned n, unsigned stage) __attribute__((always_inline)) {
+    unsigned next_k[FILLS], next_v[FILLS];      // of the tile that is copied next: the lane's rows, and which there are
+    unsigned long long next_here = 0;
+    const auto look_up = [&](unsigned n) __attribute__((always_inline)) {
       const bool cached = n < seq.cached;
       if (cached) {
-        const unsigned after = min(64 * n + 63, seq.length - 1) / (unsigned)a.page + 1;
+        const unsigned after = quotient(min(64 * n + 63, seq.length - 1), a.page_factor, a.page_shift) + 1;
         if (after > piece_end) {      // the table's next piece (uniform: all wavefronts come here together)
           __syncthreads();
-          piece = 64 * n / (unsigned)a.page;
+          piece = quotient(64 * n, a.page_factor, a.page_shift);
           piece_end = min(piece + PIECE, (unsigned)a.width);
           for (unsigned i = threadIdx.x; i < piece_end - piece; i += 64 * NW) pages_s[i] = pages[piece + i];
           __syncthreads();
         }
       }
       const Place place = place_of(a, b, hk, seq, pages_s, piece, piece_end - piece, cached, 64 * (cached ? n : n - seq.cached) + lane);
-      const unsigned long long here = __builtin_amdgcn_ballot_w64(place.there);
-      if (threadIdx.x == 0) here_s[stage] = here;
+      next_here = __builtin_amdgcn_ballot_w64(place.there);
 #pragma unroll
-      for (unsigned it = 0; it < FILLS; ++it) {
-        copy_rows(cached ? a.k_cache : a.k, place.k, it * NW + wave, lane, a.head, lds_at + stage * (2 * TILE));
-        copy_rows(cached ? a.v_cache : a.v, place.v, it * NW + wave, lane, a.head, lds_at + stage * (2 * TILE) + TILE);
-      }
+      for (unsigned it = 0; it < FILLS; ++it) next_k[it] = row_of_copy(place.k, it * NW + wave, lane), next_v[it] = row_of_copy(place.v, it * NW + wave, lane);
+    };
+    const auto fill = [&](unsigned n, unsigned stage, bool values) __attribute__((always_inline)) {
+      const void* const base = n < seq.cached ? (values ? a.v_cache : a.k_cache) : (values ? a.v : a.k);
+#pragma unroll
+      for (unsigned it = 0; it < FILLS; ++it)
+        copy_row(base, values ? next_v[it] : next_k[it], it * NW + wave, lane, a.head, lds_at + stage * (2 * TILE) + (values ? TILE : 0));
     };
 
     // as in the forward kernel: the running maximum is of the products themselves where nothing but the scale comes in between
@@ -673,22 +687,31 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
     for (unsigned db = 0; db < DB; ++db) acc[db] = zeros();
     float most = -INFINITY, sum = 0.0f;
     unsigned stage = 0;
-    if (tile < last) fill(tile, 0);
+    // Copies are asked for in the order K(n), V(n), K(n + 1), V(n + 1): the keys of the tile after the next one when those of this tile have been read, the values of the next tile when those of
+    // the last one have.  So two of them are on their way behind the one that is waited for, and each has one and a half tiles' time.
+    unsigned long long here = 0, here1 = 0;      // rows that are there, of this tile and of the next one
+    wait_for_copies();
+    if (tile < last) {
+      look_up(tile);
+      fill(tile, 0, false);
+      fill(tile, 0, true);
+      here = next_here;
+      if (tile + 1 < last) {
+        look_up(tile + 1);
+        fill(tile + 1, 1, false);
+      }
+    }
     for (unsigned n = tile; n < last; ++n) {
-      wait_for_copies();
-      __syncthreads();
-      if (n + 1 < last) fill(n + 1, stage ^ 1);
+      if (n + 1 < last) wait_for_copies_but<2 * FILLS>();
+      else wait_for_copies_but<FILLS>();
+      __syncthreads();      // the keys are there, and the values before these have been read
+      here1 = next_here;
+      if (n + 1 < last) fill(n + 1, stage ^ 1, true);
+      if (n + 2 < last) look_up(n + 2);
+      __builtin_amdgcn_sched_barrier(0);
       char* const kt = lds + stage * (2 * TILE);
       char* const vt = kt + TILE;
       const bool cached = n < seq.cached;
-      const unsigned long long here = (unsigned long long)__builtin_amdgcn_readfirstlane((unsigned)(here_s[stage] >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((unsigned)here_s[stage]);
-      stage ^= 1;
-      if (here != ~0ull) {      // values that are not there are zeros: whatever was read in their place, times a P of zero
-#pragma unroll
-        for (unsigned at = threadIdx.x; at < TILE / 16; at += 64 * NW)
-          if (!(here >> (at / (PITCH / 8)) & 1)) reinterpret_cast<u32x4*>(vt)[at] = u32x4{0u, 0u, 0u, 0u};
-        __syncthreads();
-      }
       const int first = (int)(64 * (cached ? n : n - seq.cached)) + (int)(32 * NB * kw);      // of this wavefront's keys
       float16v s[NB];
 #pragma unroll
@@ -706,6 +729,17 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
       }
       LEGO_MFMAS(FIRST_READS);
       __builtin_amdgcn_sched_barrier(0);
+      if (n + 1 < last) wait_for_copies_but<2 * FILLS>();
+      else wait_for_copies();
+      __syncthreads();      // the values are there, and the keys have been read
+      if (n + 2 < last) fill(n + 2, stage, false);
+      stage ^= 1;
+      if (here != ~0ull) {      // values that are not there are zeros: whatever was read in their place, times a P of zero
+#pragma unroll
+        for (unsigned at = threadIdx.x; at < TILE / 16; at += 64 * NW)
+          if (!(here >> (at / (PITCH / 8)) & 1)) reinterpret_cast<u32x4*>(vt)[at] = u32x4{0u, 0u, 0u, 0u};
+        __syncthreads();
+      }
       const auto operand = [&](unsigned j) { return read.transposed(vt, 2 * NB * kw + j / DB, j % DB); };
       elt8 ahead[RING];      // operands of the second products, on their way meanwhile
 #pragma unroll
@@ -724,11 +758,13 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
       }
       // what of the cache's tile is not there, and what the tree hides
       if (!cached) {
+        int j0 = first + 4 * (int)lhi;
+        asm volatile("" : "+v"(j0));      // nothing of this is made ahead of the branch
 #pragma unroll
         for (unsigned i = 0; i < NB; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int j = first + (int)(32 * i + 8 * (e / 4) + 4 * lhi) + e % 4;
+            const int j = j0 + (int)(32 * i + 8 * (e / 4)) + e % 4;
             const bool inside = j < a.drafts;
             const bool seen = inside && (shown ? shown[inside ? j : 0] != 0 : j <= (int)t);
             float x = s[i][e];
@@ -780,6 +816,7 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
         __builtin_amdgcn_sched_barrier(0);
       }
       sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      here = here1;
     }
     sum = across_sum(sum);
     most *= unit;      // in units of log2 from here on
@@ -816,9 +853,9 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
       if (count == seq.tiles) {
         elt_t* const row = mine ? static_cast<elt_t*>(a.o) + (size_t)b * a.so.batch + (size_t)t * a.so.token + (size_t)h * a.so.head : nullptr;
         store_columns<DB>(acc, row, lane, a.head, sum == 0.0f ? 0.0f : 1.0f / sum);
-      } else {      // slot: the workgroup's number and the item's, which no two parts share
-        const size_t slot = (size_t)blockIdx.x + (size_t)b * items + item;
-        const size_t at = slot * (32 * RW) + 32 * rw + l32;
+      } else {      // slot: the run's number and the item's, which no two parts share
+        const size_t slot = (size_t)worker + (size_t)b * items + item;
+        const size_t at = (slot * a.row_blocks + rb) * (32 * RW) + 32 * rw + l32;
         if (lhi == 0) a.stats[at] = float2{most, sum};
         float* const to = a.sums + at * DC;
 #pragma unroll
@@ -842,25 +879,23 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d64_kernel(Tre
 
 // The rows of items in several runs, and of those that have no tile, `share` rows of an item a workgroup: a few parts are gone through by the lanes of each row, many by teams of lanes, a row
 // after the other.  Either order is the same whenever the lengths are.
-__global__ void __launch_bounds__(256) lego_tree_join_bf16_d64_kernel(TreeArgs a, unsigned block_rows, unsigned share, unsigned chunks)
+__global__ void __launch_bounds__(256) lego_tree_join_bf16_d64_kernel(TreeArgs a, unsigned held_rows, unsigned share, unsigned chunks)
 {
   constexpr unsigned LANES = DC / 4 > 16 ? 32 : 16, TEAMS = 256 / LANES;
   __shared__ float4v sums_s[TEAMS][LANES];
   __shared__ float sum_s[TEAMS], most_s[4];
   const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = threadIdx.x % LANES, team = threadIdx.x / LANES;
-  const unsigned group = a.heads / a.key_heads, rows = group * a.drafts, items = a.key_heads * a.row_blocks;
+  const unsigned group = a.heads / a.key_heads, rows = group * a.drafts, items = a.key_heads;
   const unsigned chunk = blockIdx.x % chunks, item = blockIdx.x / chunks % items, b = blockIdx.x / chunks / items;
-  const unsigned hk = item / a.row_blocks, r0 = item % a.row_blocks * block_rows;      // the item's first row
-  const unsigned begin = chunk * share, end = min(min(begin + share, block_rows), rows - r0);      // of its rows
-  if (begin >= end) return;
+  const unsigned begin = chunk * share, end = min(begin + share, rows);
   const unsigned tiles = sequence_of(a, b).tiles, total = total_tiles(a, lane, items), run = run_of(a, total), first = tiles_before(a, lane, items, b) + item * tiles;
   const auto row_at = [&](unsigned i) {
-    const unsigned t = (r0 + i) / group, h = hk * group + (r0 + i) % group;
+    const unsigned t = i / group, h = item * group + i % group;
     return static_cast<elt_t*>(a.o) + (size_t)b * a.so.batch + (size_t)t * a.so.token + (size_t)h * a.so.head + 4 * c;
   };
   const unsigned w0 = tiles ? first / run : 0, parts = tiles ? (first + tiles - 1) / run - w0 + 1 : 0;
   if (parts == 1) return;
-  const size_t place0 = ((size_t)w0 + (size_t)b * items + item) * block_rows;      // parts are block_rows apart
+  const size_t place0 = ((size_t)w0 + (size_t)b * items + item) * held_rows;      // parts are held_rows apart
   const auto store = [&](unsigned i, float sum, const float4v& x) {
     const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (4 * c < (unsigned)a.head) *reinterpret_cast<u32x2*>(row_at(i)) = u32x2{pack(factor * x[0], factor * x[1]), pack(factor * x[2], factor * x[3])};
@@ -875,9 +910,9 @@ __global__ void __launch_bounds__(256) lego_tree_join_bf16_d64_kernel(TreeArgs a
     for (unsigned i = begin + team; i < end; i += TEAMS) {
       float most = -INFINITY, sum = 0.0f;
       float4v x = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (unsigned p = 0; p < parts; ++p) most = fmaxf(most, a.stats[place0 + i + (size_t)p * block_rows].x);
+      for (unsigned p = 0; p < parts; ++p) most = fmaxf(most, a.stats[place0 + i + (size_t)p * held_rows].x);
 #pragma unroll 2
-      for (unsigned p = 0; p < parts; ++p) add(place0 + i + (size_t)p * block_rows, most, sum, x);
+      for (unsigned p = 0; p < parts; ++p) add(place0 + i + (size_t)p * held_rows, most, sum, x);
       store(i, sum, x);
     }
     return;
@@ -885,14 +920,14 @@ __global__ void __launch_bounds__(256) lego_tree_join_bf16_d64_kernel(TreeArgs a
   for (unsigned i = begin; i < end; ++i) {
     float most = -INFINITY, sum = 0.0f;
     float4v x = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (unsigned p = threadIdx.x; p < parts; p += 256) most = fmaxf(most, a.stats[place0 + i + (size_t)p * block_rows].x);
+    for (unsigned p = threadIdx.x; p < parts; p += 256) most = fmaxf(most, a.stats[place0 + i + (size_t)p * held_rows].x);
 #pragma unroll
     for (int d = 32; d; d /= 2) most = fmaxf(most, __shfl_xor(most, d));
     if (lane == 0) most_s[wave] = most;
     __syncthreads();
     most = fmaxf(fmaxf(most_s[0], most_s[1]), fmaxf(most_s[2], most_s[3]));
 #pragma unroll 4
-    for (unsigned p = team; p < parts; p += TEAMS) add(place0 + i + (size_t)p * block_rows, most, sum, x);
+    for (unsigned p = team; p < parts; p += TEAMS) add(place0 + i + (size_t)p * held_rows, most, sum, x);
     sums_s[team][c] = x;
     if (c == 0) sum_s[team] = sum;
     __syncthreads();
@@ -913,7 +948,8 @@ __global__ void __launch_bounds__(256) lego_tree_join_bf16_d64_kernel(TreeArgs a
 hipError_t lego_tree_bf16_d64_launch(const TreeArgs& a, int row_waves, hipStream_t stream)
 {
   const auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(a.whole ? (unsigned)(a.batch * a.key_heads) * a.row_blocks : a.runs), dim3(64 * NW), 0, stream, a);
+    const unsigned workers = a.whole ? (unsigned)(a.batch * a.key_heads) : a.runs, grid = a.row_blocks == 1 ? workers : (workers + 7) / 8 * 8 * a.row_blocks;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * NW), 0, stream, a);
     return hipGetLastError();
   };
   hipError_t e = hipErrorInvalidValue;
@@ -931,8 +967,7 @@ hipError_t lego_tree_bf16_d64_launch(const TreeArgs& a, int row_waves, hipStream
         : row_waves == 2 ? launch(lego_tree_many_bf16_d64_kernel<false, false, 2>) : launch(lego_tree_many_bf16_d64_kernel<false, false, 4>);
   if (e != hipSuccess || a.whole) return e;
   // One row a workgroup while they are few, and have many parts each; 8 of many rows share the search for their parts.
-  const unsigned block = 32u * (unsigned)row_waves, rows = (unsigned)(a.drafts * (a.heads / a.key_heads)), held = rows < block ? rows : block;
-  const unsigned share = (unsigned)(a.batch * a.heads * a.drafts) <= 4096 ? 1 : 8, chunks = (held + share - 1) / share;
-  hipLaunchKernelGGL(lego_tree_join_bf16_d64_kernel, dim3((unsigned)(a.batch * a.key_heads) * a.row_blocks * chunks), dim3(256), 0, stream, a, block, share, chunks);
+  const unsigned rows = (unsigned)(a.drafts * (a.heads / a.key_heads)), share = (unsigned)(a.batch * a.key_heads) * rows <= 4096 ? 1 : 8, chunks = (rows + share - 1) / share;
+  hipLaunchKernelGGL(lego_tree_join_bf16_d64_kernel, dim3((unsigned)(a.batch * a.key_heads) * chunks), dim3(256), 0, stream, a, 32u * (unsigned)row_waves * a.row_blocks, share, chunks);
   return hipGetLastError();
 }

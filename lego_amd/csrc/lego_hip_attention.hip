@@ -121,20 +121,21 @@ inline bool plan_of(TreeArgs& a, const long long* sizes, TreePlan& plan)
   const unsigned block = 32 * plan.row_waves;
   a.row_blocks = (rows + block - 1) / block;
   a.tile = plan.row_waves == 1 ? 32 : 64;
-  const unsigned long long items = (unsigned long long)a.batch * a.key_heads * a.row_blocks;
+  const unsigned long long items = (unsigned long long)a.batch * a.key_heads;
   const unsigned long long most = ((unsigned long long)a.page * a.width + a.tile - 1) / a.tile + ((unsigned)a.drafts + a.tile - 1) / a.tile;
   if (items * most >= (1ull << 31)) return false;
   // An item of few tiles is one workgroup's; else the tiles are dealt in equal runs to as many workgroups as the chip holds at a time, but no run is shorter than a tile or two a wavefront.
   a.least = plan.row_waves == 1 ? 2 * LEGO_TREE_LEAST : LEGO_TREE_LEAST;
   a.whole = most <= (plan.row_waves == 1 ? 16 : 4);
-  const unsigned long long held = plan.row_waves == 1 && a.head <= 64 ? 768 : 512, runs = (items * most + a.least - 1) / a.least;
+  const unsigned long long chip = plan.row_waves == 1 && a.head <= 64 ? 768 : 512, held = chip > a.row_blocks ? chip / a.row_blocks : 1, runs = (items * most + a.least - 1) / a.least;
   a.runs = (unsigned)(runs < held ? runs : held);
+  quotients_by((unsigned)a.page, a.page_factor, a.page_shift);
   plan.stats = plan.all = 0;
   if (a.whole) return true;
   const unsigned pitch = a.head <= 64 ? 64 : a.head <= 96 ? 96 : 128;
   const size_t slots = (size_t)a.runs + items;
-  plan.stats = slots * block * pitch * sizeof(float);
-  plan.all = plan.stats + slots * block * sizeof(float2);
+  plan.stats = slots * a.row_blocks * block * pitch * sizeof(float);
+  plan.all = plan.stats + slots * a.row_blocks * block * sizeof(float2);
   return true;
 }
 

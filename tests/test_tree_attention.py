@@ -276,10 +276,26 @@ typedef struct { int x, y; } int2; typedef struct { float x, y; } float2;
 #include <stdint.h>
 ''' + (CSRC / "attention_args.h").read_text().replace("#include <hip/hip_runtime.h>", "").replace("#pragma once", "") + '''
 extern "C" int lookup(const int* p, unsigned n, unsigned c, bool w, unsigned at) { return page_of(p, n, c, w, at); }
+extern "C" unsigned long long wrong_quotients(unsigned d)
+{
+  unsigned factor, shift;
+  quotients_by(d, factor, shift);
+  const unsigned long long last = 0x7fffffffull;
+  unsigned long long wrong = 0;
+  for (unsigned long long i = 0; i < 4000; ++i) {      // around multiples of d from either end of the range, and the ends
+    const unsigned long long near[] = {i * d, i * d - 1, last - last % d - i * d, last - last % d - i * d - 1, i, last - i};
+    for (unsigned long long x : near)
+      if (x <= last) wrong += quotient((unsigned)x, factor, shift) != x / d;
+  }
+  return wrong;
+}
 ''')
     lib = tmp_path / "p.so"
     subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-o", str(lib), str(tmp_path / "p.cpp")], check=True, capture_output=True)
-    look = ctypes.CDLL(str(lib)).lookup
+    loaded = ctypes.CDLL(str(lib))
+    for d in list(range(1, 300)) + [(1 << i) + j for i in range(9, 31) for j in (-1, 0, 1)] + [(1 << 31) - 1]:
+        assert loaded.wrong_quotients(ctypes.c_uint(d)) == 0, d
+    look = loaded.lookup
     look.argtypes = [ctypes.POINTER(ctypes.c_int), ctypes.c_uint, ctypes.c_uint, ctypes.c_bool, ctypes.c_uint]
     table = (ctypes.c_int * 5)(5, -1, 9, 10, 1 << 30)
     assert [look(table, 5, 10, True, at) for at in range(5)] == [5, -1, 9, -1, -1]
