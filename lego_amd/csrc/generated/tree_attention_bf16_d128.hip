@@ -323,39 +323,39 @@ __device__ __forceinline__ void wait_for_reads() { asm volatile("s_waitcnt lgkmc
 constexpr unsigned NW = 4;                     // wavefronts of a workgroup
 constexpr unsigned PIECE = 1024;               // entries of a page table in LDS
 
+// Where keys and values lie, in 16-byte chunks: 32 bits of every product are enough, they are all that is left of the sum, which lies in what the strides reach.  Read once and held: as fields of the
+// arguments they are fetched one after the other at every tile (a first token 7.5 -> 7.0 us, a decoding step of 32 sequences 108 -> 106).
+struct Rows {
+  unsigned outer, row, head;      // from a page (a sequence) to the next one, from a token, from a head
+  __device__ __forceinline__ Rows(const Strides& by) : outer((unsigned)(by.batch >> 3)), row((unsigned)(by.token >> 3)), head((unsigned)(by.head >> 3))
+  {
+    asm volatile("" : "+s"(outer), "+s"(row), "+s"(head));
+  }
+};
+
 // A row of a tile, as the lane knows it that looks it up: 16-byte chunks from the base of what it lies in.
 struct Place { unsigned k, v; bool there; };
-__device__ __forceinline__ Place place_of(const TreeArgs& a, unsigned b, unsigned hk, const Sequence& seq, const int* table, unsigned piece, unsigned entries, bool cached, unsigned key)
+__device__ __forceinline__ Place place_of(const TreeArgs& a, const Rows& k, const Rows& v, const Rows& dk, const Rows& dv, unsigned b, unsigned hk, const Sequence& seq, const int* table, unsigned piece,
+                                          unsigned entries, bool cached, unsigned key)
 {
-  // 32 bits of every product are enough: they are all that is left of the sum in 16-byte chunks, which lies in what the strides reach
-  unsigned k = 0, v = 0;
-  bool there;
-  const auto chunks = [](long long elements) { return (unsigned)(elements >> 3); };
-  if (cached) {
-    const unsigned at = quotient(key, a.page_factor, a.page_shift), row = key - at * (unsigned)a.page;
-    const int page = page_of(table, entries, a.count, key < seq.length, at - piece);
-    there = page >= 0;
-    if (there) {
-      k = (unsigned)page * chunks(a.skc.batch) + row * chunks(a.skc.token) + hk * chunks(a.skc.head);
-      v = (unsigned)page * chunks(a.svc.batch) + row * chunks(a.svc.token) + hk * chunks(a.svc.head);
-    }
-  } else {
-    there = key < (unsigned)a.drafts;
-    if (there) {
-      k = b * chunks(a.sk.batch) + key * chunks(a.sk.token) + hk * chunks(a.sk.head);
-      v = b * chunks(a.sv.batch) + key * chunks(a.sv.token) + hk * chunks(a.sv.head);
-    }
+  if (!cached) {
+    const bool there = key < (unsigned)a.drafts;
+    const unsigned row = there ? key : 0u;
+    return {there ? b * dk.outer + row * dk.row + hk * dk.head : 0u, there ? b * dv.outer + row * dv.row + hk * dv.head : 0u, there};
   }
-  return {k, v, there};
+  const unsigned at = quotient(key, a.page_factor, a.page_shift), row = key - at * (unsigned)a.page;
+  const int page = page_of(table, entries, a.count, key < seq.length, at - piece);
+  const bool there = page >= 0;
+  return {there ? (unsigned)page * k.outer + row * k.row + hk * k.head : 0u, there ? (unsigned)page * v.outer + row * v.row + hk * v.head : 0u, there};
 }
 
 // Copy number g of a tile: 1 KiB of the rows' chunks.  Every instruction has all its lanes, so that each counts for one: a row that is not there reads the base's first one, and a chunk past
-// the head its row's first one, which meets zeros of Q and gives columns that nobody stores.  The lane's row of the copy is asked for (row_of_copy) well before its place is used.
+// the head its row's last one, which meets zeros of Q and gives columns that nobody stores.  The lane's row of the copy is asked for (row_of_copy) well before its place is used.
 __device__ __forceinline__ unsigned row_of_copy(unsigned own, unsigned g, unsigned lane) { return __shfl(own, 4*g + ((lane)/(16))); }
 __device__ __forceinline__ void copy_row(const void* base, unsigned at, unsigned g, unsigned lane, unsigned head, unsigned lds)
 {
   const unsigned chunk = ((lane % 16) ^ (g % 4 + 4*((lane)/(16))));
-  const char* const from = static_cast<const char*>(base) + (size_t)at * 16 + (8 * chunk < head ? 16 * chunk : 0u);
+  const char* const from = static_cast<const char*>(base) + (size_t)at * 16 + min(16 * chunk, 2 * head - 16);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds + g * 1024) : "memory", "m0");
 }
 
@@ -378,6 +378,9 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_bf16_d128_kernel(Tre
   constexpr bool RAW = !CAP && !BIAS;
   const float unit = RAW ? fabsf(a.scores.scale_log2) : 1.0f, lazy = kLazy / unit;
 
+  const Rows cache_k(a.skc), cache_v(a.svc), draft_k(a.sk), draft_v(a.sv);
+  const void *k_cache = a.k_cache, *v_cache = a.v_cache;
+  asm volatile("" : "+s"(k_cache), "+s"(v_cache));
   unsigned b, item, tile, left;      // the present sequence, item of it, tile of that; tiles of the run that are left
   Sequence seq;
   if (a.whole) {
@@ -431,13 +434,13 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_bf16_d128_kernel(Tre
           __builtin_amdgcn_wave_barrier();
         }
       }
-      const Place place = place_of(a, b, hk, seq, table, piece, piece_end - piece, cached, 32 * (cached ? n : n - seq.cached) + l32);
+      const Place place = place_of(a, cache_k, cache_v, draft_k, draft_v, b, hk, seq, table, piece, piece_end - piece, cached, 32 * (cached ? n : n - seq.cached) + l32);
       next_here = (unsigned)__builtin_amdgcn_ballot_w64(place.there);
 #pragma unroll
       for (unsigned g = 0; g < FILLS; ++g) next_k[g] = row_of_copy(place.k, g, lane), next_v[g] = row_of_copy(place.v, g, lane);
     };
     const auto fill = [&](unsigned n, const unsigned* from, bool values) __attribute__((always_inline)) {
-      const void* const base = n < seq.cached ? (values ? a.v_cache : a.k_cache) : (values ? a.v : a.k);
+      const void* const base = n < seq.cached ? (values ? v_cache : k_cache) : (values ? a.v : a.k);
 #pragma unroll
       for (unsigned g = 0; g < FILLS; ++g) copy_row(base, from[g], g, lane, a.head, lds_at + (values ? HALF : 0));
     };
@@ -609,6 +612,9 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d128_kernel(Tr
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds;
 
+  const Rows cache_k(a.skc), cache_v(a.svc), draft_k(a.sk), draft_v(a.sv);
+  const void *k_cache = a.k_cache, *v_cache = a.v_cache;
+  asm volatile("" : "+s"(k_cache), "+s"(v_cache));
   unsigned b, item, tile, left;      // the present sequence, item of it, tile of that; tiles of the run that are left
   Sequence seq;
   // the workgroups of a run, one for each block of its rows, are 8 apart: they go over its tiles side by side on one XCD, whose L2 the later ones find them in
@@ -667,13 +673,13 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_bf16_d128_kernel(Tr
           __syncthreads();
         }
       }
-      const Place place = place_of(a, b, hk, seq, pages_s, piece, piece_end - piece, cached, 64 * (cached ? n : n - seq.cached) + lane);
+      const Place place = place_of(a, cache_k, cache_v, draft_k, draft_v, b, hk, seq, pages_s, piece, piece_end - piece, cached, 64 * (cached ? n : n - seq.cached) + lane);
       next_here = __builtin_amdgcn_ballot_w64(place.there);
 #pragma unroll
       for (unsigned it = 0; it < FILLS; ++it) next_k[it] = row_of_copy(place.k, it * NW + wave, lane), next_v[it] = row_of_copy(place.v, it * NW + wave, lane);
     };
     const auto fill = [&](unsigned n, unsigned stage, bool values) __attribute__((always_inline)) {
-      const void* const base = n < seq.cached ? (values ? a.v_cache : a.k_cache) : (values ? a.v : a.k);
+      const void* const base = n < seq.cached ? (values ? v_cache : k_cache) : (values ? a.v : a.k);
 #pragma unroll
       for (unsigned it = 0; it < FILLS; ++it)
         copy_row(base, values ? next_v[it] : next_k[it], it * NW + wave, lane, a.head, lds_at + stage * (2 * TILE) + (values ? TILE : 0));
