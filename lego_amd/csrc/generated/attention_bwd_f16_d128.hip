@@ -254,6 +254,28 @@ __device__ __forceinline__ void store_columns(const float16v (&acc)[BLOCKS], elt
     }
 }
 
+// A wave's sums into LDS, times a factor, and another wave's added to them.
+template <unsigned BLOCKS>
+__device__ __forceinline__ void put(const float16v (&acc)[BLOCKS], float4v* to, unsigned lane, float factor)
+{
+#pragma unroll
+  for (unsigned db = 0; db < BLOCKS; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) to[(4 * db + g) * 64 + lane] = factor * float4v{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+}
+template <unsigned BLOCKS>
+__device__ __forceinline__ void add(float16v (&acc)[BLOCKS], float factor, const float4v* from, unsigned lane, float other)
+{
+#pragma unroll
+  for (unsigned db = 0; db < BLOCKS; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4v x = from[(4 * db + g) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[db][4 * g + e] = factor * acc[db][4 * g + e] + other * x[e];
+    }
+}
+
 }  // namespace
 
 namespace {
@@ -262,16 +284,17 @@ constexpr float kUnshift = 1.0f / (1 << 8);      // P is held as P / kUnshift
 template <unsigned V> struct Constant { static constexpr unsigned value = V; };
 constexpr unsigned RING = 3;      // operands read ahead
 
-template <bool CAP, bool BIAS, bool DOCS>
+template <bool CAP, bool BIAS, bool DOCS, unsigned HALVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_f16_d128_kernel(AttentionArgs a)
 {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 2 * 768];      // Q and dO, twice; lse, delta and documents, twice
-  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
-  const unsigned blocks = (a.keys + 32 * WAVES - 1) / (32 * WAVES), group = a.heads / a.key_heads, parts = group / a.heads_per_part;
+  constexpr unsigned RW = WAVES / HALVES, OWN = 32 * RW, SLOTS = 2 * HALVES;      // wavefronts of other keys than the others; keys of the workgroup; tiles in LDS
+  __shared__ __attribute__((aligned(1024))) char lds[SLOTS * (2 * TILE + 768)];      // Q and dO, then lse, delta and documents
+  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32, half = wave / RW;
+  const unsigned blocks = (a.keys + OWN - 1) / OWN, group = a.heads / a.key_heads, parts = group / a.heads_per_part;
   const unsigned all_parts = parts * a.key_heads * a.batch, turn = blockIdx.x % all_parts, block = blockIdx.x / all_parts;      // earlier keys may be seen by more queries
   const unsigned at_part = place(turn, all_parts), part = at_part % parts, hk = at_part / parts % a.key_heads, b = at_part / parts / a.key_heads;
-  const int k0 = (int)(32 * WAVES * block), k_last = min(k0 + (int)(32 * WAVES), a.keys) - 1;
-  const int w0 = k0 + (int)(32 * wave), key = w0 + (int)l32;
+  const int k0 = (int)(OWN * block), k_last = min(k0 + (int)OWN, a.keys) - 1;
+  const int w0 = k0 + (int)(32 * (wave % RW)), key = w0 + (int)l32;
   const int shift = a.keys - a.queries, prefix = a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : a.keys;
   const int first_row = a.causal && prefix == 0 ? -shift : 0;      // that sees a key
   // a query sees a key from this row on
@@ -303,12 +326,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_f16_d128_ker
   Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_base = (unsigned)(uintptr_t)(lds_ptr)lds, lds_at = lds_base + wave * 1024;
-  const auto fill = [&](unsigned h, const Step& step, unsigned buffer) {
+  const auto fill = [&](unsigned h, const Step& step, unsigned slot) {
+    if (!step.there()) return;
     const unsigned first = 64 * step.tile, rows = a.queries - first;
     fill_q.base = reinterpret_cast<const char*>(static_cast<const elt_t*>(a.q) + (size_t)b * a.sq.batch + (size_t)h * a.sq.head);
     fill_do.base = reinterpret_cast<const char*>(static_cast<const elt_t*>(a.dout) + (size_t)b * a.sdo.batch + (size_t)h * a.sdo.head);
     const size_t row = ((size_t)b * a.heads + h) * a.queries + first;
-    const unsigned at = lds_at + buffer * (2 * TILE), words = lds_base + 4 * TILE + buffer * 768;
+    const unsigned at = lds_at + slot * (2 * TILE), words = lds_base + SLOTS * (2 * TILE) + slot * 768;
     if (wave == 0) fill_words(a.less + row, rows, lane, words);
     if (wave == 1) fill_words(a.delta + row, rows, lane, words + 256);
     if (DOCS && wave == 2 && step.compare) fill_words(documents + first + shift, rows, lane, words + 512);
@@ -340,21 +364,34 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_f16_d128_ker
     }
     return step;
   };
-  Step now = advance(h);
+  // the tiles in turn for the halves of the workgroup
+  struct { Step step; unsigned h; } now[HALVES], next[HALVES];
   unsigned buffer = 0;
-  if (now.there()) fill(h, now, 0);
-  while (now.there()) {
-    unsigned next_h = h;
-    const Step next = advance(next_h);
+#pragma unroll
+  for (unsigned n = 0; n < HALVES; ++n) {
+    now[n].step = advance(h);
+    now[n].h = h;
+    fill(h, now[n].step, n);
+  }
+  while (now[0].step.there()) {
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) {
+      next[n].step = advance(h);
+      next[n].h = h;
+    }
     wait_for_copies();
     __syncthreads();
-    if (next.there()) fill(next_h, next, buffer ^ 1);
-    const char* const qt = lds + buffer * (2 * TILE);
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) fill(next[n].h, next[n].step, (buffer ^ HALVES) + n);
+    const Step own = now[half ? HALVES - 1 : 0].step;
+    const unsigned own_h = now[half ? HALVES - 1 : 0].h;
+    const char* const qt = lds + (buffer + half) * (2 * TILE);
     const char* const dot = qt + TILE;
-    const float* const less_s = reinterpret_cast<const float*>(lds + 4 * TILE + buffer * 768);
-    const int first = (int)(64 * now.tile);
-    const float slope = BIAS ? (CAP ? kLog2e : kLog2e * a.scores.unscale) * a.slopes[h] : 0.0f;
-    const float tile_up = a.ups[((size_t)b * a.heads + h) * end + first / 64];
+    const float* const less_s = reinterpret_cast<const float*>(lds + SLOTS * (2 * TILE) + (buffer + half) * 768);
+    const int first = (int)(64 * own.tile);
+    const bool any = HALVES == 1 || own.there();
+    const float slope = BIAS ? (CAP ? kLog2e : kLog2e * a.scores.unscale) * a.slopes[own_h] : 0.0f;
+    const float tile_up = any ? a.ups[((size_t)b * a.heads + own_h) * end + first / 64] : up;
     if (up == 0.0f) up = tile_up;
     if (tile_up < up) {
       const float down = tile_up / up;
@@ -365,7 +402,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_f16_d128_ker
           for (int r = 0; r < 16; ++r) dk[db][r] *= down;
     }
     const float shrink = up * kUnshift;
-    if (first + 63 >= from_w0) {
+    if (any && first + 63 >= from_w0) {
 #pragma unroll 1
       for (unsigned qb = 0; qb < 2; ++qb) {
         asm volatile("" : "+v"(read.row_at), "+v"(read.tr_at));      // the offsets of a step are one operation from these: they are not to be kept in registers
@@ -446,7 +483,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_f16_d128_ker
 #pragma unroll
           for (int r = 0; r < 16; r += 2) hide(r, seen(r), seen(r + 1));
         }
-        if (DOCS && now.compare) {
+        if (DOCS && own.compare) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int4v d = *reinterpret_cast<const int4v*>(reinterpret_cast<const int*>(less_s) + 128 + 32 * qb + 8 * g + 4 * lhi);
@@ -474,11 +511,25 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_f16_d128_ker
         }
       }
     }
-    now = next;
-    h = next_h;
-    buffer ^= 1;
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) now[n] = next[n];
+    buffer ^= HALVES;
   }
-  const float k_factor = up == 0.0f ? 0.0f : (CAP ? 4.0f : 1.0f) * a.scores.scale / up, v_factor = kUnshift;
+  float k_factor = up == 0.0f ? 0.0f : (CAP ? 4.0f : 1.0f) * a.scores.scale / up, v_factor = kUnshift;
+  if constexpr (HALVES == 2) {      // the second half's sums through LDS, in the tiles' place
+    __syncthreads();
+    float4v* const sums_s = reinterpret_cast<float4v*>(lds) + (wave % RW) * (2 * 64 * 4 * DB);
+    static_assert(RW * 2 * 64 * 16 * DB * 4 <= SLOTS * 2 * TILE, "sums of the second half in the tiles' place");
+    if (half) {
+      put<DB>(dk, sums_s, lane, k_factor);
+      put<DB>(dv, sums_s + 64 * 4 * DB, lane, v_factor);
+    }
+    __syncthreads();
+    if (half) return;
+    add<DB>(dk, k_factor, sums_s, lane, 1.0f);
+    add<DB>(dv, v_factor, sums_s + 64 * 4 * DB, lane, 1.0f);
+    k_factor = v_factor = 1.0f;
+  }
   {
     const int j = key;
     const bool mine = j < a.keys;
@@ -502,18 +553,19 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_f16_d128_ker
   }
 }
 
-template <bool CAP, bool BIAS, bool DOCS>
+template <bool CAP, bool BIAS, bool DOCS, unsigned HALVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_f16_d128_kernel(AttentionArgs a)
 {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 512];      // K and V, twice; the keys' documents, twice
-  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
-  const unsigned blocks = (a.queries + 32 * WAVES - 1) / (32 * WAVES);
+  constexpr unsigned RW = WAVES / HALVES, OWN = 32 * RW, SLOTS = 2 * HALVES;      // as in the forward kernel
+  __shared__ __attribute__((aligned(1024))) char lds[SLOTS * (2 * TILE + 256)];      // K and V, then the keys' documents
+  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32, half = wave / RW;
+  const unsigned blocks = (a.queries + OWN - 1) / OWN;
   const unsigned all_heads = a.heads * a.batch, block = blocks - 1 - blockIdx.x / all_heads;      // later queries may see more keys
   const unsigned head = place(blockIdx.x % all_heads, all_heads);
   const unsigned h = head % a.heads, b = head / a.heads;
   const unsigned hk = h / (a.heads / a.key_heads);
-  const int q0 = (int)(32 * WAVES * block), q_last = min(q0 + 32 * (int)WAVES, a.queries) - 1;
-  const int w0 = q0 + 32 * (int)wave, i = w0 + (int)l32;
+  const int q0 = (int)(OWN * block), q_last = min(q0 + (int)OWN, a.queries) - 1;
+  const int w0 = q0 + 32 * (int)(wave % RW), i = w0 + (int)l32;
   const Seen seen{a.keys, a.keys - a.queries, a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : -1};
   const int limit = seen.limit(i), limit_w0 = seen.limit(w0), limit_w1 = seen.limit(min(w0 + 31, q_last));
   const int* const documents = DOCS ? a.documents + (size_t)b * a.keys : nullptr;
@@ -556,10 +608,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_f16_d128_kern
   Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
-  const auto fill = [&](const Step& step, unsigned buffer) {
+  const auto fill = [&](const Step& step, unsigned slot) {
+    if (!step.there()) return;
     const unsigned first = 64 * step.tile, rows = a.keys - first;
-    const unsigned at = lds_at + buffer * (2 * TILE);
-    if (DOCS && step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + 4 * TILE + buffer * 256);
+    const unsigned at = lds_at + slot * (2 * TILE);
+    if (DOCS && step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + SLOTS * (2 * TILE) + slot * 256);
     // padding among the keys is read as zeros, whatever it holds
     const auto skip = [&](unsigned row) { return DOCS && step.padded && documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
     fill_k(lane, wave, first, rows, at, skip);
@@ -571,20 +624,28 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_f16_d128_kern
 #pragma unroll
   for (unsigned db = 0; db < DB; ++db) dq[db] = zeros();
   Walk<DOCS, decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
-  Step now = walk.next();
+  Step now[HALVES];
   unsigned buffer = 0;
-  if (now.there()) fill(now, 0);
-  while (now.there()) {
-    const Step next = walk.next();
+#pragma unroll
+  for (unsigned n = 0; n < HALVES; ++n) {
+    now[n] = walk.next();
+    fill(now[n], n);
+  }
+  while (now[0].there()) {
+    Step next[HALVES];
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) next[n] = walk.next();
     wait_for_copies();
     __syncthreads();
-    if (next.there()) fill(next, buffer ^ 1);
-    const char* const kt = lds + buffer * (2 * TILE);
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) fill(next[n], (buffer ^ HALVES) + n);
+    const Step own = now[half ? HALVES - 1 : 0];
+    const char* const kt = lds + (buffer + half) * (2 * TILE);
     const char* const vt = kt + TILE;
-    const int first = (int)(64 * now.tile);
-    const int* const document_s = reinterpret_cast<const int*>(lds + 4 * TILE + buffer * 256);
-    if (first < limit_w1) {
-asm volatile("" : "+v"(read.row_at), "+v"(read.tr_at));      // the offsets of a step are one operation from these: they are not to be kept in registers
+    const int first = (int)(64 * own.tile);
+    const int* const document_s = reinterpret_cast<const int*>(lds + SLOTS * (2 * TILE) + (buffer + half) * 256);
+    if ((HALVES == 1 || own.there()) && first < limit_w1) {
+      asm volatile("" : "+v"(read.row_at), "+v"(read.tr_at));      // the offsets of a step are one operation from these: they are not to be kept in registers
       // The operands that the products read from LDS, in their order: rows of K and of V for either half of the keys, then columns of K
       const auto operand = [&](unsigned j) {
         if (j < 4 * KS) return read.rows(j / KS % 2 ? vt : kt, j / (2 * KS), j % KS);
@@ -625,7 +686,7 @@ asm volatile("" : "+v"(read.row_at), "+v"(read.tr_at));      // the offsets of a
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[kb2][r] = 8 * (r / 4) + r % 4 < end ? s[kb2][r] : 0.0f;
         }
-        if (DOCS && now.compare) {
+        if (DOCS && own.compare) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int4v d = *reinterpret_cast<const int4v*>(document_s + 32 * kb2 + 8 * g + 4 * lhi);
@@ -671,8 +732,17 @@ asm volatile("" : "+v"(read.row_at), "+v"(read.tr_at));      // the offsets of a
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    now = next;
-    buffer ^= 1;
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) now[n] = next[n];
+    buffer ^= HALVES;
+  }
+  if constexpr (HALVES == 2) {      // the second half's sums through LDS, in the tiles' place
+    __syncthreads();
+    float4v* const sums_s = reinterpret_cast<float4v*>(lds) + (wave % RW) * (64 * 4 * DB);
+    if (half) put<DB>(dq, sums_s, lane, 1.0f);
+    __syncthreads();
+    if (half) return;
+    add<DB>(dq, 1.0f, sums_s, lane, 1.0f);
   }
   elt_t* const row = i < a.queries ? static_cast<elt_t*>(a.dq) + (size_t)b * a.sdq.batch + (size_t)i * a.sdq.token + (size_t)h * a.sdq.head : nullptr;
   store_columns<DB>(dq, row, lane, a.head, (CAP ? 4.0f : 1.0f) * a.scores.scale / up);
@@ -682,31 +752,40 @@ asm volatile("" : "+v"(read.row_at), "+v"(read.tr_at));      // the offsets of a
 
 hipError_t lego_attention_bwd_f16_d128_launch(const AttentionArgs& a, hipStream_t stream)
 {
-  const auto launch = [&](auto kernel, unsigned blocks) {
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
+  // as for the forward kernel
+  const auto launch = [&](auto whole, auto halves, int rows, unsigned of) {
+    const unsigned blocks = (unsigned)((rows + 32 * WAVES - 1) / (32 * WAVES)) * of;
+    if (blocks > 256) hipLaunchKernelGGL(whole, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
+    else hipLaunchKernelGGL(halves, dim3((unsigned)((rows + 16 * WAVES - 1) / (16 * WAVES)) * of), dim3(64 * WAVES), 0, stream, a);
     return hipGetLastError();
   };
-  const auto both = [&](auto dkv, auto dq) {
-    const unsigned own = 32 * WAVES, keys = ((unsigned)a.keys + own - 1) / own, queries = (unsigned)(a.queries + 32 * WAVES - 1) / (32 * WAVES);
-    const unsigned blocks = keys * (unsigned)(a.heads / a.heads_per_part) * (unsigned)a.batch;
-    const hipError_t e = launch(dkv, blocks);
-    return e != hipSuccess ? e : launch(dq, queries * (unsigned)a.heads * (unsigned)a.batch);
+  const auto both = [&](auto dkv, auto dkv_halves, auto dq, auto dq_halves) {
+    const hipError_t e = launch(dkv, dkv_halves, a.keys, (unsigned)(a.heads / a.heads_per_part) * (unsigned)a.batch);
+    return e != hipSuccess ? e : launch(dq, dq_halves, a.queries, (unsigned)(a.heads * a.batch));
   };
   if ((a.capped != 0) == true && (a.slopes != nullptr) == true && (a.documents != nullptr) == true)
-    return both(lego_attention_dkv_f16_d128_kernel<true, true, true>, lego_attention_dq_f16_d128_kernel<true, true, true>);
+    return both(lego_attention_dkv_f16_d128_kernel<true, true, true, 1>, lego_attention_dkv_f16_d128_kernel<true, true, true, 2>,
+                lego_attention_dq_f16_d128_kernel<true, true, true, 1>, lego_attention_dq_f16_d128_kernel<true, true, true, 2>);
   if ((a.capped != 0) == true && (a.slopes != nullptr) == true && (a.documents != nullptr) == false)
-    return both(lego_attention_dkv_f16_d128_kernel<true, true, false>, lego_attention_dq_f16_d128_kernel<true, true, false>);
+    return both(lego_attention_dkv_f16_d128_kernel<true, true, false, 1>, lego_attention_dkv_f16_d128_kernel<true, true, false, 2>,
+                lego_attention_dq_f16_d128_kernel<true, true, false, 1>, lego_attention_dq_f16_d128_kernel<true, true, false, 2>);
   if ((a.capped != 0) == true && (a.slopes != nullptr) == false && (a.documents != nullptr) == true)
-    return both(lego_attention_dkv_f16_d128_kernel<true, false, true>, lego_attention_dq_f16_d128_kernel<true, false, true>);
+    return both(lego_attention_dkv_f16_d128_kernel<true, false, true, 1>, lego_attention_dkv_f16_d128_kernel<true, false, true, 2>,
+                lego_attention_dq_f16_d128_kernel<true, false, true, 1>, lego_attention_dq_f16_d128_kernel<true, false, true, 2>);
   if ((a.capped != 0) == true && (a.slopes != nullptr) == false && (a.documents != nullptr) == false)
-    return both(lego_attention_dkv_f16_d128_kernel<true, false, false>, lego_attention_dq_f16_d128_kernel<true, false, false>);
+    return both(lego_attention_dkv_f16_d128_kernel<true, false, false, 1>, lego_attention_dkv_f16_d128_kernel<true, false, false, 2>,
+                lego_attention_dq_f16_d128_kernel<true, false, false, 1>, lego_attention_dq_f16_d128_kernel<true, false, false, 2>);
   if ((a.capped != 0) == false && (a.slopes != nullptr) == true && (a.documents != nullptr) == true)
-    return both(lego_attention_dkv_f16_d128_kernel<false, true, true>, lego_attention_dq_f16_d128_kernel<false, true, true>);
+    return both(lego_attention_dkv_f16_d128_kernel<false, true, true, 1>, lego_attention_dkv_f16_d128_kernel<false, true, true, 2>,
+                lego_attention_dq_f16_d128_kernel<false, true, true, 1>, lego_attention_dq_f16_d128_kernel<false, true, true, 2>);
   if ((a.capped != 0) == false && (a.slopes != nullptr) == true && (a.documents != nullptr) == false)
-    return both(lego_attention_dkv_f16_d128_kernel<false, true, false>, lego_attention_dq_f16_d128_kernel<false, true, false>);
+    return both(lego_attention_dkv_f16_d128_kernel<false, true, false, 1>, lego_attention_dkv_f16_d128_kernel<false, true, false, 2>,
+                lego_attention_dq_f16_d128_kernel<false, true, false, 1>, lego_attention_dq_f16_d128_kernel<false, true, false, 2>);
   if ((a.capped != 0) == false && (a.slopes != nullptr) == false && (a.documents != nullptr) == true)
-    return both(lego_attention_dkv_f16_d128_kernel<false, false, true>, lego_attention_dq_f16_d128_kernel<false, false, true>);
+    return both(lego_attention_dkv_f16_d128_kernel<false, false, true, 1>, lego_attention_dkv_f16_d128_kernel<false, false, true, 2>,
+                lego_attention_dq_f16_d128_kernel<false, false, true, 1>, lego_attention_dq_f16_d128_kernel<false, false, true, 2>);
   if ((a.capped != 0) == false && (a.slopes != nullptr) == false && (a.documents != nullptr) == false)
-    return both(lego_attention_dkv_f16_d128_kernel<false, false, false>, lego_attention_dq_f16_d128_kernel<false, false, false>);
+    return both(lego_attention_dkv_f16_d128_kernel<false, false, false, 1>, lego_attention_dkv_f16_d128_kernel<false, false, false, 2>,
+                lego_attention_dq_f16_d128_kernel<false, false, false, 1>, lego_attention_dq_f16_d128_kernel<false, false, false, 2>);
   return hipErrorInvalidValue;
 }

@@ -252,6 +252,28 @@ __device__ __forceinline__ void store_columns(const float16v (&acc)[BLOCKS], elt
     }
 }
 
+// A wave's sums into LDS, times a factor, and another wave's added to them.
+template <unsigned BLOCKS>
+__device__ __forceinline__ void put(const float16v (&acc)[BLOCKS], float4v* to, unsigned lane, float factor)
+{
+#pragma unroll
+  for (unsigned db = 0; db < BLOCKS; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) to[(4 * db + g) * 64 + lane] = factor * float4v{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+}
+template <unsigned BLOCKS>
+__device__ __forceinline__ void add(float16v (&acc)[BLOCKS], float factor, const float4v* from, unsigned lane, float other)
+{
+#pragma unroll
+  for (unsigned db = 0; db < BLOCKS; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4v x = from[(4 * db + g) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[db][4 * g + e] = factor * acc[db][4 * g + e] + other * x[e];
+    }
+}
+
 }  // namespace
 
 namespace {
@@ -260,18 +282,19 @@ namespace {
 constexpr float kLazy = 8.0f;
 constexpr unsigned RING = 4;      // operands read ahead
 
-template <bool CAP, bool BIAS, bool DOCS>
+template <bool CAP, bool BIAS, bool DOCS, unsigned HALVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d128_kernel(AttentionArgs a)
 {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE + 512];      // K and V, twice; the keys' documents, twice
-  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32;
-  const unsigned blocks = (a.queries + 32 * WAVES - 1) / (32 * WAVES);
+  constexpr unsigned RW = WAVES / HALVES, OWN = 32 * RW, SLOTS = 2 * HALVES;      // wavefronts of other rows than the others; queries of the workgroup; tiles in LDS
+  __shared__ __attribute__((aligned(1024))) char lds[SLOTS * (2 * TILE + 256)];      // K and V, then the keys' documents
+  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32, half = wave / RW;
+  const unsigned blocks = (a.queries + OWN - 1) / OWN;
   const unsigned all_heads = a.heads * a.batch, block = blocks - 1 - blockIdx.x / all_heads;      // later queries may see more keys
   const unsigned head = place(blockIdx.x % all_heads, all_heads);
   const unsigned h = head % a.heads, b = head / a.heads;
   const unsigned hk = h / (a.heads / a.key_heads);
-  const int q0 = (int)(32 * WAVES * block), q_last = min(q0 + 32 * (int)WAVES, a.queries) - 1;
-  const int w0 = q0 + 32 * (int)wave;                      // the wavefront's first query
+  const int q0 = (int)(OWN * block), q_last = min(q0 + (int)OWN, a.queries) - 1;
+  const int w0 = q0 + 32 * (int)(wave % RW);                      // the wavefront's first query
   const int i = w0 + (int)l32;                              // the lane's query
   const Seen seen{a.keys, a.keys - a.queries, a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : -1};
   const int limit = seen.limit(i), limit_w0 = seen.limit(w0), limit_w1 = seen.limit(min(w0 + 31, q_last));
@@ -306,10 +329,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d128_ke
   const Reader read(lane);
   typedef __attribute__((address_space(3))) void* lds_ptr;
   const unsigned lds_at = (unsigned)(uintptr_t)(lds_ptr)lds + wave * 1024;
-  const auto fill = [&](const Step& step, unsigned buffer) {
+  const auto fill = [&](const Step& step, unsigned slot) {
+    if (!step.there()) return;
     const unsigned first = 64 * step.tile, rows = a.keys - first;
-    const unsigned at = lds_at + buffer * (2 * TILE);
-    if (DOCS && step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + 4 * TILE + buffer * 256);
+    const unsigned at = lds_at + slot * (2 * TILE);
+    if (DOCS && step.compare && wave == 0) fill_words(documents + first, rows, lane, lds_at + SLOTS * (2 * TILE) + slot * 256);
     // padding among the keys is read as zeros, whatever it holds
     const auto skip = [&](unsigned row) { return DOCS && step.padded && documents[min(first + row, (unsigned)a.keys - 1)] < 0; };
     fill_k(lane, wave, first, rows, at, skip);
@@ -322,19 +346,28 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d128_ke
   for (unsigned db = 0; db < DB; ++db) acc[db] = zeros();
   float most = -INFINITY, sum = 0.0f;      // of the lane's own keys; the halves agree on `most`
   Walk<DOCS, decltype(look)> walk(look, lane, 0, (unsigned)(seen.limit(q_last) + 63) / 64);
-  Step now = walk.next();
+  // the walk's tiles in turn for the halves of the workgroup
+  Step now[HALVES];
   unsigned buffer = 0;
-  if (now.there()) fill(now, 0);
-  while (now.there()) {
-    const Step next = walk.next();
+#pragma unroll
+  for (unsigned n = 0; n < HALVES; ++n) {
+    now[n] = walk.next();
+    fill(now[n], n);
+  }
+  while (now[0].there()) {
+    Step next[HALVES];
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) next[n] = walk.next();
     wait_for_copies();
-    __syncthreads();                       // the tile is there, and the other buffer is read no more
-    if (next.there()) fill(next, buffer ^ 1);
-    const char* const kt = lds + buffer * (2 * TILE);
+    __syncthreads();                       // the tiles are there, and the other buffers are read no more
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) fill(next[n], (buffer ^ HALVES) + n);
+    const Step own = now[half ? HALVES - 1 : 0];
+    const char* const kt = lds + (buffer + half) * (2 * TILE);
     const char* const vt = kt + TILE;
-    const int first = (int)(64 * now.tile);
-    const int* const document_s = reinterpret_cast<const int*>(lds + 4 * TILE + buffer * 256);
-    if (first < limit_w1) {
+    const int first = (int)(64 * own.tile);
+    const int* const document_s = reinterpret_cast<const int*>(lds + SLOTS * (2 * TILE) + (buffer + half) * 256);
+    if ((HALVES == 1 || own.there()) && first < limit_w1) {
       float16v s[2] = {zeros(), zeros()};
 #pragma unroll
       for (unsigned ks = 0; ks < KS; ++ks)
@@ -372,7 +405,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d128_ke
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[kb2][r] = (int)(32 * kb2 + 8 * (r / 4) + r % 4) < end ? s[kb2][r] : -INFINITY;
       }
-      if (DOCS && now.compare) {
+      if (DOCS && own.compare) {
 #pragma unroll
         for (unsigned kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
@@ -422,10 +455,30 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d128_ke
       }
       sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
-    now = next;
-    buffer ^= 1;
+#pragma unroll
+    for (unsigned n = 0; n < HALVES; ++n) now[n] = next[n];
+    buffer ^= HALVES;
   }
   sum = across_sum(sum);
+  most *= unit;      // in units of log2 from here on
+  if constexpr (HALVES == 2) {      // the second half's sums through LDS, in the tiles' place
+    __syncthreads();
+    float4v* const acc_s = reinterpret_cast<float4v*>(lds) + (wave % RW) * (64 * 4 * DB);
+    float2* const stat_s = reinterpret_cast<float2*>(lds + RW * (64 * 16 * DB * 4)) + (wave % RW) * 64;
+    static_assert(RW * (64 * 16 * DB * 4 + 64 * 8) <= SLOTS * 2 * TILE, "sums of the second half in the tiles' place");
+    if (half) {
+      put<DB>(acc, acc_s, lane, 1.0f);
+      stat_s[lane] = float2{most, sum};
+    }
+    __syncthreads();
+    if (half) return;
+    const float2 o = stat_s[lane];
+    const float top = fmaxf(most, o.x);
+    const float f0 = most == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(most - top), f1 = o.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(o.x - top);
+    most = top;
+    sum = f0 * sum + f1 * o.y;
+    add<DB>(acc, f0, acc_s, lane, f1);
+  }
   const size_t row_at = (size_t)b * a.so.batch + (size_t)min(i, a.queries - 1) * a.so.token + (size_t)h * a.so.head;
   const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -440,25 +493,33 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_bf16_d128_ke
       for (int r = 0; r < 16; ++r) acc[db][r] -= static_cast<float>(static_cast<elt_t>(acc[db][r]));
     store_columns<DB>(acc, i < a.queries ? static_cast<elt_t*>(a.o_rest) + row_at : nullptr, lane, a.head, 1.0f);
   }
-  if (i < a.queries && lhi == 0) a.lse[((size_t)b * a.heads + h) * a.queries + i] = sum == 0.0f ? -INFINITY : kLn2 * (unit * most + __builtin_amdgcn_logf(sum));
+  if (i < a.queries && lhi == 0) a.lse[((size_t)b * a.heads + h) * a.queries + i] = sum == 0.0f ? -INFINITY : kLn2 * (most + __builtin_amdgcn_logf(sum));
 }
 
 }  // namespace
 
 hipError_t lego_attention_fwd_bf16_d128_launch(const AttentionArgs& a, hipStream_t stream)
 {
-  const unsigned blocks = (unsigned)((a.queries + 32 * WAVES - 1) / (32 * WAVES)) * (unsigned)a.heads * (unsigned)a.batch;
-  const auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
+  // As many workgroups as the chip holds with twice the tiles in LDS, or fewer: half of the rows each, and the tiles in turn for the halves of its wavefronts, so that a row's way through the keys
+  // is half as long.  Measured (bf16, heads of 128, causal, slopes; forward and backward, us): 4 heads of 1531 tokens, 48
+  // workgroups, 39 + 122 -> 28 + 74; 4 heads of 8192, 256, 232 + 592 -> 154 + 378; 36 heads of 1531, 432, 51 + 158 -> 68 + 172.
+  const unsigned heads = (unsigned)(a.heads * a.batch), blocks = (unsigned)((a.queries + 32 * WAVES - 1) / (32 * WAVES)) * heads;
+  const auto launch = [&](auto whole, auto halves) {
+    if (blocks > 256) hipLaunchKernelGGL(whole, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
+    else hipLaunchKernelGGL(halves, dim3((unsigned)((a.queries + 16 * WAVES - 1) / (16 * WAVES)) * heads), dim3(64 * WAVES), 0, stream, a);
     return hipGetLastError();
   };
   if ((a.capped != 0) == true && (a.slopes != nullptr) == true)
-    return a.documents ? launch(lego_attention_fwd_bf16_d128_kernel<true, true, true>) : launch(lego_attention_fwd_bf16_d128_kernel<true, true, false>);
+    return a.documents ? launch(lego_attention_fwd_bf16_d128_kernel<true, true, true, 1>, lego_attention_fwd_bf16_d128_kernel<true, true, true, 2>)
+                       : launch(lego_attention_fwd_bf16_d128_kernel<true, true, false, 1>, lego_attention_fwd_bf16_d128_kernel<true, true, false, 2>);
   if ((a.capped != 0) == true && (a.slopes != nullptr) == false)
-    return a.documents ? launch(lego_attention_fwd_bf16_d128_kernel<true, false, true>) : launch(lego_attention_fwd_bf16_d128_kernel<true, false, false>);
+    return a.documents ? launch(lego_attention_fwd_bf16_d128_kernel<true, false, true, 1>, lego_attention_fwd_bf16_d128_kernel<true, false, true, 2>)
+                       : launch(lego_attention_fwd_bf16_d128_kernel<true, false, false, 1>, lego_attention_fwd_bf16_d128_kernel<true, false, false, 2>);
   if ((a.capped != 0) == false && (a.slopes != nullptr) == true)
-    return a.documents ? launch(lego_attention_fwd_bf16_d128_kernel<false, true, true>) : launch(lego_attention_fwd_bf16_d128_kernel<false, true, false>);
+    return a.documents ? launch(lego_attention_fwd_bf16_d128_kernel<false, true, true, 1>, lego_attention_fwd_bf16_d128_kernel<false, true, true, 2>)
+                       : launch(lego_attention_fwd_bf16_d128_kernel<false, true, false, 1>, lego_attention_fwd_bf16_d128_kernel<false, true, false, 2>);
   if ((a.capped != 0) == false && (a.slopes != nullptr) == false)
-    return a.documents ? launch(lego_attention_fwd_bf16_d128_kernel<false, false, true>) : launch(lego_attention_fwd_bf16_d128_kernel<false, false, false>);
+    return a.documents ? launch(lego_attention_fwd_bf16_d128_kernel<false, false, true, 1>, lego_attention_fwd_bf16_d128_kernel<false, false, true, 2>)
+                       : launch(lego_attention_fwd_bf16_d128_kernel<false, false, false, 1>, lego_attention_fwd_bf16_d128_kernel<false, false, false, 2>);
   return hipErrorInvalidValue;
 }

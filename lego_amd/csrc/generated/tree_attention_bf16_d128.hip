@@ -251,6 +251,28 @@ __device__ __forceinline__ void store_columns(const float16v (&acc)[BLOCKS], elt
     }
 }
 
+// A wave's sums into LDS, times a factor, and another wave's added to them.
+template <unsigned BLOCKS>
+__device__ __forceinline__ void put(const float16v (&acc)[BLOCKS], float4v* to, unsigned lane, float factor)
+{
+#pragma unroll
+  for (unsigned db = 0; db < BLOCKS; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) to[(4 * db + g) * 64 + lane] = factor * float4v{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+}
+template <unsigned BLOCKS>
+__device__ __forceinline__ void add(float16v (&acc)[BLOCKS], float factor, const float4v* from, unsigned lane, float other)
+{
+#pragma unroll
+  for (unsigned db = 0; db < BLOCKS; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4v x = from[(4 * db + g) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[db][4 * g + e] = factor * acc[db][4 * g + e] + other * x[e];
+    }
+}
+
 }  // namespace
 
 namespace {

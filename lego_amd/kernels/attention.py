@@ -95,7 +95,7 @@ def emit():
     for dt, elt in ELEMENTS.items():
         for head in HEADS:
             params = dict(_tile_params(head, WAVES), banner=BANNER, elt=elt, dt=dt, tag=f"{dt}_d{head}", place=place, launch_layout=launch,
-                          PSHIFT=PSHIFT[dt], RING=3 if head == 128 else 4)
+                          PSHIFT=PSHIFT[dt], RING=3 if head == 128 else 4, FEW=512 if head == 64 else 256)
             params |= dict(LEAST=TREE_LEAST, JOIN_ROWS=JOIN_ROWS, JOIN_MANY=JOIN_MANY, JOIN_FEW=JOIN_FEW, PIECE=TREE_PIECE)
             units.append(Emitted(f"tree_attention_{dt}_d{head}.hip", template("tree_attention.hip.j2").render(**params), [f"lego_tree_{dt}_d{head}_launch"]))
             for way in ("fwd", "bwd"):

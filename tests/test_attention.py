@@ -203,6 +203,19 @@ def test_prefix(queries, keys, documents, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("kind", ["all", "scores", "documents", "prefix"])
+def test_more_heads_than_the_chip_holds(kind, dim, dtype):
+    """From some number of workgroups on they are not cut in halves: two blocks of each of 264 heads."""
+    q, k, v, dout = make(2, 150, 150, 132, 66, dim, dtype, seed=13)
+    how = {"all": {}, "scores": dict(causal=True, softcap=6.0, slopes=torch.linspace(0, 0.5, 132).cuda()),
+           "documents": dict(causal=True, documents=torch.tensor([pack([30, 71, 40], 9), pack([150])], dtype=torch.int32, device="cuda")),
+           "prefix": dict(causal=True, prefix=torch.tensor([70, 0], dtype=torch.int32, device="cuda"))}[kind]
+    check(q, k, v, dout, **how)
+
+
+@pytest.mark.gpu
 def test_prefix_below_zero_is_none():
     q, k, v, _ = make(2, 70, 70, 2, 2, 64, torch.bfloat16)
     with_none = ops.attention(q, k, v, causal=True)
