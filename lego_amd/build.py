@@ -316,10 +316,11 @@ def collect():
     h += [f"hipError_t lego_attention_{way}_{d}_d{head}_launch(const AttentionArgs&, hipStream_t);"
           for way in ("fwd", "bwd") for d in mat["ELEMENTS"] for head in mat["HEADS"]]
     h += ["hipError_t lego_attention_tiles_launch(const int*, int2*, int, int, hipStream_t);",
+          "hipError_t lego_attention_order_launch(const AttentionArgs&, hipStream_t);",
           "hipError_t lego_attention_delta_launch(const AttentionArgs&, int, hipStream_t);",
           "hipError_t lego_attention_join_launch(const AttentionArgs&, int, hipStream_t);",
           "hipError_t lego_rotary_launch(const RotaryArgs&, int, int, int, int, hipStream_t);",
-          f"#define LEGO_ATTENTION_MAX_HEAD {mat['MAX_HEAD']}", f"#define LEGO_ROTARY_MAX_PART {mro['MOST']}", ""]
+          f"#define LEGO_ATTENTION_MAX_HEAD {mat['MAX_HEAD']}", f"#define LEGO_ATTENTION_ORDERED {mat['ORDERED']}", f"#define LEGO_ROTARY_MAX_PART {mro['MOST']}", ""]
     return units, "\n".join(h)
 
 

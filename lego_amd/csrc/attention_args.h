@@ -23,6 +23,7 @@ struct AttentionArgs {
   const float* slopes;          // [head], or null
   const int* documents;         // [batch][key], or null
   int2* tiles;                  // [batch][tile of 64 keys]: lowest and highest document
+  int *order_queries, *order_keys;      // [batch][block of 128]: the blocks with the most work first, or null: as they come
   const int* prefix;            // [batch], or null
   float* parts;                 // dk and dv of parts of the query heads that share a key head: [part][dk, dv][batch][key head][key][head element], or null
   Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
@@ -30,6 +31,7 @@ struct AttentionArgs {
   int batch, queries, keys, heads, key_heads, head;
   int causal, capped;
   int heads_per_part;           // query heads whose sums one workgroup forms
+  int halve_queries, halve_keys;      // workgroups of 64 and not 128 of them, whose wavefronts share the tiles out in halves
 };
 
 struct RotaryArgs {

@@ -290,8 +290,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dkv_bf16_d96_ker
   __shared__ __attribute__((aligned(1024))) char lds[SLOTS * (2 * TILE + 768)];      // Q and dO, then lse, delta and documents
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32, half = wave / RW;
   const unsigned blocks = (a.keys + OWN - 1) / OWN, group = a.heads / a.key_heads, parts = group / a.heads_per_part;
-  const unsigned all_parts = parts * a.key_heads * a.batch, turn = blockIdx.x % all_parts, block = blockIdx.x / all_parts;      // earlier keys may be seen by more queries
-  const unsigned at_part = place(turn, all_parts), part = at_part % parts, hk = at_part / parts % a.key_heads, b = at_part / parts / a.key_heads;
+  const unsigned all_parts = parts * a.key_heads * a.batch, turn = blockIdx.x / all_parts;
+  const unsigned at_part = place(blockIdx.x % all_parts, all_parts), part = at_part % parts, hk = at_part / parts % a.key_heads, b = at_part / parts / a.key_heads;
+  const unsigned block = DOCS && a.order_keys ? __builtin_amdgcn_readfirstlane(a.order_keys[b * blocks + turn]) : turn;      // earlier keys may be seen by more queries
   const int k0 = (int)(OWN * block), k_last = min(k0 + (int)OWN, a.keys) - 1;
   const int w0 = k0 + (int)(32 * (wave % RW)), key = w0 + (int)l32;
   const int shift = a.keys - a.queries, prefix = a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : a.keys;
@@ -548,9 +549,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kern
   __shared__ __attribute__((aligned(1024))) char lds[SLOTS * (2 * TILE + 256)];      // K and V, then the keys' documents
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32, half = wave / RW;
   const unsigned blocks = (a.queries + OWN - 1) / OWN;
-  const unsigned all_heads = a.heads * a.batch, block = blocks - 1 - blockIdx.x / all_heads;      // later queries may see more keys
+  const unsigned all_heads = a.heads * a.batch, turn = blockIdx.x / all_heads;
   const unsigned head = place(blockIdx.x % all_heads, all_heads);
   const unsigned h = head % a.heads, b = head / a.heads;
+  const unsigned block = DOCS && a.order_queries ? __builtin_amdgcn_readfirstlane(a.order_queries[b * blocks + turn]) : blocks - 1 - turn;      // later queries may see more keys
   const unsigned hk = h / (a.heads / a.key_heads);
   const int q0 = (int)(OWN * block), q_last = min(q0 + (int)OWN, a.queries) - 1;
   const int w0 = q0 + 32 * (int)(wave % RW), i = w0 + (int)l32;
@@ -731,16 +733,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_dq_bf16_d96_kern
 
 hipError_t lego_attention_bwd_bf16_d96_launch(const AttentionArgs& a, hipStream_t stream)
 {
-  // as for the forward kernel
-  const auto launch = [&](auto whole, auto halves, int rows, unsigned of) {
-    const unsigned blocks = (unsigned)((rows + 32 * WAVES - 1) / (32 * WAVES)) * of;
-    if (blocks > 256) hipLaunchKernelGGL(whole, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
-    else hipLaunchKernelGGL(halves, dim3((unsigned)((rows + 16 * WAVES - 1) / (16 * WAVES)) * of), dim3(64 * WAVES), 0, stream, a);
+  const auto launch = [&](auto whole, auto halves, bool halve, int rows, unsigned of) {
+    const unsigned own = halve ? 16 * WAVES : 32 * WAVES;
+    hipLaunchKernelGGL(halve ? halves : whole, dim3(((unsigned)rows + own - 1) / own * of), dim3(64 * WAVES), 0, stream, a);
     return hipGetLastError();
   };
   const auto both = [&](auto dkv, auto dkv_halves, auto dq, auto dq_halves) {
-    const hipError_t e = launch(dkv, dkv_halves, a.keys, (unsigned)(a.heads / a.heads_per_part) * (unsigned)a.batch);
-    return e != hipSuccess ? e : launch(dq, dq_halves, a.queries, (unsigned)(a.heads * a.batch));
+    const hipError_t e = launch(dkv, dkv_halves, a.halve_keys != 0, a.keys, (unsigned)(a.heads / a.heads_per_part) * (unsigned)a.batch);
+    return e != hipSuccess ? e : launch(dq, dq_halves, a.halve_queries != 0, a.queries, (unsigned)(a.heads * a.batch));
   };
   if ((a.capped != 0) == true && (a.slopes != nullptr) == true && (a.documents != nullptr) == true)
     return both(lego_attention_dkv_bf16_d96_kernel<true, true, true, 1>, lego_attention_dkv_bf16_d96_kernel<true, true, true, 2>,

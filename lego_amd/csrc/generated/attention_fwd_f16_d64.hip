@@ -289,9 +289,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
   __shared__ __attribute__((aligned(1024))) char lds[SLOTS * (2 * TILE + 256)];      // K and V, then the keys' documents
   const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l32 = lane % 32, lhi = lane / 32, half = wave / RW;
   const unsigned blocks = (a.queries + OWN - 1) / OWN;
-  const unsigned all_heads = a.heads * a.batch, block = blocks - 1 - blockIdx.x / all_heads;      // later queries may see more keys
+  const unsigned all_heads = a.heads * a.batch, turn = blockIdx.x / all_heads;
   const unsigned head = place(blockIdx.x % all_heads, all_heads);
   const unsigned h = head % a.heads, b = head / a.heads;
+  const unsigned block = DOCS && a.order_queries ? __builtin_amdgcn_readfirstlane(a.order_queries[b * blocks + turn]) : blocks - 1 - turn;      // later queries may see more keys
   const unsigned hk = h / (a.heads / a.key_heads);
   const int q0 = (int)(OWN * block), q_last = min(q0 + (int)OWN, a.queries) - 1;
   const int w0 = q0 + 32 * (int)(wave % RW);                      // the wavefront's first query
@@ -500,12 +501,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) lego_attention_fwd_f16_d64_kern
 
 hipError_t lego_attention_fwd_f16_d64_launch(const AttentionArgs& a, hipStream_t stream)
 {
-  // As many workgroups as the chip holds with twice the tiles in LDS, or fewer: half of the rows each, and the tiles in turn for the halves of its wavefronts, so that a row's way through the keys
-  // is half as long.  Measured (f16, heads of 64, causal, slopes; forward and backward, us): 4 heads of 1531 tokens, 48 workgroups, 30.5 + 82 -> 19.8 + 54; 36 heads, 432, 39 + 97 -> 33 + 86; 64 heads, 768, 43 + 118 -> 47 + 128.
-  const unsigned heads = (unsigned)(a.heads * a.batch), blocks = (unsigned)((a.queries + 32 * WAVES - 1) / (32 * WAVES)) * heads;
   const auto launch = [&](auto whole, auto halves) {
-    if (blocks > 512) hipLaunchKernelGGL(whole, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
-    else hipLaunchKernelGGL(halves, dim3((unsigned)((a.queries + 16 * WAVES - 1) / (16 * WAVES)) * heads), dim3(64 * WAVES), 0, stream, a);
+    const unsigned own = a.halve_queries ? 16 * WAVES : 32 * WAVES, blocks = ((unsigned)a.queries + own - 1) / own * (unsigned)(a.heads * a.batch);
+    hipLaunchKernelGGL(a.halve_queries ? halves : whole, dim3(blocks), dim3(64 * WAVES), 0, stream, a);
     return hipGetLastError();
   };
   if ((a.capped != 0) == true && (a.slopes != nullptr) == true)

@@ -30,6 +30,40 @@ __global__ void __launch_bounds__(256) lego_attention_tiles_kernel(const int* __
   if (lane == 0) tiles[at] = int2{low, high};
 }
 
+// The blocks of 128 queries (blockIdx.y 0) or keys (1) of a batch by the tiles that they share a document with, the most first.  A launch of few rounds of workgroups ends when its last heavy one does: for
+// 16 heads of 8192 tokens in 7 documents, 1024 workgroups in two rounds, forward 98 -> 84 us, dk and dv 191 -> 167, dq 146 -> 129 at 6 a launch.
+__global__ void __launch_bounds__(1024) lego_attention_order_kernel(AttentionArgs a)
+{
+  __shared__ unsigned work_s[512];
+  const unsigned b = blockIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const bool of_keys = blockIdx.y != 0;
+  int* const order = of_keys ? a.order_keys : a.order_queries;
+  if (!order) return;
+  const int rows = of_keys ? a.keys : a.queries, shift = a.keys - a.queries, prefix = a.causal ? (a.prefix ? max(a.prefix[b], 0) : 0) : a.keys;
+  const unsigned blocks = (unsigned)(rows + 127) / 128;
+  const int tiles = (a.keys + 63) / 64;
+  const int2* const at = a.tiles + (size_t)b * tiles;
+  for (unsigned block = wave; block < blocks; block += 16) {
+    const int r0 = (int)(128 * block), r1 = min(r0 + 128, rows) - 1, p0 = of_keys ? r0 : r0 + shift, p1 = of_keys ? r1 : r1 + shift;      // rows, positions
+    int2 own = at[p0 / 64];
+    for (int t = p0 / 64 + 1; t <= p1 / 64; ++t) own = int2{min(own.x, at[t].x), max(own.y, at[t].y)};
+    const int begin = of_keys ? max(p0 < prefix ? 0 : p0, shift) / 64 : 0, end = of_keys ? tiles : (min(a.keys, max(p1 + 1, prefix)) + 63) / 64;
+    unsigned work = 0;
+    for (int base = begin; base < end; base += 64) {
+      const int t = base + (int)lane;
+      const int2 other = t < end ? at[t] : int2{0, -1};
+      work += __popcll(__ballot(!(other.y < 0 || own.y < 0 || other.y < own.x || own.y < other.x)));
+    }
+    if (lane == 0) work_s[block] = work;
+  }
+  __syncthreads();
+  if (threadIdx.x >= blocks) return;
+  const unsigned own = work_s[threadIdx.x];
+  unsigned rank = 0;
+  for (unsigned j = 0; j < blocks; ++j) rank += work_s[j] > own || (work_s[j] == own && j < threadIdx.x);
+  order[b * blocks + rank] = (int)threadIdx.x;
+}
+
 // 64 queries of a head a workgroup, 16 lanes a query.
 template <class E>
 __global__ void __launch_bounds__(256) lego_attention_delta_kernel(AttentionArgs a, unsigned tiles, float shift)
@@ -110,6 +144,12 @@ hipError_t lego_attention_tiles_launch(const int* documents, int2* tiles, int ba
 {
   const unsigned count = (unsigned)batch * (((unsigned)keys + 63) / 64);
   hipLaunchKernelGGL(lego_attention_tiles_kernel, dim3((count + 3) / 4), dim3(256), 0, stream, documents, tiles, (unsigned)batch, (unsigned)keys);
+  return hipGetLastError();
+}
+
+hipError_t lego_attention_order_launch(const AttentionArgs& a, hipStream_t stream)
+{
+  hipLaunchKernelGGL(lego_attention_order_kernel, dim3((unsigned)a.batch, 2), dim3(1024), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -354,8 +354,10 @@ hipError_t lego_attention_bwd_bf16_d64_launch(const AttentionArgs&, hipStream_t)
 hipError_t lego_attention_bwd_bf16_d96_launch(const AttentionArgs&, hipStream_t);
 hipError_t lego_attention_bwd_bf16_d128_launch(const AttentionArgs&, hipStream_t);
 hipError_t lego_attention_tiles_launch(const int*, int2*, int, int, hipStream_t);
+hipError_t lego_attention_order_launch(const AttentionArgs&, hipStream_t);
 hipError_t lego_attention_delta_launch(const AttentionArgs&, int, hipStream_t);
 hipError_t lego_attention_join_launch(const AttentionArgs&, int, hipStream_t);
 hipError_t lego_rotary_launch(const RotaryArgs&, int, int, int, int, hipStream_t);
 #define LEGO_ATTENTION_MAX_HEAD 128
+#define LEGO_ATTENTION_ORDERED 512
 #define LEGO_ROTARY_MAX_PART 256

@@ -71,19 +71,48 @@ inline int heads_per_part(const AttentionArgs& a)
   return 1;
 }
 
-struct Room { size_t delta, less, ups, parts, all; };
+// As many workgroups of 128 rows as the chip holds with twice the tiles in LDS, or fewer: half of the rows each, and the tiles in turn for the halves of the wavefronts, so that a row's way through the
+// other side is half as long.  Measured, causal with slopes, forward + backward, us.  fp16 heads of 64: 4 of 1531 tokens, 48 workgroups, 30.5 + 82 -> 19.8 + 54; 36 of them, 432, 39 + 97 -> 33 + 86; 64
+// of them, 768, 43 + 118 -> 47 + 128, not cut.  bf16 heads of 128: 4 of 1531 tokens, 39 + 122 -> 28 + 74; 4 of 8192, 256 workgroups, 232 + 592 -> 154 + 378; 36 of 1531, 432, 51 + 158 -> 68 + 172, not cut.
+inline bool halve(const AttentionArgs& a, int rows, long long heads) { return (rows + 127) / 128 * heads <= (a.head <= 64 ? 512 : 256); }
+
+// With documents the blocks' work follows no rule: where there are several rounds of workgroups, but not so many that the last one counts for little, they are ordered by it.
+inline bool ordered(int rows) { return (rows + 127) / 128 <= LEGO_ATTENTION_ORDERED; }
+
+inline void plan_attention(AttentionArgs& a)
+{
+  a.heads_per_part = heads_per_part(a);
+  a.halve_queries = halve(a, a.queries, (long long)a.heads * a.batch);
+  a.halve_keys = halve(a, a.keys, (long long)(a.heads / a.heads_per_part) * a.batch);
+}
+
+struct Room { size_t order_queries, order_keys, delta, less, ups, parts, all; };
 inline Room room_of(const AttentionArgs& a, bool documents, bool backward)
 {
   Room r = {};
-  r.delta = r.all = documents ? tiles_bytes(a) : 0;
+  const bool queries = documents && !a.halve_queries && ordered(a.queries), keys = documents && backward && !a.halve_keys && ordered(a.keys);
+  r.order_queries = documents ? tiles_bytes(a) : 0;
+  r.order_keys = r.order_queries + (queries ? up16((size_t)a.batch * ((a.queries + 127) / 128) * sizeof(int)) : 0);
+  r.delta = r.all = r.order_keys + (keys ? up16((size_t)a.batch * ((a.keys + 127) / 128) * sizeof(int)) : 0);
   if (!backward) return r;
   const size_t rows = (size_t)a.batch * a.heads;
   r.less = r.delta + up16(rows * a.queries * sizeof(float));
   r.ups = r.less + up16(rows * a.queries * sizeof(float));
   r.parts = r.ups + up16(rows * ((a.queries + 63) / 64) * sizeof(float));
-  const int per = heads_per_part(a), parts = a.heads / a.key_heads / per;
+  const int parts = a.heads / a.key_heads / a.heads_per_part;
   r.all = r.parts + (parts > 1 ? (size_t)parts * 2 * a.batch * a.key_heads * a.keys * a.head * sizeof(float) : 0);
   return r;
+}
+
+// The passes over the documents, before the kernels that use them.
+inline hipError_t look_at_documents(AttentionArgs& a, const Room& room, void* workspace, hipStream_t stream)
+{
+  char* const at = static_cast<char*>(workspace);
+  a.tiles = reinterpret_cast<int2*>(at);
+  a.order_queries = room.order_keys > room.order_queries ? reinterpret_cast<int*>(at + room.order_queries) : nullptr;
+  a.order_keys = room.delta > room.order_keys ? reinterpret_cast<int*>(at + room.order_keys) : nullptr;
+  const hipError_t e = lego_attention_tiles_launch(a.documents, a.tiles, a.batch, a.keys, stream);
+  return e != hipSuccess || !(a.order_queries || a.order_keys) ? e : lego_attention_order_launch(a, stream);
 }
 
 inline hipError_t forward(const AttentionArgs& a, int element, hipStream_t stream)
@@ -193,6 +222,7 @@ int lego_hip_attention_workspace_bytes(const long long* sizes, int documents, in
 {
   AttentionArgs a = {};
   if (!bytes || !take_sizes(a, sizes)) return kInvalid;
+  plan_attention(a);
   *bytes = room_of(a, documents != 0, backward != 0).all;
   return 0;
 }
@@ -205,14 +235,12 @@ int lego_hip_attention_fwd(const void* q, const void* k, const void* v, void* ou
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (rest && !aligned16(rest)) || !lse || !aligned4(lse) || !strides || element < 0 || element > 1) return kInvalid;
   if (!take_sizes(a, sizes) || !take(a.sq, strides) || !take(a.sk, strides + 3) || !take(a.sv, strides + 6) || !take(a.so, strides + 9)) return kInvalid;
   if (!take_mask(a, scale, softcap, slopes, documents, prefix, causal)) return kInvalid;
-  if (documents && (!aligned16(workspace) || workspace_bytes < room_of(a, true, false).all)) return kInvalid;
+  plan_attention(a);
+  const Room room = room_of(a, documents != nullptr, false);
+  if (documents && (!aligned16(workspace) || workspace_bytes < room.all)) return kInvalid;
   a.q = q, a.k = k, a.v = v, a.o = out, a.o_rest = rest, a.lse = lse;
-  if (documents) {
-    a.tiles = static_cast<int2*>(workspace);
-    const hipError_t e = lego_attention_tiles_launch(documents, a.tiles, a.batch, a.keys, as_stream(stream));
-    if (e != hipSuccess) return (int)e;
-  }
-  return (int)forward(a, element, as_stream(stream));
+  const hipError_t e = documents ? look_at_documents(a, room, workspace, as_stream(stream)) : hipSuccess;
+  return e != hipSuccess ? (int)e : (int)forward(a, element, as_stream(stream));
 }
 
 int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const void* rest, const float* lse, void* dq, void* dk, void* dv,
@@ -227,14 +255,14 @@ int lego_hip_attention_bwd(const void* dout, const void* q, const void* k, const
   for (int t = 0; t < 8; ++t)
     if (!take(*into[t], strides + 3 * t)) return kInvalid;
   if (!take_mask(a, scale, softcap, slopes, documents, prefix, causal)) return kInvalid;
+  plan_attention(a);
   const Room room = room_of(a, documents != nullptr, true);
   if (!aligned16(workspace) || workspace_bytes < room.all) return kInvalid;
   char* const at = static_cast<char*>(workspace);
   a.q = q, a.k = k, a.v = v, a.out = out, a.rest = rest, a.dout = dout, a.lse = const_cast<float*>(lse), a.dq = dq, a.dk = dk, a.dv = dv;
-  a.tiles = reinterpret_cast<int2*>(at), a.delta = reinterpret_cast<float*>(at + room.delta), a.less = reinterpret_cast<float*>(at + room.less), a.ups = reinterpret_cast<float*>(at + room.ups);
+  a.delta = reinterpret_cast<float*>(at + room.delta), a.less = reinterpret_cast<float*>(at + room.less), a.ups = reinterpret_cast<float*>(at + room.ups);
   a.parts = room.all > room.parts ? reinterpret_cast<float*>(at + room.parts) : nullptr;
-  a.heads_per_part = heads_per_part(a);
-  hipError_t e = documents ? lego_attention_tiles_launch(documents, a.tiles, a.batch, a.keys, as_stream(stream)) : hipSuccess;
+  hipError_t e = documents ? look_at_documents(a, room, workspace, as_stream(stream)) : hipSuccess;
   if (e == hipSuccess) e = lego_attention_delta_launch(a, element, as_stream(stream));
   if (e == hipSuccess) e = backward(a, element, as_stream(stream));
   if (e == hipSuccess && a.parts) e = lego_attention_join_launch(a, element, as_stream(stream));

@@ -216,6 +216,18 @@ def test_more_heads_than_the_chip_holds(kind, dim, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries", [520, 390])
+@pytest.mark.parametrize("kind", ["packed", "unordered", "padded"])
+def test_documents_in_order_of_their_work(kind, queries, causal):
+    """Five blocks (four of queries) of each of 66 heads, the ones with the most work first."""
+    rows = {"packed": pack([200, 3, 300, 17]), "unordered": torch.randint(0, 4, (520,), generator=torch.Generator().manual_seed(5)).tolist(), "padded": pack([129, 200], 191)}[kind]
+    documents = torch.tensor([rows], dtype=torch.int32, device="cuda")
+    prefix = torch.tensor([250], dtype=torch.int32, device="cuda") if causal and kind == "packed" else None
+    check(*make(1, queries, 520, 66, 66, 128, torch.bfloat16, seed=21), causal=causal, documents=documents, prefix=prefix)
+
+
+@pytest.mark.gpu
 def test_prefix_below_zero_is_none():
     q, k, v, _ = make(2, 70, 70, 2, 2, 64, torch.bfloat16)
     with_none = ops.attention(q, k, v, causal=True)
