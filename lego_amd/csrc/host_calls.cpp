@@ -9,11 +9,16 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
+#include <memory>
+#include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -294,6 +299,24 @@ at::Tensor attention_forward(const at::Tensor& q, const at::Tensor& k, const at:
                                 current_stream()) == 0 ? out : at::Tensor();
 }
 
+// Gradients whose own gradient may be asked for (create_graph): it is an error and not zero by what they came from.
+void once(variable_list& grads, const char* name, const variable_list& from)
+{
+  if (!at::GradMode::is_enabled()) return;
+  variable_list defined;
+  for (const at::Tensor& t : grads)
+    if (t.defined()) defined.push_back(t);
+  torch::autograd::edge_list edges = torch::autograd::collect_next_edges(from);
+  if (std::any_of(edges.begin(), edges.end(), [](const torch::autograd::Edge& e) { return e.is_valid(); }))
+    torch::autograd::set_history(defined, std::make_shared<torch::autograd::Error>(std::string(name) + " has no second derivative", std::move(edges)));
+}
+
+// A tensor that a node has saved and gets back through whatever hooks there are.
+bool as_saved(const at::Tensor& t, const at::Device& device, std::initializer_list<at::ScalarType> types, int64_t elements)
+{
+  return t.device() == device && std::find(types.begin(), types.end(), t.scalar_type()) != types.end() && t.numel() == elements;
+}
+
 struct Attention : torch::autograd::Function<Attention> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Mask& m)
   {
@@ -317,6 +340,8 @@ struct Attention : torch::autograd::Function<Attention> {
       TORCH_CHECK_VALUE(t.device() == dout.device() && t.scalar_type() == dout.scalar_type() && t.dim() == 4 && in_chunks(t), "the saved tensors must be as they were");
     TORCH_CHECK_VALUE(k.sizes() == v.sizes() && out.sizes() == q.sizes() && rest.sizes() == q.sizes() && out.is_contiguous() && rest.is_contiguous() && lse.is_contiguous() &&
                       lse.numel() == q.size(0) * q.size(1) * q.size(2) && lse.scalar_type() == at::kFloat && lse.device() == q.device(), "the saved tensors must be as they were");
+    const auto beside = [&](const at::Tensor& t, at::ScalarType type, int64_t elements) { return !t.defined() || (as_saved(t, q.device(), {type}, elements) && t.is_contiguous()); };
+    TORCH_CHECK_VALUE(beside(saved[6], at::kFloat, q.size(2)) && beside(saved[7], at::kInt, k.size(0) * k.size(1)) && beside(saved[8], at::kInt, q.size(0)), "the saved tensors must be as they were");
     const c10::DeviceGuard on(q.device());
     long long sizes[6], strides[24];
     attention_sizes(q, k, sizes);
@@ -332,7 +357,9 @@ struct Attention : torch::autograd::Function<Attention> {
                                             static_cast<const int*>(data(&saved[7])), static_cast<const int*>(data(&saved[8])), ctx->saved_data["causal"].toBool(),
                                             attention_element(q.scalar_type()), workspace.mutable_data_ptr(), need, current_stream());
     TORCH_CHECK(code == 0, "lego_hip_attention_bwd failed with hipError_t ", code);
-    return {dq, dk, dv, at::Tensor()};
+    variable_list all = {dq, dk, dv, at::Tensor()};
+    once(all, "attention", {q, k, v, grads[0]});
+    return all;
   }
 };
 
@@ -470,11 +497,17 @@ struct Rotary : torch::autograd::Function<Rotary> {
         TORCH_CHECK_VALUE(!t.defined() || (t.is_cuda() && t.dim() == 4 && t.scalar_type() == first.scalar_type() && t.device() == first.device() && rotary_element(t.scalar_type()) >= 0 &&
                                            t.size(1) == saved[0].size(-1) && t.size(3) >= 2 * saved[1].size(0) && (saved[0].dim() == 1 || t.size(0) == saved[0].size(0))),
                           "the gradients must have the shapes of q and k");
+      TORCH_CHECK_VALUE(!dq.defined() || !dk.defined() || (dq.size(0) == dk.size(0) && dq.size(1) == dk.size(1) && dq.size(3) == dk.size(3)), "the gradients must have the shapes of q and k");
+      TORCH_CHECK_VALUE(as_saved(saved[0], first.device(), {at::kInt, at::kLong}, saved[0].dim() == 1 ? first.size(1) : first.size(0) * first.size(1)) && saved[1].dim() == 1 &&
+                            as_saved(saved[1], first.device(), {at::kDouble}, saved[1].size(0)) && saved[1].is_contiguous(),
+                        "the saved tensors must be as they were");
       out = turn(first, dq.defined() && dk.defined() ? &dk : nullptr, saved[0], saved[1], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["magnitude"].toDouble(), true);
       TORCH_CHECK(out.first.defined(), "lego_hip_rotary refuses the gradients");
       if (!dq.defined()) std::swap(out.first, out.second);
     }
-    return {out.first, out.second, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    variable_list all = {out.first, out.second, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    once(all, "rotary", {dq, dk});
+    return all;
   }
 };
 

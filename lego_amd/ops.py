@@ -610,6 +610,23 @@ def attention_bwd(dout, q, k, v, out, lse, causal=False, scale=None, softcap=0.0
     return dq, dk, dv
 
 
+class _Once(torch.autograd.Function):
+    """Gradients whose own gradient may be asked for: it is an error and not zero by what they came from."""
+
+    @staticmethod
+    def forward(ctx, name, count, *tensors):
+        ctx.name = name
+        return tuple(t.view_as(t) for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} has no second derivative")
+
+
+def _once(name, grads, *sources):
+    return _Once.apply(name, len(grads), *grads, *sources) if torch.is_grad_enabled() else grads
+
+
 class LEGOAttention(torch.autograd.Function):
     """The node of ``attention``."""
 
@@ -621,10 +638,11 @@ class LEGOAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, slopes, documents, prefix, rest = ctx.saved_tensors
-        return attention_bwd(dout, q, k, v, out, lse, *ctx.how, slopes, documents, prefix, rest) + (None,) * 6
+        with torch.no_grad():
+            grads = attention_bwd(dout, q, k, v, out, lse, *ctx.how, slopes, documents, prefix, rest)
+        return _once("attention", grads, q, k, v, dout) + (None,) * 6
 
 
 def attention(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, documents=None, prefix=None):
@@ -773,14 +791,15 @@ class LEGORotary(torch.autograd.Function):
         return tuple(_rotary(q, k, positions, frequencies, interleaved, magnitude, 0))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, frequencies = ctx.saved_tensors
-        if dq is None or dk is None:
-            one = dk if dq is None else dq
-            got = None if one is None else _rotary(one, None, positions, frequencies, *ctx.how, 1)[0]
-            return (None, got, None, None, None, None) if dq is None else (got, None, None, None, None, None)
-        return (*_rotary(dq, dk, positions, frequencies, *ctx.how, 1), None, None, None, None)
+        given = [t for t in (dq, dk) if t is not None]
+        if not given:
+            return (None,) * 6
+        with torch.no_grad():
+            got = _rotary(given[0], given[1] if len(given) == 2 else None, positions, frequencies, *ctx.how, 1)
+        got = iter(_once("rotary", tuple(got[:len(given)]), *given))
+        return (*(None if t is None else next(got) for t in (dq, dk)), None, None, None, None)
 
 
 def rotary(q, k, positions, frequencies, interleaved=False, magnitude=1.0):

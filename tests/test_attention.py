@@ -283,6 +283,39 @@ def test_autograd_gradients_and_repeats():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("node", ["call", "python"])
+def test_no_second_derivative(node):
+    """What would need one raises, and is no gradient with a part missing."""
+    q, k, v, _ = make(1, 20, 20, 2, 2, 64, torch.bfloat16)
+    q.requires_grad_()
+    attend = (lambda: ops.attention(q, k, v, causal=True)) if node == "call" else (lambda: ops.LEGOAttention.apply(q, k, v, True, None, 0.0, None, None, None))
+    out = attend()
+    (dq,) = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)
+    (plain,) = torch.autograd.grad(attend().float().square().sum(), q)
+    assert torch.equal(dq.detach(), plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.float().square().sum() + out.float().sum(), q)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_that_come_back_as_others():
+    """A hook that hands back what was not saved is an error before anything is launched; one that keeps them on the host is not."""
+    q, k, v, dout = make(1, 20, 20, 2, 2, 64, torch.bfloat16, layout="fused")
+    q = q.detach().requires_grad_()
+    documents = torch.zeros(1, 20, dtype=torch.int32, device="cuda")
+    how = dict(causal=True, slopes=torch.tensor([0.1, 0.2], device="cuda"), documents=documents)
+    (want,) = torch.autograd.grad(ops.attention(q, k, v, **how), q, dout)
+    with torch.autograd.graph.save_on_cpu():
+        out = ops.attention(q, k, v, **how)
+    assert torch.equal(torch.autograd.grad(out, q, dout)[0], want)
+    for other in (lambda t: t.cpu(), lambda t: t[:, :10] if t.dim() > 1 else t[:1], lambda t: t.long() if t.dtype == torch.int32 else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+            out = ops.attention(q, k, v, **how)
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.autograd.grad(out, q, dout)
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """A step along a random direction changes sum(out * dout) by the gradient's part in it.  fp32 sums of fp16 outputs: an output's rounding, 2^-11 relative, adds up like
     noise over the outputs, which a step of 2^-5 of values near one, over three directions, stands well above."""

@@ -164,6 +164,23 @@ def test_refusals_of_the_entry_point():
 
 
 @pytest.mark.gpu
+def test_second_derivatives_and_saved_tensors():
+    """What would need the gradient's own gradient raises; saved tensors that come back as others are an error before anything is launched."""
+    q, k = (torch.randn(2, 9, h, 16, device="cuda", dtype=torch.float32).requires_grad_() for h in (4, 2))
+    at, f = torch.arange(9, device="cuda"), ops.rotary_frequencies(16)
+    turned = ops.rotary(q, k, at, f)
+    dq, dk = torch.autograd.grad(turned[0].square().sum() + turned[1].square().sum(), (q, k), create_graph=True)
+    assert torch.allclose(dq, 2 * q, atol=1e-4) and torch.allclose(dk, 2 * k, atol=1e-4)      # lengths stay: 32-bit roundings of numbers below 8
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.square().sum() + turned[0].sum(), q)
+    for other in (lambda t: t.cpu(), lambda t: t[:5], lambda t: t.float()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+            turned = ops.rotary(q, k, at, f)
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.autograd.grad(turned[0].sum() + turned[1].sum(), (q, k))
+
+
+@pytest.mark.gpu
 def test_refusals():
     q, k = torch.randn(2, 6, 4, 64, device="cuda"), torch.randn(2, 6, 2, 64, device="cuda")
     p, f = torch.arange(6, device="cuda"), ops.rotary_frequencies(64)
