@@ -132,7 +132,6 @@ __device__ __forceinline__ void fill_words(const void* base, unsigned rows, unsi
 // The scheduler's next instructions of a kind: it would read an operand from LDS only when the one before is used, and wait for each.
 #define LEGO_MFMAS(N) __builtin_amdgcn_sched_group_barrier(0x008, N, 0)
 #define LEGO_READS(N) __builtin_amdgcn_sched_group_barrier(0x100, N, 0)
-#define LEGO_ARITHMETIC(N) __builtin_amdgcn_sched_group_barrier(0x402, N, 0)
 
 __device__ __forceinline__ void wait_for_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 

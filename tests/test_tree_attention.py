@@ -126,6 +126,37 @@ def test_scores(how, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("drafts", [3, 13, 40])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_scores_of_all_numbers_of_rows(dim, drafts, dtype):
+    """12, 52 and 160 rows a key head."""
+    x = make([300, 40, 1111, 0, 77], drafts, 8, 2, dim, 16, dtype, seed=4)
+    slopes = torch.tensor([2.0 ** -i for i in range(8)], device="cuda")
+    positions = x["lengths"][:, None] + torch.arange(drafts, dtype=torch.int32, device="cuda") // 2
+    check(**x, softcap=6.0)
+    check(**x, slopes=slopes, positions=positions)
+    check(**x, softcap=6.0, scale=-0.3, slopes=slopes, positions=positions)
+    check(**x, scale=-0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafts", [1, 5, 20, 40])
+def test_tables_longer_than_a_piece(drafts):
+    """Pages of 1 to 3 rows: the kernels hold 256 or 1024 entries of a table at a time."""
+    for rows, lengths in ((1, [2500, 3, 1100]), (2, [4200]), (3, [3, 3500])):
+        check(**make(lengths, drafts, 8, 2, 64, rows, torch.bfloat16, seed=rows))
+
+
+@pytest.mark.gpu
+def test_many_sequences_side_by_side():
+    """More than 64 of them, in runs that begin and end anywhere, with blocks of rows side by side."""
+    lengths = [(37 * i) % 501 for i in range(130)]
+    check(**make(lengths, 2, 4, 2, 64, 16, torch.bfloat16, seed=8))
+    check(**make(lengths[:70], 70, 4, 2, 64, 16, torch.float16, seed=9))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lengths", [[0, 200, 64, 1], [0]])
 def test_over_the_cache_alone(lengths):
     how = make(lengths, 3, 4, 2, 64, 16, torch.bfloat16, trees=False) | dict(k=None, v=None)
