@@ -2,8 +2,8 @@
 //
 // Rotary positions: pairs (a, b) of the first `part` elements of a head become magnitude * (a cos t - b sin t, b cos t + a sin t) with
 // t = position * frequency, the other elements are copied; with -t it is the gradient.  Queries and keys in one launch.
-// Bound by memory: every element is read and written once.  A workgroup takes 1 tokens with all their heads, so that a token's angles are computed once,
-// into LDS: the product in 64 bits and reduced to a part of a turn there (a position of a million has lost all its digits in a 32-bit angle), sine and cosine
+// Bound by memory: every element is read and written once, 16384 tokens of 40 bf16 heads of 128 in 60 us, 5.6 TB/s of reads and writes.  A workgroup takes 1 token with all its heads (four of
+// them are 5 % faster on inputs from the caches and 9 % slower on inputs from memory), so that a token's angles are computed once, into LDS: the product in 64 bits and reduced to a part of a turn there (a position of a million has lost all its digits in a 32-bit angle), sine and cosine
 // of what remains in 32.  A lane then turns one 16-byte vector at a time, or two where a pair's elements lie half the part apart.
 // Index expressions printed from LEGO layouts:
 //   unit of a token's heads   OrderBy(Row(1, heads, units)).TileBy([1, heads, units]).inv(u)
