@@ -5,6 +5,9 @@
 // lane of each half: the scores are computed transposed, S^T = K Q^T, so that a query's scores lie in two lanes, its maximum and sum cost one exchange between
 // the halves, and its factors are a lane's own.  P^T is the second operand of O^T = V^T P^T as it lies in the registers.  Tiles of 64 keys go from memory into LDS
 // without passing registers, the next one while the present one is computed.
+// Bound by the matrix cores and, level with them, by the vector unit, which has an exponential and five more instructions a score to issue and with a cap another exponential and a reciprocal: 2 x 32
+// bf16 heads of 128, 8192 tokens, causal with prefixes, in 1.25 ms, 1.0 PFLOP/s of what is seen, both pipes 58 % busy; with a cap and 2 x 16 heads of 4096, 0.20 ms, 680 TFLOP/s, MFMA 32 %, vector 62 %.
+// Wavefronts of 32 queries: LDS then delivers as many operands as the matrix cores take.  Two wavefronts a SIMD, one's softmax beside the other's products.
 // P is rounded to the operands' type for the product with V, as is everything that MFMAs of 16-bit operands take; its sum is of the unrounded values, in fp32.
 // Index expressions printed from LEGO layouts:
 //   LDS tile   OrderBy(GenP((64, 8), row*8 + (chunk ^ key(row)))).TileBy([64, 8])

@@ -382,6 +382,7 @@ __device__ __forceinline__ void copy_row(const void* base, unsigned at, unsigned
 
 // Up to 32 rows: a workgroup's tiles of an item are shared out among its wavefronts, and each goes through its own by itself, with no other one to wait for, in tiles of 32 keys; eight of them and more
 // on a CU keep the memory busy.  The keys of the next tile come while the products with the present values are formed, its values while those with the keys are.  The sums meet in LDS at the end.
+// A step of 32 sequences of 37 to 8192 tokens, 32 bf16 heads of 128 to 8 (537 MB of keys and values): 107 us, 5.0 TB/s, and 7 us for the join; with wavefronts that share tiles behind barriers 135 us.
 template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_f16_d128_kernel(TreeArgs a)
 {
@@ -620,6 +621,9 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_few_f16_d128_kernel(Tree
 }
 
 // More rows: wavefronts of 32 rows share tiles of 64 keys, two pairs of them or four.
+// 8 sequences of 1021 to 16384 tokens, trees of 48 drafts, 32 bf16 heads of 128 to 8, capped (285 MB of keys and values, 55 GFLOP): 167 us and 19 for the join, MFMA 22 % busy, vector unit 53 %.  The
+// forward kernel takes nearly as long for dense tensors that come from memory as these do (32 x 256 rows of 8 heads, 8192 keys: 470 us, and 546 here).  Two blocks of 128 rows for 192: three of 64, which
+// waste none, take 240 us, as they have each tile of keys brought to LDS for half as many rows.
 template <bool CAP, bool BIAS, unsigned RW>
 __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_f16_d128_kernel(TreeArgs a)
 {
@@ -904,7 +908,7 @@ __global__ void __launch_bounds__(64 * NW, 2) lego_tree_many_f16_d128_kernel(Tre
   } while (true);
 }
 
-// The rows of items in several runs, and of those that have no tile, `share` rows of an item a workgroup: a few parts are gone through by the lanes of each row, many by teams of lanes, a row
+// The rows of items in several runs, and of those that have no tile, `share` rows of an item a workgroup: a few parts of several rows are gone through by the lanes of each row, others by teams of lanes, a row
 // after the other.  Either order is the same whenever the lengths are.
 __global__ void __launch_bounds__(256) lego_tree_join_f16_d128_kernel(TreeArgs a, unsigned held_rows, unsigned share, unsigned chunks)
 {
@@ -933,7 +937,7 @@ __global__ void __launch_bounds__(256) lego_tree_join_f16_d128_kernel(TreeArgs a
     sum += f * stat.y;
     if (4 * c < DC) x += f * *reinterpret_cast<const float4v*>(a.sums + place * DC + 4 * c);
   };
-  if (parts <= 8) {
+  if (share > 1 && parts <= 8) {
     for (unsigned i = begin + team; i < end; i += TEAMS) {
       float most = -INFINITY, sum = 0.0f;
       float4v x = {0.0f, 0.0f, 0.0f, 0.0f};

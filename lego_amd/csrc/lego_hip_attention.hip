@@ -154,9 +154,12 @@ inline bool plan_of(TreeArgs& a, const long long* sizes, TreePlan& plan)
   const unsigned long long items = (unsigned long long)a.batch * a.key_heads;
   const unsigned long long most = ((unsigned long long)a.page * a.width + a.tile - 1) / a.tile + ((unsigned)a.drafts + a.tile - 1) / a.tile;
   if (items * most >= (1ull << 31)) return false;
-  // An item of few tiles is one workgroup's; else the tiles are dealt in equal runs to as many workgroups as the chip holds at a time, but no run is shorter than a tile or two a wavefront.
+  // An item of few tiles is one workgroup's, and there is nothing to join; of more, where there are enough items.  Else the tiles are dealt in equal runs to as many workgroups as the chip holds at a time,
+  // but no run is shorter than a tile or two a wavefront.  One launch / runs and join, fp16 heads of 64, four to a key head, us: one token, 4 items of 1000 keys 12.2 / 13.2, of 1500 15.4 / 10.7, 256 items
+  // of 2000 keys 26 / 36; 24 drafts, 4 items of 375 16.3 / 17.2, of 500 19.1 / 17.2, 64 of 750 25 / 27, of 1000 31 / 29, 256 of 2000 58 / 62.
   a.least = plan.row_waves == 1 ? 2 * LEGO_TREE_LEAST : LEGO_TREE_LEAST;
-  a.whole = most <= (plan.row_waves == 1 ? 16 : 4);
+  const unsigned long long blocks = items * a.row_blocks;
+  a.whole = most <= (plan.row_waves == 1 ? (blocks >= 256 ? 65 : 33) : blocks >= 256 ? 33 : blocks >= 64 ? 13 : 7);
   const unsigned long long chip = plan.row_waves == 1 && a.head <= 64 ? 768 : 512, held = chip > a.row_blocks ? chip / a.row_blocks : 1, runs = (items * most + a.least - 1) / a.least;
   a.runs = (unsigned)(runs < held ? runs : held);
   quotients_by((unsigned)a.page, a.page_factor, a.page_shift);

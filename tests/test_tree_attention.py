@@ -154,6 +154,9 @@ def test_many_sequences_side_by_side():
     lengths = [(37 * i) % 501 for i in range(130)]
     check(**make(lengths, 2, 4, 2, 64, 16, torch.bfloat16, seed=8))
     check(**make(lengths[:70], 70, 4, 2, 64, 16, torch.float16, seed=9))
+    lengths = [(677 * i) % 2901 for i in range(70)]
+    check(**make(lengths, 2, 4, 2, 64, 16, torch.bfloat16, seed=10))
+    check(**make(lengths[:20], 20, 4, 1, 128, 32, torch.bfloat16, seed=11))
 
 
 @pytest.mark.gpu
@@ -337,7 +340,7 @@ def test_refusals_of_the_entry_points():
     lib = runtime.load_library()
     longs = lambda *v: (ctypes.c_longlong * len(v))(*v)      # noqa: E731
     need = ctypes.c_ulonglong(0)
-    good = (2, 3, 4, 2, 64, 16, 100, 50)
+    good = (2, 3, 4, 2, 64, 16, 100, 200)
     assert lib.lego_hip_tree_attention_workspace_bytes(longs(*good), ctypes.byref(need)) == 0 and need.value > 0
     assert lib.lego_hip_tree_attention_workspace_bytes(longs(2, 3, 4, 2, 64, 16, 100, 8), ctypes.byref(need)) == 0 and need.value == 0
     bads = [tuple(0 if j == i else x for j, x in enumerate(good)) for i in range(8)] + [(2, 3, 4, 3, 64, 16, 100, 50), (2, 3, 4, 2, 60, 16, 100, 50), (2, 3, 4, 2, 136, 16, 100, 50),
