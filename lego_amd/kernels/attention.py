@@ -111,4 +111,4 @@ def emit():
         banner=BANNER, stat=stat, ORDERED=ORDERED, ORDER_FIGURES="forward 98 -> 84 us, dk and dv 191 -> 167, dq 146 -> 129 at 6 a launch", PSHIFT=PSHIFT["f16"], stat_layout="OrderBy(Row(batch, heads, queries)).TileBy([batch, heads, queries])[b, h, i]",
         parts_layout="OrderBy(Row(parts, 2, batch, key heads, keys, head))"),
         ["lego_attention_tiles_launch", "lego_attention_order_launch", "lego_attention_delta_launch", "lego_attention_join_launch"]))
-    return units, dict(HEADS=HEADS, ORDERED=ORDERED, TREE_LEAST=TREE_LEAST, JOIN_ROWS=JOIN_ROWS, JOIN_MANY=JOIN_MANY, JOIN_FEW=JOIN_FEW, MAX_HEAD=MAX_HEAD, ELEMENTS=tuple(ELEMENTS))
+    return units, dict(HEADS=HEADS, ORDERED=ORDERED, TREE_LEAST=TREE_LEAST, MAX_HEAD=MAX_HEAD, ELEMENTS=tuple(ELEMENTS))

@@ -656,7 +656,7 @@ def attention(q, k, v, causal=False, scale=None, softcap=0.0, slopes=None, docum
     number is padding, which sees and is seen by nothing, whatever it holds).  A query that sees nothing gives zeros, and takes and gives no gradient.
     A NaN or infinity in a key or value reaches the queries that see it, and may reach others within 64 positions of those.
 
-    Inside a captured graph call ``attention_fwd`` and ``attention_bwd``: autograd's own bookkeeping of leaves is not made for it."""
+    There is no second derivative: asking for one raises.  Inside a captured graph call ``attention_fwd`` and ``attention_bwd``: autograd's own bookkeeping of leaves is not made for it."""
     out = _host().attention(q, k, v, causal, scale, softcap, slopes, documents, prefix)
     if out is not None:
         return out
@@ -807,7 +807,7 @@ def rotary(q, k, positions, frequencies, interleaved=False, magnitude=1.0):
 
     q and k are ``[batch, token, head, element]``, positions (int32 or int64) ``[batch, token]`` or ``[token]``.  The first ``part = 2 * len(frequencies)`` elements
     of a head are turned: pair i by ``positions * frequencies[i]`` radians (float64, as ``rotary_frequencies`` makes them) and times ``magnitude``; pair i is elements
-    ``(i, i + part/2)``, or ``(2i, 2i + 1)`` where ``interleaved``.  The others stay."""
+    ``(i, i + part/2)``, or ``(2i, 2i + 1)`` where ``interleaved``.  The others stay.  There is no second derivative: asking for one raises."""
     out = _host().rotary(q, k, positions, frequencies, interleaved, magnitude)
     if out is not None:
         return out
